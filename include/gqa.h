@@ -208,6 +208,31 @@ int gqa_create_paged_layers(const gqa_config* cfg, int32_t page_size, int32_t n_
                             gqa_ctx** out_ctx);
 int gqa_paged_layers(gqa_ctx* ctx, int32_t* n_layers, int32_t* layer);
 
+/* ---- E4M3 K/V cache -----------------------------------------------------------
+ * No reference counterpart (the board's cache holds bf16 words).  gqa_create_kv8 is gqa_create (page_size 0, n_pages 0,
+ * n_layers 1) or gqa_create_paged_layers (page_size >= 64) with a cache of one byte per value and one scale byte per row:
+ * half the bytes, so about half a decode step's time.  A row is the D values of a token of a kv head, K and V apart;
+ * its value is code * 2^(byte - 127), the code an E4M3 number (8 bits, OCP) and byte the least one with
+ * 448 * 2^(byte - 127) >= the row's largest finite |x| (1 at the least).  Each value is rounded once, to nearest even:
+ * by at most 2^-4 of itself, or 2^-10 * 2^(byte - 127) below 2^-6 * 2^(byte - 127); infinities and NaN become NaN, and
+ * finite values beyond 1.875 * 2^127 that value.  Codes and scale bytes of a new context are zero.
+ * Every entry point works as on a bf16 context, with bf16 rows crossing the boundary: the rows given to gqa_load_kv,
+ * gqa_append_kv, gqa_decode_append, gqa_prefill_append and the layer stage are quantised as they are written (in the
+ * same launch for the decode step), attention sees the stored values (those of rows appended by the call too), and
+ * gqa_read_kv returns them as bf16, which holds them exactly.  Device operands are 16-byte aligned, in
+ * gqa_load_kv_device and gqa_append_kv_device too.  Differences:
+ *   - decode takes every group of 1 .. 16 query heads per kv head; prefill the bf16 kernels' groups.  Decode's error
+ *     against exact attention over the stored values is as of the bf16 cache.
+ *   - prefill (and transactions) read the attended rows back into a bf16 workspace first, which grows to the longest
+ *     kv_len seen (a call that grows it synchronises the device), and the layer stage passes through it: uses of it on
+ *     several streams follow each other, and these calls return GQA_ERR_UNSUPPORTED under a stream capture.  Decode,
+ *     append, load, read and the heads' entry points below need no workspace.
+ *   - KV260 numerics and gqa_decode_append_noalloc are for bf16 caches.
+ * gqa_cache_pointers returns the codes' pools; gqa_kv8_scales the active layer's scale bytes ([B][H_kv][L_cap], paged
+ * [n_pages][H_kv][page_size]; GQA_ERR_UNSUPPORTED on a bf16 context). */
+int gqa_create_kv8(const gqa_config* cfg, int32_t page_size, int32_t n_pages, int32_t n_layers, gqa_ctx** out_ctx);
+int gqa_kv8_scales(gqa_ctx* ctx, void** k_scale, void** v_scale);
+
 /* ---- K/V cache --------------------------------------------------------------
  * gqa_load_kv replaces the KV branch of _service_request + _transfer(DEST_K_CACHE /
  * DEST_V_CACHE) (attn_driver.py:378-422) and the cache write of kv_cache_ram.sv:77-83:
@@ -302,6 +327,9 @@ int gqa_prefill_append_device(gqa_ctx* ctx, int32_t b, const void* q, const void
 /* gqa_load_kv_device: gqa_load_kv from device memory (k, v are [H_kv][n][D] in HBM). */
 int gqa_load_kv_device(gqa_ctx* ctx, int32_t b, int32_t start_pos, int32_t n,
                        const void* k, const void* v, void* stream);
+/* gqa_read_kv_device: gqa_read_kv into device memory (k, v are [H_kv][n][D] bf16 in HBM, 16-byte aligned), from a bf16 or
+ * an E4M3 cache. */
+int gqa_read_kv_device(gqa_ctx* ctx, int32_t b, int32_t start_pos, int32_t n, void* k, void* v, void* stream);
 /* Device addresses of the K and V caches ([B][H_kv][L_cap][D] bf16) and L_cap. */
 int gqa_cache_pointers(gqa_ctx* ctx, void** k_cache, void** v_cache, int32_t* l_cap);
 
@@ -367,6 +395,50 @@ int gqa_layer_qkv_device(gqa_ctx* ctx, int32_t b, const void* x, int32_t n_token
                          float rms_eps, int32_t q_pos_base, int32_t kv_pos_base, int32_t kv_row0,
                          int32_t rope, void* q_out, void* stream);
 int gqa_layer_times(gqa_ctx* ctx, float* out_us, int32_t n);
+
+/* ---- heads: norms, RoPE and scatter ---------------------------------------------------
+ * No reference counterpart (the board's layer has no per-head norms).  For callers that project by themselves (or with
+ * gqa_w4_project_device): qkv is [n_tokens][ld] bf16 in device memory, a row the Q heads, the K heads and the V heads of a
+ * token, D columns each (ld >= (H_q + 2 H_kv) * D, a multiple of 8).  Each Q head is normalised with q_weight and each K
+ * head with k_weight ([D] bf16; NULL: that side is not), y = h / sqrt(mean(h^2) + eps) * w over the head's D values, then
+ * the pair (2p, 2p + 1) of each Q and K head is rotated by position * rope_base^(-2p/D) (rope_base 0: no rotation, else
+ * > 1), then Q goes to q_out and K and V into the cache, bf16 or E4M3.  fp32 up to one rounding, angles in 64 bits (the
+ * layer stage rounds the angle to fp32 as the board does: its rotations differ from these by up to 2^-24 of the angle).
+ * gqa_qk_norm_rope_device: the tokens of sequence b; Q at positions q_pos_base .., K at kv_pos_base .., cache rows
+ * kv_row0 ..; q_out is [H_q][n_tokens][D].
+ * gqa_qk_norm_rope_step_device: one token of each sequence (n_tokens = batch): positions [B] and rows [B] in device
+ * memory, rows NULL for rows = positions; q_out is [B][H_q][D].  A sequence with a negative position, or a row outside
+ * 0 .. max_seq_len - 1, is left out: neither its Q nor its cache is written.  Positions of sequences that are not left
+ * out stay below 2^30.
+ * qkv must not overlap q_out or the cache, and all operands are 16-byte aligned (else GQA_ERR_RANGE). */
+int gqa_qk_norm_rope_device(gqa_ctx* ctx, int32_t b, const void* qkv, int64_t ld, int32_t n_tokens, const void* q_weight,
+                            const void* k_weight, float eps, int32_t q_pos_base, int32_t kv_pos_base, int32_t kv_row0,
+                            double rope_base, void* q_out, void* stream);
+int gqa_qk_norm_rope_step_device(gqa_ctx* ctx, const void* qkv, int64_t ld, const void* q_weight, const void* k_weight,
+                                 float eps, const int32_t* positions, const int32_t* rows, double rope_base, void* q_out,
+                                 void* stream);
+
+/* ---- 4-bit weights -----------------------------------------------------------------------
+ * No reference counterpart.  The projection of a few tokens is the stream of its weights; 4-bit ones are a quarter of
+ * it.  A matrix [rows][hidden] has codes c of 0 .. 15 and one bf16 scale s per row and group of `group` columns (32, 64 or
+ * 128, dividing hidden; other groups: GQA_ERR_UNSUPPORTED): w = (c - 8) * s.  rows up to 2^20, hidden up to 2^16.
+ * gqa_w4_pack_device lays codes [rows][hidden / 2] (a byte: the even column in its low four bits) and scales
+ * [rows][hidden / group] out for the products, once; gqa_w4_bytes gives the sizes of the two results.
+ * gqa_w4_project_device: y [n_tokens][ldy] bf16 (the first `rows` of each row) = norm(x) W^T for x [n_tokens][hidden] bf16,
+ * norm(x) = x / sqrt(mean(x^2) + rms_eps) * rms_weight, or x with rms_weight NULL.  x * rms_weight is rounded to bf16,
+ * sums are fp32.  n_tokens up to GQA_W4_MAX_TOKENS; a token's result does not depend on the others of the call.
+ * gqa_w4_unpack_device: the packed matrix as bf16 [rows][hidden], for long prompts (gqa_layer_qkv_device).
+ * The context gives device and stream.  Operands are 16-byte aligned (codes any, scales and y 2-byte) and outputs must
+ * not overlap inputs, else GQA_ERR_RANGE.  None of these calls allocates or synchronises. */
+#define GQA_W4_MAX_TOKENS (1 << 16)
+int gqa_w4_bytes(int32_t rows, int32_t hidden, int32_t group, int64_t* w_bytes, int64_t* scale_bytes);
+int gqa_w4_pack_device(gqa_ctx* ctx, const void* codes, const void* scales, int32_t rows, int32_t hidden, int32_t group,
+                       void* w, void* w_scales, void* stream);
+int gqa_w4_unpack_device(gqa_ctx* ctx, const void* w, const void* w_scales, int32_t rows, int32_t hidden, int32_t group,
+                         void* out, void* stream);
+int gqa_w4_project_device(gqa_ctx* ctx, const void* x, int32_t n_tokens, int32_t hidden, const void* w,
+                          const void* w_scales, int32_t group, int32_t rows, const void* rms_weight, float rms_eps, void* y,
+                          int64_t ldy, void* stream);
 
 /* ---- prepared decode steps ---------------------------------------------------------
  * No reference counterpart (the board's transaction is driven by CSR writes).  For serving loops

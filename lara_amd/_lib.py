@@ -56,6 +56,7 @@ GQA_DECODE_MERGE_FUSED = 2
 GQA_OPT_PREFILL_KERNEL = 6
 GQA_OPT_LAYER = 7
 GQA_MAX_LAYERS = 1024
+GQA_W4_MAX_TOKENS = 1 << 16
 GQA_PREFILL_KERNEL_AUTO = 0
 GQA_PREFILL_KERNEL_SHARED = 1
 GQA_PREFILL_KERNEL_ROWS = 2
@@ -96,6 +97,8 @@ _SIGNATURES = {
     "gqa_create_paged": [POINTER(GqaConfig), c_int32, c_int32, POINTER(c_void_p)],
     "gqa_create_paged_layers": [POINTER(GqaConfig), c_int32, c_int32, c_int32, POINTER(c_void_p)],
     "gqa_paged_layers": [_CTX, _P32, _P32],
+    "gqa_create_kv8": [POINTER(GqaConfig), c_int32, c_int32, c_int32, POINTER(c_void_p)],
+    "gqa_kv8_scales": [_CTX, POINTER(c_void_p), POINTER(c_void_p)],
     "gqa_destroy": [_CTX],
     "gqa_get_config": [_CTX, POINTER(GqaConfig)],
     "gqa_set_option": [_CTX, c_int32, c_int64],
@@ -115,6 +118,7 @@ _SIGNATURES = {
     "gqa_read_output": [_CTX, _P16, c_int64],
     "gqa_read_perf": [_CTX, POINTER(c_uint64), POINTER(c_uint64), POINTER(c_uint64), POINTER(c_double)],
     "gqa_load_kv_device": [_CTX, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p],
+    "gqa_read_kv_device": [_CTX, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p],
     "gqa_append_kv_device": [_CTX, c_void_p, c_void_p, c_void_p, c_void_p],
     "gqa_decode_device": [_CTX, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
     "gqa_decode_append_device": [_CTX, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
@@ -135,6 +139,15 @@ _SIGNATURES = {
                          c_int32, c_int32],
     "gqa_layer_qkv_device": [_CTX, c_int32, c_void_p, c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_void_p,
                              c_float, c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p],
+    "gqa_qk_norm_rope_device": [_CTX, c_int32, c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_float, c_int32, c_int32,
+                                c_int32, c_double, c_void_p, c_void_p],
+    "gqa_qk_norm_rope_step_device": [_CTX, c_void_p, c_int64, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_double,
+                                     c_void_p, c_void_p],
+    "gqa_w4_bytes": [c_int32, c_int32, c_int32, POINTER(c_int64), POINTER(c_int64)],
+    "gqa_w4_pack_device": [_CTX, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p],
+    "gqa_w4_unpack_device": [_CTX, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p, c_void_p],
+    "gqa_w4_project_device": [_CTX, c_void_p, c_int32, c_int32, c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_float,
+                              c_void_p, c_int64, c_void_p],
     "gqa_layer_times": [_CTX, _PF, c_int32],
     "gqa_graph_capture_decode_append": [_CTX, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                         POINTER(c_void_p)],

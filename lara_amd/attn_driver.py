@@ -286,7 +286,9 @@ class AttentionAccelerator:
     ``bitstream_path`` and ``overlay`` are accepted for compatibility; a bitstream path is
     only hashed into the run profile.  The keyword-only arguments size the engine; the
     defaults reproduce the board contract (32 Q / 8 KV heads, D = 128, L <= 512, one
-    sequence).
+    sequence).  ``kv_format="e4m3"`` keeps the K/V cache in 8 bits (rows quantised as they are
+    written, one power-of-two scale per row of a kv head; ``read_kv`` returns the stored values);
+    "exact" numerics only.
     """
 
     def __init__(
@@ -307,6 +309,7 @@ class AttentionAccelerator:
         page_size: int | None = None,
         n_pages: int | None = None,
         n_layers: int | None = None,
+        kv_format: str = "bf16",
     ) -> None:
         self._closed = True
         self._ctx = ctypes.c_void_p()
@@ -331,9 +334,17 @@ class AttentionAccelerator:
         if n_layers is not None and not self.paged:
             raise ValueError("a multi-layer cache is paged: give page_size with n_layers")
         self.n_layers = int(n_layers) if n_layers is not None else 1
-        if self.paged:
-            if n_pages is None:
-                n_pages = self.batch * -(-self.max_seq_len // int(page_size))
+        if kv_format not in ("bf16", "e4m3"):
+            raise ValueError(f"kv_format must be 'bf16' or 'e4m3', got {kv_format!r}")
+        self.kv_format = kv_format
+        if self.paged and n_pages is None:
+            n_pages = self.batch * -(-self.max_seq_len // int(page_size))
+        if kv_format == "e4m3":
+            if self.paged and int(page_size) == 0:
+                raise ValueError("page_size must be a power of two >= 64")
+            rc = lib.gqa_create_kv8(ctypes.byref(cfg), int(page_size or 0), int(n_pages) if self.paged else 0, self.n_layers,
+                                    ctypes.byref(self._ctx))
+        elif self.paged:
             if n_layers is not None:
                 rc = lib.gqa_create_paged_layers(ctypes.byref(cfg), int(page_size), int(n_pages), self.n_layers,
                                                  ctypes.byref(self._ctx))
@@ -666,6 +677,12 @@ class AttentionAccelerator:
         self._call("gqa_read_kv", int(b), int(start_pos), int(n), _lib.as_u16_ptr(k), _lib.as_u16_ptr(v))
         return k, v
 
+    def read_kv_device(self, b: int, start_pos: int, n: int, k_ptr: int, v_ptr: int, *, stream: int | None = None) -> None:
+        """Rows start_pos.. of sequence ``b`` into device memory as bf16 [H_kv, n, D] (``gqa_read_kv_device``); enqueued,
+        not synchronised."""
+        self._call("gqa_read_kv_device", int(b), int(start_pos), int(n), ctypes.c_void_p(k_ptr), ctypes.c_void_p(v_ptr),
+                   ctypes.c_void_p(stream) if stream else None)
+
     # ---- attention ----------------------------------------------------------------------------
     def decode_step(self, q: np.ndarray, ctx_lens, *, k_rows: np.ndarray | None = None,
                     v_rows: np.ndarray | None = None, positions=None, return_lse: bool = False):
@@ -982,6 +999,52 @@ class AttentionAccelerator:
                    ctypes.c_void_p(rms_weight_ptr) if rms_weight_ptr else None, float(rms_eps), int(q_pos_base),
                    int(kv_pos_base), int(kv_row0), int(bool(rope)), ctypes.c_void_p(q_out_ptr),
                    ctypes.c_void_p(stream) if stream else None)
+
+    def qk_norm_rope_device(self, qkv_ptr: int, ld: int, n_tokens: int, q_weight_ptr: int | None, k_weight_ptr: int | None,
+                            q_out_ptr: int, *, b: int = 0, q_pos_base: int = 0, kv_pos_base: int = 0, kv_row0: int = 0,
+                            eps: float = RMS_NORM_EPS, rope_base: float = 10000.0, stream: int | None = None) -> None:
+        """Per-head norms of Q and K, RoPE and scatter of sequence ``b``'s projected rows [n_tokens, ld] (device pointers;
+        ``gqa_qk_norm_rope_device``): Q to ``q_out_ptr`` [H_q, n_tokens, D], K/V into rows kv_row0..; a weight of None
+        leaves that side unnormalised, ``rope_base`` 0 unrotated.  Enqueued, not synchronised."""
+        self._call("gqa_qk_norm_rope_device", int(b), ctypes.c_void_p(qkv_ptr), int(ld), int(n_tokens),
+                   ctypes.c_void_p(q_weight_ptr) if q_weight_ptr else None,
+                   ctypes.c_void_p(k_weight_ptr) if k_weight_ptr else None, float(eps), int(q_pos_base), int(kv_pos_base),
+                   int(kv_row0), float(rope_base), ctypes.c_void_p(q_out_ptr), ctypes.c_void_p(stream) if stream else None)
+
+    def qk_norm_rope_step_device(self, qkv_ptr: int, ld: int, q_weight_ptr: int | None, k_weight_ptr: int | None,
+                                 positions_ptr: int, q_out_ptr: int, *, rows_ptr: int | None = None,
+                                 eps: float = RMS_NORM_EPS, rope_base: float = 10000.0, stream: int | None = None) -> None:
+        """The same for one token of every sequence ([batch, ld]): int32 ``positions`` (-1: left out) and cache ``rows``
+        (None: the positions) in device memory, Q to [batch, H_q, D] (``gqa_qk_norm_rope_step_device``)."""
+        self._call("gqa_qk_norm_rope_step_device", ctypes.c_void_p(qkv_ptr), int(ld),
+                   ctypes.c_void_p(q_weight_ptr) if q_weight_ptr else None,
+                   ctypes.c_void_p(k_weight_ptr) if k_weight_ptr else None, float(eps), ctypes.c_void_p(positions_ptr),
+                   ctypes.c_void_p(rows_ptr) if rows_ptr else None, float(rope_base), ctypes.c_void_p(q_out_ptr),
+                   ctypes.c_void_p(stream) if stream else None)
+
+    def w4_pack_device(self, codes_ptr: int, scales_ptr: int, rows: int, hidden: int, group: int, w_ptr: int,
+                       w_scales_ptr: int, *, stream: int | None = None) -> None:
+        """Lays a 4-bit matrix out for ``w4_project_device`` (``gqa_w4_pack_device``; ``lara_amd.w4.packed_bytes`` gives
+        the sizes, ``lara_amd.w4.quantize`` makes codes and scales)."""
+        self._call("gqa_w4_pack_device", ctypes.c_void_p(codes_ptr), ctypes.c_void_p(scales_ptr), int(rows), int(hidden),
+                   int(group), ctypes.c_void_p(w_ptr), ctypes.c_void_p(w_scales_ptr),
+                   ctypes.c_void_p(stream) if stream else None)
+
+    def w4_unpack_device(self, w_ptr: int, w_scales_ptr: int, rows: int, hidden: int, group: int, out_ptr: int, *,
+                         stream: int | None = None) -> None:
+        """A packed 4-bit matrix as bf16 [rows, hidden] (``gqa_w4_unpack_device``)."""
+        self._call("gqa_w4_unpack_device", ctypes.c_void_p(w_ptr), ctypes.c_void_p(w_scales_ptr), int(rows), int(hidden),
+                   int(group), ctypes.c_void_p(out_ptr), ctypes.c_void_p(stream) if stream else None)
+
+    def w4_project_device(self, x_ptr: int, n_tokens: int, hidden: int, w_ptr: int, w_scales_ptr: int, group: int, rows: int,
+                          y_ptr: int, *, rms_weight_ptr: int | None = None, rms_eps: float = RMS_NORM_EPS,
+                          ldy: int | None = None, stream: int | None = None) -> None:
+        """y [n_tokens, ldy] = (RMSNorm of) x [n_tokens, hidden] times a packed 4-bit matrix (``gqa_w4_project_device``);
+        enqueued, not synchronised."""
+        self._call("gqa_w4_project_device", ctypes.c_void_p(x_ptr), int(n_tokens), int(hidden), ctypes.c_void_p(w_ptr),
+                   ctypes.c_void_p(w_scales_ptr), int(group), int(rows),
+                   ctypes.c_void_p(rms_weight_ptr) if rms_weight_ptr else None, float(rms_eps), ctypes.c_void_p(y_ptr),
+                   int(rows if ldy is None else ldy), ctypes.c_void_p(stream) if stream else None)
 
     def layer_stage_us(self) -> tuple[float, float, float]:
         """Device time (us) of the RMSNorm, projection and RoPE stages of the last ``run_layer``

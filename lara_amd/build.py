@@ -18,7 +18,8 @@ REPO_ROOT = PKG_DIR.parent
 CSRC = PKG_DIR / "csrc"
 BUILD_DIR = REPO_ROOT / "_build"
 LIB_PATH = PKG_DIR / "libgqa.so"
-SOURCES = ("gqa_api.hip", "decode.hip", "kv_cache.hip", "layer.hip", "prefill.hip", "probe.hip", "rtl_exact.hip")
+SOURCES = ("gqa_api.hip", "decode.hip", "decode_kv8.hip", "heads.hip", "kv8.hip", "kv_cache.hip", "layer.hip", "prefill.hip",
+           "probe.hip", "rtl_exact.hip", "w4.hip")
 DATA = PKG_DIR / "data"
 
 HIP_FLAGS = [

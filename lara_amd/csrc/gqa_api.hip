@@ -65,11 +65,22 @@ struct gqa_ctx {
     int max_splits_cap = 0;
     float scale = 0.f;
     hipStream_t stream = nullptr;
-    uint16_t* k_cache = nullptr;  // the active layer's K pool (k_pool + layer * kv_words)
+    uint16_t* k_cache = nullptr;  // the active layer's K pool (k_pool + layer * kv_bytes)
     uint16_t* v_cache = nullptr;
     uint16_t* k_pool = nullptr;   // the allocations: n_layers pools back to back
     uint16_t* v_pool = nullptr;
     int n_layers = 1, layer = 0;
+    // E4M3 cache (gqa_create_kv8): k_cache and v_cache are rows of codes, one byte a value, and every row has a scale byte.
+    bool kv8 = false;
+    uint8_t* k_scale = nullptr;  // the active layer's
+    uint8_t* v_scale = nullptr;
+    uint8_t* k_scale_pool = nullptr;
+    uint8_t* v_scale_pool = nullptr;
+    uint8_t* kv8_ws = nullptr;       // bf16 rows of one sequence: what prefill reads, and the layer stage and the host
+    size_t kv8_ws_bytes = 0;         // forms pass through (grow-only)
+    hipEvent_t ev_kv8_ws = nullptr;  // the last use of it has ended
+    hipStream_t kv8_ws_stream = nullptr;  // where that was (only compared: it may be gone)
+    bool kv8_ws_used = false;
     float* part_o = nullptr;
     float* part_ml = nullptr;
     int32_t* arrivals = nullptr;  // [B*H_kv] split arrival counters of the fused merge, then the row ticket
@@ -165,9 +176,29 @@ void last_hip_error(hipError_t e, const char* what) {
     snprintf(g_last_error, sizeof(g_last_error), "%s: %s", what, hipGetErrorString(e));
 }
 
-inline size_t kv_words(const gqa_ctx* c) {
-    if (c->paged) return (size_t)c->n_pages * c->cfg.n_kv_heads * c->page_size * c->cfg.head_dim;
-    return (size_t)c->cfg.batch * c->cfg.n_kv_heads * c->l_cap * c->cfg.head_dim;
+// Rows of a layer's K (and of its V) pool, and the values and bytes in them.
+inline size_t kv_rows(const gqa_ctx* c) {
+    if (c->paged) return (size_t)c->n_pages * c->cfg.n_kv_heads * c->page_size;
+    return (size_t)c->cfg.batch * c->cfg.n_kv_heads * c->l_cap;
+}
+inline int kv_value_bytes(const gqa_ctx* c) { return c->kv8 ? 1 : 2; }
+inline size_t kv_bytes(const gqa_ctx* c) { return kv_rows(c) * c->cfg.head_dim * kv_value_bytes(c); }
+
+// Makes `layer` the one that the context's cache pointers name.
+void point_at_layer(gqa_ctx* c, int layer) {
+    const size_t off = kv_bytes(c) * (size_t)layer;
+    c->k_cache = (uint16_t*)((uint8_t*)c->k_pool + off);
+    c->v_cache = (uint16_t*)((uint8_t*)c->v_pool + off);
+    if (c->kv8) {
+        c->k_scale = c->k_scale_pool + kv_rows(c) * (size_t)layer;
+        c->v_scale = c->v_scale_pool + kv_rows(c) * (size_t)layer;
+    }
+}
+
+// The active layer's cache as the E4M3 kernels and the row reader take it.
+Kv8Cache cache_view(const gqa_ctx* c) {
+    return Kv8Cache{(uint8_t*)c->k_cache, (uint8_t*)c->v_cache, c->k_scale, c->v_scale, c->cfg.n_kv_heads, c->l_cap,
+                    c->cfg.max_seq_len, c->paged ? c->table_dev : nullptr, c->page_shift, c->max_pages};
 }
 
 // Row (in units of D elements) of token t of (b, h) in the cache, or -1 (unmapped page).
@@ -218,9 +249,9 @@ int plan_splits(int batch, int n_kv_heads, int n_cu, int waves) {
 constexpr int64_t kDecodeSplitMinBytes = 128 << 10;
 constexpr int kUnsplitUnits = 32;
 
-int plan_chunk(int batch, int n_kv_heads, int group, int n_cu, int max_len, int waves, int head_dim) {
-    const int quantum = waves * decode_round_keys(group);
-    const int64_t unit_bytes = (int64_t)max_len * head_dim * 2 * 2;
+int plan_chunk(int batch, int n_kv_heads, int round_keys, int n_cu, int max_len, int waves, int row_bytes) {
+    const int quantum = waves * round_keys;
+    const int64_t unit_bytes = (int64_t)max_len * row_bytes * 2;
     if (unit_bytes <= (batch * (int64_t)n_kv_heads >= kUnsplitUnits ? 2 : 1) * kDecodeSplitMinBytes)
         return std::max(quantum, (max_len + quantum - 1) / quantum * quantum);
     const int splits = plan_splits(batch, n_kv_heads, n_cu, waves);
@@ -292,26 +323,27 @@ struct DecodeShape {
 };
 
 DecodeShape plan_decode_shape(int batch, int n_kv_heads, int group, int head_dim, int n_cu, int max_len,
-                              int chunk_opt, int merge_option) {
+                              int chunk_opt, int merge_option, bool kv8 = false) {
     const int64_t units = (int64_t)batch * n_kv_heads;
+    const int round_keys = kv8 ? kKv8RoundKeys : decode_round_keys(group), row_bytes = kv8 ? head_dim : 2 * head_dim;
     auto in_chunks = [&](int chunk, int waves) {
         const int splits = decode_split_count(max_len, chunk);
         return DecodeShape{chunk, splits, waves, fuse_merge(merge_option, (int)units, splits, n_cu)};
     };
     auto shape = [&](int waves) {
-        return in_chunks(chunk_opt > 0 ? chunk_opt : plan_chunk(batch, n_kv_heads, group, n_cu, max_len, waves, head_dim),
+        return in_chunks(chunk_opt > 0 ? chunk_opt : plan_chunk(batch, n_kv_heads, round_keys, n_cu, max_len, waves, row_bytes),
                          waves);
     };
     const DecodeShape big = shape(kDecodeWaves);
     if (units * big.max_splits <= kSmallDecodeGrid) return shape(kDecodeWavesSmall);
     if (chunk_opt > 0 || merge_option != GQA_DECODE_MERGE_AUTO || big.max_splits <= 1) return big;
-    const int shortest = kDecodeWaves * decode_round_keys(group);
+    const int shortest = kDecodeWaves * round_keys;
     DecodeShape plain = big;
     if (!big.fused && big.chunk == shortest) {
         const DecodeShape twice = in_chunks(2 * shortest, kDecodeWaves);
         if (twice.fused) plain = twice;
     }
-    if (units > kFusedPlanUnits || units * max_len * head_dim * 2 * 2 > kFusedPlanBytes || (plain.fused && head_dim <= 64))
+    if (units > kFusedPlanUnits || units * max_len * row_bytes * 2 > kFusedPlanBytes || (plain.fused && head_dim <= 64))
         return plain;
     const int splits = std::max(1, std::min(kFusedPlanSplits, (int)(kFusedPlanGrid * n_cu) / (int)units));
     const int even = (max_len + splits - 1) / splits;
@@ -367,9 +399,11 @@ int profile_enable(gqa_ctx* c, int on) {
 // run_decode launches it, a prepared step (gqa_graph) keeps it for its replays.
 int plan_decode(gqa_ctx* c, const void* q, const int32_t* lens, const void* k_new, const void* v_new,
                 const int32_t* positions, void* o, float* lse, int max_len, DecodeArgs* out, bool* combine) {
-    if (!decode_supported(c->cfg.head_dim, c->group) || c->numerics != GQA_NUMERICS_EXACT) return GQA_ERR_UNSUPPORTED;
+    if (!(c->kv8 ? decode_kv8_supported(c->cfg.head_dim, c->group) : decode_supported(c->cfg.head_dim, c->group)) ||
+        c->numerics != GQA_NUMERICS_EXACT)
+        return GQA_ERR_UNSUPPORTED;
     const DecodeShape shape = plan_decode_shape(c->cfg.batch, c->cfg.n_kv_heads, c->group, c->cfg.head_dim, c->n_cu,
-                                                max_len, c->chunk_opt, c->decode_merge);
+                                                max_len, c->chunk_opt, c->decode_merge, c->kv8);
     const int chunk = shape.chunk;
     const int max_splits = shape.max_splits;
     if (max_splits > c->max_splits_cap) return GQA_ERR_RANGE;
@@ -398,12 +432,23 @@ int plan_decode(gqa_ctx* c, const void* q, const int32_t* lens, const void* k_ne
     a.max_pages = c->max_pages;
     a.zero_row = c->zero_row;
     a.longest_first = c->cfg.batch > 1;
-    a.cached = decode_cached_loads((int64_t)c->cfg.batch * c->cfg.n_kv_heads, max_len, c->cfg.head_dim) ? 1 : 0;
+    a.cached = decode_cached_loads((int64_t)c->cfg.batch * c->cfg.n_kv_heads, max_len, c->cfg.head_dim * kv_value_bytes(c)) ? 1 : 0;
+    a.k_scale = c->k_scale;
+    a.v_scale = c->v_scale;
+    a.group = c->group;
     a.waves = shape.waves;
     a.arrivals = shape.fused ? c->arrivals : nullptr;
     *combine = max_splits > 1 && a.arrivals == nullptr;
     a.ticket = (c->cfg.batch > 1 && max_splits == 1) ? c->arrivals + (size_t)c->cfg.batch * c->cfg.n_kv_heads : nullptr;
     return GQA_OK;
+}
+
+// The launches of a planned decode step, with the Launch of each.
+hipError_t launch_step(int head_dim, int group, const DecodeArgs& a, const Launch& l) {
+    return a.k_scale != nullptr ? launch_decode_kv8(head_dim, a, l) : launch_decode(head_dim, group, a, l);
+}
+hipError_t launch_step_merge(int head_dim, int group, const DecodeArgs& a, const Launch& l) {
+    return a.k_scale != nullptr ? launch_decode_kv8_merge(head_dim, a, l) : launch_combine(head_dim, group, a, l);
 }
 
 int run_decode(gqa_ctx* c, const void* q, const int32_t* lens, const void* k_new, const void* v_new,
@@ -412,8 +457,8 @@ int run_decode(gqa_ctx* c, const void* q, const int32_t* lens, const void* k_new
     bool combine = false;
     const int rc = plan_decode(c, q, lens, k_new, v_new, positions, o, lse, max_len, &a, &combine);
     if (rc != GQA_OK) return rc;
-    HIP_TRY(launch_decode(c->cfg.head_dim, c->group, a, timed(c, GQA_TIMER_DECODE, s)));
-    if (combine) HIP_TRY(launch_combine(c->cfg.head_dim, c->group, a, timed(c, GQA_TIMER_COMBINE, s)));
+    HIP_TRY(launch_step(c->cfg.head_dim, c->group, a, timed(c, GQA_TIMER_DECODE, s)));
+    if (combine) HIP_TRY(launch_step_merge(c->cfg.head_dim, c->group, a, timed(c, GQA_TIMER_COMBINE, s)));
     return GQA_OK;
 }
 
@@ -531,10 +576,17 @@ bool take_auto_ws(gqa_ctx* c, hipStream_t s) {
     return true;
 }
 
-int run_prefill(gqa_ctx* c, int32_t b, const void* q, int32_t q_len, int32_t q_pos_base, int32_t kv_len,
-                int32_t kv_pos_base, int32_t causal, void* o, float* lse, hipStream_t s,
-                const void* k_new = nullptr, const void* v_new = nullptr, int32_t n_new = 0) {
-    if (c->paged) c->pages.touch(b);
+// The bf16 rows that a prefill launch reads: those of sequence b in the context's cache, or a copy of them.
+struct PrefillRows {
+    uint16_t* k;
+    uint16_t* v;
+    int l_cap;
+    const int32_t* table;  // its block table, or nullptr: rows in order
+};
+
+int run_prefill_rows(gqa_ctx* c, int32_t b, const PrefillRows& from, const void* q, int32_t q_len, int32_t q_pos_base,
+                     int32_t kv_len, int32_t kv_pos_base, int32_t causal, void* o, float* lse, hipStream_t s,
+                     const void* k_new, const void* v_new, int32_t n_new) {
     if (c->numerics == GQA_NUMERICS_KV260) {
         if (c->paged) return GQA_ERR_UNSUPPORTED;
         const size_t seq = (size_t)b * c->cfg.n_kv_heads * c->l_cap * c->cfg.head_dim;
@@ -612,11 +664,10 @@ int run_prefill(gqa_ctx* c, int32_t b, const void* q, int32_t q_len, int32_t q_p
         plan = plan_for(1, 1);  // one segment
     const bool rows = c->prefill_kernel == GQA_PREFILL_KERNEL_ROWS || (plan_auto && segs == 0);
     PrefillArgs a{};
-    const size_t seq_off = c->paged ? 0 : (size_t)b * c->cfg.n_kv_heads * c->l_cap * c->cfg.head_dim;
     a.q = (const uint16_t*)q;
-    a.kc = c->k_cache + seq_off;
-    a.vc = c->v_cache + seq_off;
-    a.block_table = c->paged ? c->table_dev + (size_t)b * c->max_pages : nullptr;
+    a.kc = from.k;
+    a.vc = from.v;
+    a.block_table = from.table;
     a.page_shift = c->page_shift;
     a.k_new = (const uint16_t*)k_new;
     a.v_new = (const uint16_t*)v_new;
@@ -624,7 +675,7 @@ int run_prefill(gqa_ctx* c, int32_t b, const void* q, int32_t q_len, int32_t q_p
     a.n_new = n_new;
     a.n_q_heads = c->cfg.n_q_heads;
     a.n_kv_heads = c->cfg.n_kv_heads;
-    a.l_cap = c->l_cap;
+    a.l_cap = from.l_cap;
     a.q_len = q_len;
     a.kv_len = kv_len;
     a.q_pos_base = q_pos_base;
@@ -660,6 +711,84 @@ int run_prefill(gqa_ctx* c, int32_t b, const void* q, int32_t q_len, int32_t q_p
     c->last_prefill_kernel = a.pair ? GQA_PREFILL_KERNEL_PAIRED : GQA_PREFILL_KERNEL_SHARED;
     c->last_prefill_segs = plan.n_segs;
     return GQA_OK;
+}
+
+int ensure_buffer(uint8_t** buf, size_t* cap, size_t bytes);
+
+// The E4M3 context's bf16 workspace for a use on s, at least `bytes` of it; done_kv8_ws ends the use.  There is one: a use
+// waits for the one before it wherever that was (uses on one stream follow each other anyway), so streams that take
+// turns are ordered by it.  Not under a capture: a graph replays beside uses that it knows nothing of.
+int take_kv8_ws(gqa_ctx* c, size_t bytes, hipStream_t s) {
+    if (stream_capturing(s)) return GQA_ERR_UNSUPPORTED;
+    if (bytes > c->kv8_ws_bytes) {  // in powers of two: a growing history does not allocate at each step
+        size_t grown = 1 << 20;
+        while (grown < bytes) grown *= 2;
+        int rc = ensure_buffer(&c->kv8_ws, &c->kv8_ws_bytes, grown);
+        if (rc == GQA_ERR_OOM) rc = ensure_buffer(&c->kv8_ws, &c->kv8_ws_bytes, bytes);
+        if (rc != GQA_OK) return rc;
+    }
+    // (A caller's handle does not name a stream for good, so only the context's own stream goes without the wait.)
+    if (c->kv8_ws_used && !(s == c->stream && c->kv8_ws_stream == s)) HIP_TRY(hipStreamWaitEvent(s, c->ev_kv8_ws, 0));
+    return GQA_OK;
+}
+int done_kv8_ws(gqa_ctx* c, hipStream_t s) {
+    HIP_TRY(hipEventRecord(c->ev_kv8_ws, s));
+    c->kv8_ws_stream = s;
+    c->kv8_ws_used = true;
+    return GQA_OK;
+}
+
+// Quantises bf16 rows [H_kv][n][D] into rows start .. of sequence b.
+hipError_t write_kv8(gqa_ctx* c, int b, int start, int n, const void* k, const void* v, hipStream_t s) {
+    Kv8WriteArgs w{};
+    w.cache = cache_view(c);
+    w.k = (const uint16_t*)k;
+    w.v = (const uint16_t*)v;
+    w.b = b;
+    w.start = start;
+    w.n = n;
+    w.n_rows = (int64_t)c->cfg.n_kv_heads * n;
+    return launch_kv8_write(c->cfg.head_dim, w, timed(c, GQA_TIMER_APPEND, s));
+}
+
+// Rows start .. of sequence b as bf16 [H_kv][out_rows][D].
+hipError_t read_rows(gqa_ctx* c, int b, int start, int n, int64_t out_rows, void* k, void* v, hipStream_t s) {
+    KvReadArgs r{};
+    r.cache = cache_view(c);
+    r.b = b;
+    r.start = start;
+    r.n = n;
+    r.out_rows = out_rows;
+    r.k = (uint16_t*)k;
+    r.v = (uint16_t*)v;
+    return launch_kv_read(c->cfg.head_dim, r, timed(c, GQA_TIMER_APPEND, s));
+}
+
+int run_prefill(gqa_ctx* c, int32_t b, const void* q, int32_t q_len, int32_t q_pos_base, int32_t kv_len,
+                int32_t kv_pos_base, int32_t causal, void* o, float* lse, hipStream_t s,
+                const void* k_new = nullptr, const void* v_new = nullptr, int32_t n_new = 0) {
+    if (c->paged) c->pages.touch(b);
+    const size_t D = c->cfg.head_dim;
+    if (!c->kv8) {
+        const size_t seq_off = c->paged ? 0 : (size_t)b * c->cfg.n_kv_heads * c->l_cap * D;
+        const PrefillRows rows = {c->k_cache + seq_off, c->v_cache + seq_off, c->l_cap,
+                                  c->paged ? c->table_dev + (size_t)b * c->max_pages : nullptr};
+        return run_prefill_rows(c, b, rows, q, q_len, q_pos_base, kv_len, kv_pos_base, causal, o, lse, s, k_new, v_new, n_new);
+    }
+    // E4M3: the new rows are quantised into the cache, every row that is attended is read back as bf16 and the bf16
+    // kernels run on the copy: the new rows are attended as they are stored.
+    if (!prefill_supported(c->cfg.head_dim, c->group)) return GQA_ERR_UNSUPPORTED;
+    const int cap = std::max(64, (kv_len + 63) / 64 * 64);
+    const size_t side = (size_t)c->cfg.n_kv_heads * cap * D;
+    int rc = take_kv8_ws(c, 2 * side * 2, s);
+    if (rc != GQA_OK) return rc;
+    uint16_t* const k = (uint16_t*)c->kv8_ws;
+    if (n_new > 0) HIP_TRY(write_kv8(c, b, kv_len - n_new, n_new, k_new, v_new, s));
+    HIP_TRY(read_rows(c, b, 0, kv_len, cap, k, k + side, s));
+    rc = run_prefill_rows(c, b, PrefillRows{k, k + side, cap, nullptr}, q, q_len, q_pos_base, kv_len, kv_pos_base, causal, o,
+                          lse, s, nullptr, nullptr, 0);
+    const int done = done_kv8_ws(c, s);
+    return rc != GQA_OK ? rc : done;
 }
 
 int finish_sync(gqa_ctx* c) {
@@ -843,7 +972,8 @@ int tune_projection(gqa_ctx* c, ProjectionPlan* p, Gemm&& gemm, hipStream_t s) {
 // row0.. of sequence b.
 int run_layer_qkv(gqa_ctx* c, int32_t b, const void* x, int32_t n_tokens, int32_t hidden, const void* wq,
                   const void* wk, const void* wv, const void* gamma, float eps, int32_t q_pos_base,
-                  int32_t kv_pos_base, int32_t row0, int32_t rope, void* q_out, hipStream_t s, bool stage_events) {
+                  int32_t kv_pos_base, int32_t row0, int32_t rope, void* q_out, hipStream_t s, bool stage_events,
+                  uint16_t* kv_out = nullptr) {
     const int D = c->cfg.head_dim, nq = c->cfg.n_q_heads * D, nkv = c->cfg.n_kv_heads * D;
     const int ld = nq + 2 * nkv;
     RopeArgs ra{};
@@ -860,6 +990,13 @@ int run_layer_qkv(gqa_ctx* c, int32_t b, const void* x, int32_t n_tokens, int32_
     ra.page_shift = c->page_shift;
     ra.l_cap = c->l_cap;
     ra.row0 = row0;
+    if (kv_out != nullptr) {  // K and V rows apart from the cache, [H_kv][n_tokens][D] each
+        ra.kc = kv_out;
+        ra.vc = kv_out + (size_t)n_tokens * nkv;
+        ra.block_table = nullptr;
+        ra.l_cap = n_tokens;
+        ra.row0 = 0;
+    }
     if (stage_events && !c->ev_layer[0])
         for (int i = 0; i < 4; ++i) HIP_TRY(hipEventCreate(&c->ev_layer[i]));
     c->layer_timed = false;
@@ -877,7 +1014,7 @@ int run_layer_qkv(gqa_ctx* c, int32_t b, const void* x, int32_t n_tokens, int32_
     memcpy(fa.theta, c->theta, sizeof(fa.theta));
     fa.rope = ra;
     // The one-launch stage reads its inputs while it writes: an output that overlaps one takes the general path.
-    const size_t pool_bytes = kv_words(c) * 2;
+    const size_t pool_bytes = kv_bytes(c);
     const struct { const void* p; size_t n; } ins[] = {{x, (size_t)n_tokens * hidden * 2}, {gamma, gamma ? (size_t)hidden * 2 : 0},
                                                        {wq, (size_t)nq * hidden * 2}, {wk, (size_t)nkv * hidden * 2},
                                                        {wv, (size_t)nkv * hidden * 2}};
@@ -984,6 +1121,31 @@ int run_layer_qkv(gqa_ctx* c, int32_t b, const void* x, int32_t n_tokens, int32_
     return GQA_OK;
 }
 
+// The layer stage into the context's cache; an E4M3 cache takes its rows from the stage's bf16 ones (in the workspace).
+int run_layer_stage(gqa_ctx* c, int32_t b, const void* x, int32_t n_tokens, int32_t hidden, const void* wq, const void* wk,
+                    const void* wv, const void* gamma, float eps, int32_t q_pos_base, int32_t kv_pos_base, int32_t row0,
+                    int32_t rope, void* q_out, hipStream_t s, bool stage_events) {
+    uint16_t* rows = nullptr;
+    const size_t side = (size_t)n_tokens * c->cfg.n_kv_heads * c->cfg.head_dim;
+    if (c->kv8) {
+        const int rc = take_kv8_ws(c, 2 * side * 2, s);
+        if (rc != GQA_OK) return rc;
+        rows = (uint16_t*)c->kv8_ws;
+    }
+    int rc = run_layer_qkv(c, b, x, n_tokens, hidden, wq, wk, wv, gamma, eps, q_pos_base, kv_pos_base, row0, rope, q_out, s,
+                           stage_events, rows);
+    if (!c->kv8) return rc;
+    if (rc == GQA_OK) {
+        const hipError_t e = write_kv8(c, b, row0, n_tokens, rows, rows + side, s);
+        if (e != hipSuccess) {
+            last_hip_error(e, "quantising the layer's K/V rows");
+            rc = GQA_ERR_HIP;
+        }
+    }
+    const int done = done_kv8_ws(c, s);
+    return rc != GQA_OK ? rc : done;
+}
+
 int layer_times(gqa_ctx* c) {
     HIP_TRY(hipEventSynchronize(c->ev_layer[3]));
     for (int i = 0; i < 3; ++i) {
@@ -1030,7 +1192,8 @@ int grow_forced_workspace(gqa_ctx* c, int target_wgs) {
     return GQA_OK;
 }
 
-int create_ctx(const gqa_config* cfg, int32_t page_size, int32_t n_pages, int32_t n_layers, gqa_ctx** out_ctx) {
+int create_ctx(const gqa_config* cfg, int32_t page_size, int32_t n_pages, int32_t n_layers, gqa_ctx** out_ctx,
+               bool kv8 = false) {
     if (!cfg || !out_ctx) return GQA_ERR_NULL;
     *out_ctx = nullptr;
     const gqa_config& k = *cfg;
@@ -1039,7 +1202,9 @@ int create_ctx(const gqa_config* cfg, int32_t page_size, int32_t n_pages, int32_
         !(k.scale >= 0.f) || !isfinite(k.scale))
         return GQA_ERR_BAD_CFG;
     const int group = k.n_q_heads / k.n_kv_heads;
-    if (!decode_supported(k.head_dim, group) && !prefill_supported(k.head_dim, group)) return GQA_ERR_UNSUPPORTED;
+    if (!(kv8 ? decode_kv8_supported(k.head_dim, group) : decode_supported(k.head_dim, group)) &&
+        !prefill_supported(k.head_dim, group))
+        return GQA_ERR_UNSUPPORTED;
 
     int n = 0;
     if (hipGetDeviceCount(&n) != hipSuccess || n < 1) return GQA_ERR_NO_DEVICE;
@@ -1052,6 +1217,7 @@ int create_ctx(const gqa_config* cfg, int32_t page_size, int32_t n_pages, int32_
     gqa_ctx* c = new gqa_ctx();
     c->cfg = k;
     c->group = group;
+    c->kv8 = kv8;
     c->l_cap = ((k.max_seq_len + 63) / 64) * 64;
     // Enough partial slots for any plan: the automatic one at either work-group shape, or forced
     // chunks down to kMinSplitCap keys.
@@ -1084,10 +1250,13 @@ int create_ctx(const gqa_config* cfg, int32_t page_size, int32_t n_pages, int32_
         if (rc != GQA_OK) return;
         if (hipMalloc(p, bytes) != hipSuccess) rc = GQA_ERR_OOM;
     };
-    alloc((void**)&c->k_pool, kv_words(c) * 2 * (size_t)n_layers);
-    alloc((void**)&c->v_pool, kv_words(c) * 2 * (size_t)n_layers);
-    c->k_cache = c->k_pool;
-    c->v_cache = c->v_pool;
+    alloc((void**)&c->k_pool, kv_bytes(c) * (size_t)n_layers);
+    alloc((void**)&c->v_pool, kv_bytes(c) * (size_t)n_layers);
+    if (kv8) {
+        alloc((void**)&c->k_scale_pool, kv_rows(c) * (size_t)n_layers);
+        alloc((void**)&c->v_scale_pool, kv_rows(c) * (size_t)n_layers);
+    }
+    point_at_layer(c, 0);
     alloc((void**)&c->part_o, units * c->max_splits_cap * group * D * sizeof(float));
     alloc((void**)&c->part_ml, units * c->max_splits_cap * group * 2 * sizeof(float));
     alloc((void**)&c->arrivals, (units + 1) * sizeof(int32_t));
@@ -1112,6 +1281,7 @@ int create_ctx(const gqa_config* cfg, int32_t page_size, int32_t n_pages, int32_
     if (rc == GQA_OK) {
         bool ok = hipEventCreate(&c->ev_begin) == hipSuccess && hipEventCreate(&c->ev_end) == hipSuccess;
         for (int i = 0; i < 4 && ok; ++i) ok = hipEventCreate(&c->ev_t[i]) == hipSuccess;
+        ok = ok && hipEventCreateWithFlags(&c->ev_kv8_ws, hipEventDisableTiming | hipEventDisableSystemFence) == hipSuccess;
         ok = ok && hipEventCreateWithFlags(&c->ev_auto_ws, hipEventDisableTiming | hipEventDisableSystemFence) == hipSuccess;
         for (hipEvent_t& e : c->ev_part) ok = ok && hipEventCreateWithFlags(&e, hipEventDisableTiming) == hipSuccess;
         if (!ok) rc = GQA_ERR_HIP;
@@ -1119,8 +1289,10 @@ int create_ctx(const gqa_config* cfg, int32_t page_size, int32_t n_pages, int32_
     // Zero the caches (every layer's pool) once so rows beyond every sequence's length hold finite words.
     if (rc == GQA_OK && (hipMemsetAsync(c->zero_row, 0, D * 2, c->stream) != hipSuccess ||
                          hipMemsetAsync(c->arrivals, 0, (units + 1) * sizeof(int32_t), c->stream) != hipSuccess ||
-                         hipMemsetAsync(c->k_pool, 0, kv_words(c) * 2 * (size_t)n_layers, c->stream) != hipSuccess ||
-                         hipMemsetAsync(c->v_pool, 0, kv_words(c) * 2 * (size_t)n_layers, c->stream) != hipSuccess ||
+                         hipMemsetAsync(c->k_pool, 0, kv_bytes(c) * (size_t)n_layers, c->stream) != hipSuccess ||
+                         hipMemsetAsync(c->v_pool, 0, kv_bytes(c) * (size_t)n_layers, c->stream) != hipSuccess ||
+                         (kv8 && hipMemsetAsync(c->k_scale_pool, 0, kv_rows(c) * (size_t)n_layers, c->stream) != hipSuccess) ||
+                         (kv8 && hipMemsetAsync(c->v_scale_pool, 0, kv_rows(c) * (size_t)n_layers, c->stream) != hipSuccess) ||
                          (c->paged && hipMemsetAsync(c->table_dev, 0xFF, (size_t)k.batch * c->max_pages * 4,
                                                      c->stream) != hipSuccess) ||  // every entry -1: unmapped
                          hipStreamSynchronize(c->stream) != hipSuccess))
@@ -1299,12 +1471,33 @@ int gqa_create_paged_layers(const gqa_config* cfg, int32_t page_size, int32_t n_
     return create_ctx(cfg, page_size, n_pages, n_layers, out_ctx);
 }
 
+int gqa_create_kv8(const gqa_config* cfg, int32_t page_size, int32_t n_pages, int32_t n_layers, gqa_ctx** out_ctx) {
+    if (!cfg || !out_ctx) return GQA_ERR_NULL;
+    *out_ctx = nullptr;
+    if (page_size == 0 ? (n_pages != 0 || n_layers != 1)
+                       : (page_size < 64 || page_size > (1 << 16) || (page_size & (page_size - 1)) != 0 || n_pages < 1 ||
+                          n_layers < 1 || n_layers > GQA_MAX_LAYERS))
+        return GQA_ERR_BAD_CFG;
+    return create_ctx(cfg, page_size, n_pages, n_layers, out_ctx, true);
+}
+
+int gqa_kv8_scales(gqa_ctx* c, void** k_scale, void** v_scale) {
+    if (!c) return GQA_ERR_NULL;
+    if (!c->kv8) return GQA_ERR_UNSUPPORTED;
+    if (k_scale) *k_scale = c->k_scale;
+    if (v_scale) *v_scale = c->v_scale;
+    return GQA_OK;
+}
+
 int gqa_destroy(gqa_ctx* c) {
     if (!c) return GQA_ERR_NULL;
     (void)hipSetDevice(c->cfg.device);
     if (c->stream) (void)hipStreamSynchronize(c->stream);
     (void)hipFree(c->k_pool);
     (void)hipFree(c->v_pool);
+    (void)hipFree(c->k_scale_pool);
+    (void)hipFree(c->v_scale_pool);
+    (void)hipFree(c->kv8_ws);
     (void)hipFree(c->part_o);
     (void)hipFree(c->part_ml);
     (void)hipFree(c->arrivals);
@@ -1324,6 +1517,7 @@ int gqa_destroy(gqa_ctx* c) {
     for (hipEvent_t e : c->ev_part)
         if (e) (void)hipEventDestroy(e);
     if (c->ev_auto_ws) (void)hipEventDestroy(c->ev_auto_ws);
+    if (c->ev_kv8_ws) (void)hipEventDestroy(c->ev_kv8_ws);
     if (c->ev_begin) (void)hipEventDestroy(c->ev_begin);
     if (c->ev_end) (void)hipEventDestroy(c->ev_end);
     for (int i = 0; i < GQA_TIMER_COUNT; ++i) {
@@ -1380,15 +1574,13 @@ int gqa_set_option(gqa_ctx* c, int32_t option, int64_t value) {
             return GQA_OK;
         case GQA_OPT_LAYER: {
             if (value < 0 || value >= c->n_layers) return GQA_ERR_RANGE;
-            const size_t off = kv_words(c) * (size_t)value;
             c->layer = (int)value;
-            c->k_cache = c->k_pool + off;
-            c->v_cache = c->v_pool + off;
+            point_at_layer(c, c->layer);
             return GQA_OK;
         }
         case GQA_OPT_NUMERICS:
             if (value != GQA_NUMERICS_EXACT && value != GQA_NUMERICS_KV260) return GQA_ERR_RANGE;
-            if (value == GQA_NUMERICS_KV260 && ((c->cfg.head_dim != 64 && c->cfg.head_dim != 128) || c->paged))
+            if (value == GQA_NUMERICS_KV260 && ((c->cfg.head_dim != 64 && c->cfg.head_dim != 128) || c->paged || c->kv8))
                 return GQA_ERR_UNSUPPORTED;
             c->numerics = (int)value;
             return GQA_OK;
@@ -1503,6 +1695,20 @@ int gqa_load_kv(gqa_ctx* c, int32_t b, int32_t start_pos, int32_t n, const uint1
     if (rc != GQA_OK) return rc;
     if (n == 0) return GQA_OK;
     HIP_TRY(hipSetDevice(c->cfg.device));
+    if (c->kv8) {
+        if (!rows_backed(c, b, start_pos, n)) return GQA_ERR_RANGE;
+        if (c->paged) c->pages.touch(b);
+        const size_t side = (size_t)c->cfg.n_kv_heads * n * c->cfg.head_dim;
+        rc = take_kv8_ws(c, 2 * side * 2, c->stream);
+        if (rc != GQA_OK) return rc;
+        uint16_t* const rows = (uint16_t*)c->kv8_ws;
+        HIP_TRY(hipEventRecord(c->ev_begin, c->stream));
+        HIP_TRY(hipMemcpyAsync(rows, k, side * 2, hipMemcpyHostToDevice, c->stream));
+        HIP_TRY(hipMemcpyAsync(rows + side, v, side * 2, hipMemcpyHostToDevice, c->stream));
+        HIP_TRY(write_kv8(c, b, start_pos, n, rows, rows + side, c->stream));
+        rc = done_kv8_ws(c, c->stream);
+        return rc != GQA_OK ? rc : finish_sync(c);
+    }
     if (c->paged) {
         if (!rows_backed(c, b, start_pos, n)) return GQA_ERR_RANGE;
         c->pages.touch(b);
@@ -1554,6 +1760,12 @@ int gqa_load_kv_device(gqa_ctx* c, int32_t b, int32_t start_pos, int32_t n, cons
     if (n < 0 || start_pos < 0 || (int64_t)start_pos + n > c->cfg.max_seq_len) return GQA_ERR_RANGE;
     if (n == 0) return GQA_OK;
     hipStream_t s = pick_stream(c, stream);
+    if (c->kv8) {
+        if (!aligned16(k) || !aligned16(v) || !rows_backed(c, b, start_pos, n)) return GQA_ERR_RANGE;
+        if (c->paged) c->pages.touch(b);
+        HIP_TRY(write_kv8(c, b, start_pos, n, k, v, s));
+        return GQA_OK;
+    }
     if (c->paged) {
         if (!rows_backed(c, b, start_pos, n)) return GQA_ERR_RANGE;
         c->pages.touch(b);
@@ -1579,6 +1791,20 @@ int gqa_read_kv(gqa_ctx* c, int32_t b, int32_t start_pos, int32_t n, uint16_t* k
     if (rc != GQA_OK) return rc;
     if (n == 0) return GQA_OK;
     HIP_TRY(hipSetDevice(c->cfg.device));
+    if (c->kv8) {
+        if (!rows_backed(c, b, start_pos, n)) return GQA_ERR_RANGE;
+        const size_t side = (size_t)c->cfg.n_kv_heads * n * c->cfg.head_dim;
+        rc = take_kv8_ws(c, 2 * side * 2, c->stream);
+        if (rc != GQA_OK) return rc;
+        uint16_t* const rows = (uint16_t*)c->kv8_ws;
+        HIP_TRY(read_rows(c, b, start_pos, n, n, rows, rows + side, c->stream));
+        HIP_TRY(hipMemcpyAsync(k, rows, side * 2, hipMemcpyDeviceToHost, c->stream));
+        HIP_TRY(hipMemcpyAsync(v, rows + side, side * 2, hipMemcpyDeviceToHost, c->stream));
+        rc = done_kv8_ws(c, c->stream);
+        if (rc != GQA_OK) return rc;
+        HIP_TRY(hipStreamSynchronize(c->stream));
+        return GQA_OK;
+    }
     if (c->paged) {
         if (!rows_backed(c, b, start_pos, n)) return GQA_ERR_RANGE;
         rc = copy_rows_paged(c, b, start_pos, n, nullptr, nullptr, k, v, hipMemcpyDeviceToHost, c->stream);
@@ -1594,6 +1820,17 @@ int gqa_read_kv(gqa_ctx* c, int32_t b, int32_t start_pos, int32_t n, uint16_t* k
         HIP_TRY(hipMemcpyAsync(v + dst, c->v_cache + src, n * D * 2, hipMemcpyDeviceToHost, c->stream));
     }
     HIP_TRY(hipStreamSynchronize(c->stream));
+    return GQA_OK;
+}
+
+int gqa_read_kv_device(gqa_ctx* c, int32_t b, int32_t start_pos, int32_t n, void* k, void* v, void* stream) {
+    if (!c || !k || !v) return GQA_ERR_NULL;
+    if (b < 0 || b >= c->cfg.batch) return GQA_ERR_STREAM_DEST;
+    if (n < 0 || start_pos < 0 || (int64_t)start_pos + n > c->cfg.max_seq_len) return GQA_ERR_RANGE;
+    if (!aligned16(k) || !aligned16(v)) return GQA_ERR_RANGE;
+    if (n == 0) return GQA_OK;
+    if (!rows_backed(c, b, start_pos, n)) return GQA_ERR_RANGE;
+    HIP_TRY(read_rows(c, b, start_pos, n, n, k, v, pick_stream(c, stream)));
     return GQA_OK;
 }
 
@@ -1621,6 +1858,18 @@ int gqa_append_kv_device(gqa_ctx* c, const void* k_rows, const void* v_rows, con
                          void* stream) {
     if (!c || !k_rows || !v_rows || !positions) return GQA_ERR_NULL;
     hipStream_t s = pick_stream(c, stream);
+    if (c->kv8) {
+        if (!aligned16(k_rows) || !aligned16(v_rows)) return GQA_ERR_RANGE;
+        Kv8WriteArgs w{};
+        w.cache = cache_view(c);
+        w.k = (const uint16_t*)k_rows;
+        w.v = (const uint16_t*)v_rows;
+        w.n = 1;
+        w.n_rows = (int64_t)c->cfg.batch * c->cfg.n_kv_heads;
+        w.positions = positions;
+        HIP_TRY(launch_kv8_write(c->cfg.head_dim, w, timed(c, GQA_TIMER_APPEND, s)));
+        return GQA_OK;
+    }
     HIP_TRY(launch_append((const uint16_t*)k_rows, (const uint16_t*)v_rows, positions, c->k_cache, c->v_cache,
                           c->cfg.batch, c->cfg.n_kv_heads, c->cfg.head_dim, c->l_cap, c->cfg.max_seq_len,
                           c->paged ? c->table_dev : nullptr, c->page_shift, c->max_pages,
@@ -1760,7 +2009,7 @@ int gqa_decode_append_noalloc(const gqa_config* cfg, void* k_cache, void* v_cach
     a.lse = lse;
     a.zero_row = dev->zero;
     a.longest_first = k.batch > 1;
-    a.cached = decode_cached_loads((int64_t)k.batch * k.n_kv_heads, k.max_seq_len, k.head_dim) ? 1 : 0;
+    a.cached = decode_cached_loads((int64_t)k.batch * k.n_kv_heads, k.max_seq_len, 2 * k.head_dim) ? 1 : 0;
     a.waves = shape.waves;
     // The same merge as the context entry point's default (GQA_DECODE_MERGE_AUTO), when the counters
     // cover the units.
@@ -1895,8 +2144,8 @@ int gqa_layer_qkv_device(gqa_ctx* c, int32_t b, const void* x, int32_t n_tokens,
     if (!rows_backed(c, b, kv_row0, n_tokens)) return GQA_ERR_RANGE;
     if (!(rms_eps >= 0.f) || !isfinite(rms_eps)) return GQA_ERR_RANGE;
     HIP_TRY(hipSetDevice(c->cfg.device));
-    return run_layer_qkv(c, b, x, n_tokens, hidden, wq, wk, wv, rms_weight, rms_eps, q_pos_base, kv_pos_base, kv_row0,
-                         rope, q_out, pick_stream(c, stream), false);
+    return run_layer_stage(c, b, x, n_tokens, hidden, wq, wk, wv, rms_weight, rms_eps, q_pos_base, kv_pos_base, kv_row0,
+                           rope, q_out, pick_stream(c, stream), false);
 }
 
 int gqa_submit_layer(gqa_ctx* c, int32_t b, const uint16_t* x, int32_t n_tokens, int32_t hidden, const uint16_t* wq,
@@ -1938,8 +2187,8 @@ int gqa_submit_layer(gqa_ctx* c, int32_t b, const uint16_t* x, int32_t n_tokens,
     HIP_TRY(hipMemcpyAsync(dwk, wk, wkb, hipMemcpyHostToDevice, c->stream));
     HIP_TRY(hipMemcpyAsync(dwv, wv, wkb, hipMemcpyHostToDevice, c->stream));
     if (rms_weight) HIP_TRY(hipMemcpyAsync(dg, rms_weight, gb, hipMemcpyHostToDevice, c->stream));
-    rc = run_layer_qkv(c, b, dx, n_tokens, hidden, dwq, dwk, dwv, rms_weight ? dg : nullptr, rms_eps, q_pos_base,
-                       kv_pos_base, 0, rope, c->q_dev, c->stream, true);
+    rc = run_layer_stage(c, b, dx, n_tokens, hidden, dwq, dwk, dwv, rms_weight ? dg : nullptr, rms_eps, q_pos_base,
+                         kv_pos_base, 0, rope, c->q_dev, c->stream, true);
     if (rc != GQA_OK) return rc;
     HIP_TRY(hipStreamSynchronize(c->stream));
     rc = layer_times(c);
@@ -1955,6 +2204,158 @@ int gqa_layer_times(gqa_ctx* c, float* out_us, int32_t n) {
     int rc = layer_times(c);
     if (rc != GQA_OK) return rc;
     for (int i = 0; i < n; ++i) out_us[i] = c->layer_us[i];
+    return GQA_OK;
+}
+
+// ---- heads and 4-bit projections ------------------------------------------------------
+
+namespace {
+
+// The context's device for the length of a call; the caller's is put back.
+struct DeviceScope {
+    int before = -1;
+    hipError_t status;
+    explicit DeviceScope(int device) {
+        status = hipGetDevice(&before);
+        if (status == hipSuccess && before != device) status = hipSetDevice(device);
+        else before = -1;
+    }
+    ~DeviceScope() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+};
+
+constexpr int kHeadsMaxPosition = 1 << 30;
+
+int run_heads(gqa_ctx* c, HeadsArgs& a, const void* qkv, int64_t ld, const void* q_weight, const void* k_weight, float eps,
+              double rope_base, void* q_out, hipStream_t s) {
+    const int64_t width = (int64_t)(c->cfg.n_q_heads + 2 * c->cfg.n_kv_heads) * c->cfg.head_dim;
+    if (ld < width || ld % 8 != 0 || !aligned16(qkv) || !aligned16(q_weight) || !aligned16(k_weight) || !aligned16(q_out))
+        return GQA_ERR_RANGE;
+    if (!(eps >= 0.f) || !isfinite(eps)) return GQA_ERR_RANGE;
+    if (!(rope_base == 0.0 || rope_base > 1.0) || !isfinite(rope_base)) return GQA_ERR_RANGE;
+    // The kernel reads the rows while it writes Q and the cache.
+    const size_t in = ((size_t)(a.n_tokens - 1) * ld + width) * 2, out = (size_t)a.n_tokens * c->cfg.n_q_heads * c->cfg.head_dim * 2;
+    if (overlaps(qkv, in, q_out, out) || overlaps(qkv, in, c->k_cache, kv_bytes(c)) || overlaps(qkv, in, c->v_cache, kv_bytes(c)))
+        return GQA_ERR_RANGE;
+    a.x = (const uint16_t*)qkv;
+    a.ld = ld;
+    a.n_q_heads = c->cfg.n_q_heads;
+    a.wq = (const uint16_t*)q_weight;
+    a.wk = (const uint16_t*)k_weight;
+    a.eps = eps;
+    a.log2_base = rope_base > 0.0 ? log2(rope_base) : 0.0;
+    a.q_out = (uint16_t*)q_out;
+    a.cache = cache_view(c);
+    const DeviceScope device(c->cfg.device);
+    HIP_TRY(device.status);
+    HIP_TRY(launch_qk_norm_rope(c->cfg.head_dim, a, timed(c, GQA_TIMER_ROPE, s)));
+    return GQA_OK;
+}
+
+// Largest matrix side of the 4-bit products: packed sizes and grids stay in range.
+constexpr int32_t kW4MaxRows = 1 << 20, kW4MaxHidden = 1 << 16;
+
+int check_w4(int32_t rows, int32_t hidden, int32_t group) {
+    if (group != 32 && group != 64 && group != 128) return GQA_ERR_UNSUPPORTED;
+    if (rows < 1 || rows > kW4MaxRows || hidden < group || hidden > kW4MaxHidden || hidden % group != 0) return GQA_ERR_RANGE;
+    return GQA_OK;
+}
+
+}  // namespace
+
+int gqa_qk_norm_rope_device(gqa_ctx* c, int32_t b, const void* qkv, int64_t ld, int32_t n_tokens, const void* q_weight,
+                            const void* k_weight, float eps, int32_t q_pos_base, int32_t kv_pos_base, int32_t kv_row0,
+                            double rope_base, void* q_out, void* stream) {
+    if (!c || !qkv || !q_out) return GQA_ERR_NULL;
+    if (b < 0 || b >= c->cfg.batch) return GQA_ERR_STREAM_DEST;
+    if (n_tokens < 1 || kv_row0 < 0 || (int64_t)kv_row0 + n_tokens > c->cfg.max_seq_len) return GQA_ERR_RANGE;
+    if (q_pos_base < 0 || kv_pos_base < 0 || (int64_t)q_pos_base + n_tokens > kHeadsMaxPosition ||
+        (int64_t)kv_pos_base + n_tokens > kHeadsMaxPosition)
+        return GQA_ERR_RANGE;
+    if (!rows_backed(c, b, kv_row0, n_tokens)) return GQA_ERR_RANGE;
+    HeadsArgs a{};
+    a.n_tokens = n_tokens;
+    a.b = b;
+    a.pos_base = q_pos_base;
+    a.k_pos_base = kv_pos_base;
+    a.row0 = kv_row0;
+    return run_heads(c, a, qkv, ld, q_weight, k_weight, eps, rope_base, q_out, pick_stream(c, stream));
+}
+
+int gqa_qk_norm_rope_step_device(gqa_ctx* c, const void* qkv, int64_t ld, const void* q_weight, const void* k_weight, float eps,
+                                 const int32_t* positions, const int32_t* rows, double rope_base, void* q_out, void* stream) {
+    if (!c || !qkv || !positions || !q_out) return GQA_ERR_NULL;
+    HeadsArgs a{};
+    a.n_tokens = c->cfg.batch;
+    a.positions = positions;
+    a.rows = rows;
+    return run_heads(c, a, qkv, ld, q_weight, k_weight, eps, rope_base, q_out, pick_stream(c, stream));
+}
+
+int gqa_w4_bytes(int32_t rows, int32_t hidden, int32_t group, int64_t* w_bytes, int64_t* scale_bytes) {
+    if (!w_bytes || !scale_bytes) return GQA_ERR_NULL;
+    const int rc = check_w4(rows, hidden, group);
+    if (rc != GQA_OK) return rc;
+    *w_bytes = w4_packed_bytes(rows, hidden);
+    *scale_bytes = w4_scale_bytes(rows, hidden, group);
+    return GQA_OK;
+}
+
+int gqa_w4_pack_device(gqa_ctx* c, const void* codes, const void* scales, int32_t rows, int32_t hidden, int32_t group,
+                       void* w, void* w_scales, void* stream) {
+    if (!c || !codes || !scales || !w || !w_scales) return GQA_ERR_NULL;
+    const int rc = check_w4(rows, hidden, group);
+    if (rc != GQA_OK) return rc;
+    const size_t in = (size_t)rows * hidden / 2, in_scales = (size_t)rows * (hidden / group) * 2;
+    const size_t out = w4_packed_bytes(rows, hidden), out_scales = w4_scale_bytes(rows, hidden, group);
+    if (!aligned16(w) || !aligned16(w_scales) || (reinterpret_cast<uintptr_t>(scales) & 1) || overlaps(codes, in, w, out) ||
+        overlaps(codes, in, w_scales, out_scales) || overlaps(scales, in_scales, w, out) ||
+        overlaps(scales, in_scales, w_scales, out_scales) || overlaps(w, out, w_scales, out_scales))
+        return GQA_ERR_RANGE;
+    const DeviceScope device(c->cfg.device);
+    HIP_TRY(device.status);
+    const W4PackArgs a = {(const uint8_t*)codes, (const uint16_t*)scales, rows, hidden, group, (uint32_t*)w, (uint16_t*)w_scales};
+    HIP_TRY(launch_w4_pack(a, Launch{pick_stream(c, stream)}));
+    return GQA_OK;
+}
+
+int gqa_w4_unpack_device(gqa_ctx* c, const void* w, const void* w_scales, int32_t rows, int32_t hidden, int32_t group, void* out,
+                         void* stream) {
+    if (!c || !w || !w_scales || !out) return GQA_ERR_NULL;
+    const int rc = check_w4(rows, hidden, group);
+    if (rc != GQA_OK) return rc;
+    const size_t bytes = (size_t)rows * hidden * 2;
+    if (!aligned16(w) || !aligned16(w_scales) || !aligned16(out) || overlaps(out, bytes, w, w4_packed_bytes(rows, hidden)) ||
+        overlaps(out, bytes, w_scales, w4_scale_bytes(rows, hidden, group)))
+        return GQA_ERR_RANGE;
+    const DeviceScope device(c->cfg.device);
+    HIP_TRY(device.status);
+    const W4UnpackArgs a = {(const uint32_t*)w, (const uint16_t*)w_scales, rows, hidden, group, (uint16_t*)out};
+    HIP_TRY(launch_w4_unpack(a, Launch{pick_stream(c, stream)}));
+    return GQA_OK;
+}
+
+int gqa_w4_project_device(gqa_ctx* c, const void* x, int32_t n_tokens, int32_t hidden, const void* w, const void* w_scales,
+                          int32_t group, int32_t rows, const void* rms_weight, float rms_eps, void* y, int64_t ldy, void* stream) {
+    if (!c || !x || !w || !w_scales || !y) return GQA_ERR_NULL;
+    const int rc = check_w4(rows, hidden, group);
+    if (rc != GQA_OK) return rc;
+    if (n_tokens < 1 || n_tokens > GQA_W4_MAX_TOKENS || ldy < rows) return GQA_ERR_RANGE;
+    if (!(rms_eps >= 0.f) || !isfinite(rms_eps)) return GQA_ERR_RANGE;
+    if (!aligned16(x) || !aligned16(rms_weight) || !aligned16(w) || !aligned16(w_scales) || (reinterpret_cast<uintptr_t>(y) & 1))
+        return GQA_ERR_RANGE;
+    // The kernel reads x and the weights while it writes y.
+    const size_t out = ((size_t)(n_tokens - 1) * ldy + rows) * 2;
+    if (overlaps(y, out, x, (size_t)n_tokens * hidden * 2) || overlaps(y, out, w, w4_packed_bytes(rows, hidden)) ||
+        overlaps(y, out, w_scales, w4_scale_bytes(rows, hidden, group)) ||
+        overlaps(y, out, rms_weight, rms_weight ? (size_t)hidden * 2 : 0))
+        return GQA_ERR_RANGE;
+    const DeviceScope device(c->cfg.device);
+    HIP_TRY(device.status);
+    const W4ProjectArgs a = {(const uint16_t*)x, (const uint16_t*)rms_weight, (const uint32_t*)w, (const uint16_t*)w_scales,
+                             n_tokens, hidden, group, rows, rms_eps, (uint16_t*)y, ldy};
+    HIP_TRY(launch_w4_project(a, timed(c, GQA_TIMER_PROJECTION, pick_stream(c, stream))));
     return GQA_OK;
 }
 
@@ -1988,8 +2389,8 @@ int gqa_graph_launch(gqa_graph* g, void* stream) {
     HIP_TRY(hipSetDevice(c->cfg.device));
     Launch l;
     l.stream = pick_stream(c, stream);
-    HIP_TRY(launch_decode(c->cfg.head_dim, c->group, g->args, l));
-    if (g->combine) HIP_TRY(launch_combine(c->cfg.head_dim, c->group, g->args, l));
+    HIP_TRY(launch_step(c->cfg.head_dim, c->group, g->args, l));
+    if (g->combine) HIP_TRY(launch_step_merge(c->cfg.head_dim, c->group, g->args, l));
     return GQA_OK;
 }
 
@@ -2007,14 +2408,10 @@ int gqa_start(gqa_ctx* c) {
     const Txn& t = c->txn;
     HIP_TRY(hipEventRecord(c->ev_t[1], c->stream));
     // The transaction reads the layer it was submitted on, whichever layer is active now.
-    uint16_t* const k_active = c->k_cache;
-    uint16_t* const v_active = c->v_cache;
-    c->k_cache = c->k_pool + kv_words(c) * (size_t)t.layer;
-    c->v_cache = c->v_pool + kv_words(c) * (size_t)t.layer;
+    point_at_layer(c, t.layer);
     int rc = run_prefill(c, t.b, c->q_dev, t.q_len, t.q_pos_base, t.kv_len, t.kv_pos_base, t.causal, c->o_dev,
                          nullptr, c->stream);
-    c->k_cache = k_active;
-    c->v_cache = v_active;
+    point_at_layer(c, c->layer);
     if (rc != GQA_OK) return rc;
     HIP_TRY(hipEventRecord(c->ev_t[2], c->stream));
     const size_t bytes = (size_t)c->cfg.n_q_heads * t.q_len * c->cfg.head_dim * 2;

@@ -41,13 +41,19 @@ struct Launch {
     hipEvent_t stop = nullptr;
 };
 
+// `lds`: bytes of dynamic shared memory.
+template <typename... KArgs, typename... Args>
+inline hipError_t launch_kernel_lds(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t lds, const Launch& l, Args... args) {
+    if (l.start != nullptr || l.stop != nullptr)
+        hipExtLaunchKernelGGL(kernel, grid, block, lds, l.stream, l.start, l.stop, 0, args...);
+    else
+        hipLaunchKernelGGL(kernel, grid, block, lds, l.stream, args...);
+    return hipGetLastError();
+}
+
 template <typename... KArgs, typename... Args>
 inline hipError_t launch_kernel(void (*kernel)(KArgs...), dim3 grid, dim3 block, const Launch& l, Args... args) {
-    if (l.start != nullptr || l.stop != nullptr)
-        hipExtLaunchKernelGGL(kernel, grid, block, 0, l.stream, l.start, l.stop, 0, args...);
-    else
-        hipLaunchKernelGGL(kernel, grid, block, 0, l.stream, args...);
-    return hipGetLastError();
+    return launch_kernel_lds(kernel, grid, block, 0, l, args...);
 }
 
 // Split-KV decode launch description.  All pointers are device pointers.
@@ -96,15 +102,20 @@ struct DecodeArgs {
     // launches that are a short latency chain (plan_decode_shape).  Both kernels of a plan use the
     // same count, so the in-launch merge and the merge launch fold in the same order.
     int32_t waves;
+    // E4M3 cache (k_scale != nullptr): kc and vc are rows of codes, k_scale and v_scale their scale bytes, one per row
+    // (kv8_device.h); the rows appended by the launch are quantised.  group: query heads per kv head (E4M3 kernels only).
+    uint8_t* k_scale;
+    uint8_t* v_scale;
+    int32_t group;
 };
 constexpr int kDecodeWaves = 8;
 constexpr int kDecodeWavesSmall = 4;
-// Whether a decode launch over `units` (sequence, kv head) units of at most max_len keys reads
+// Whether a decode launch over `units` (sequence, kv head) units of at most max_len keys of row_bytes each for K and V reads
 // its K/V with plain loads: when they fit the L2s of the XCDs (4 MiB each) several times over, a
 // step finds them where the last one left them.
 constexpr int64_t kDecodeCachedBytes = 24ll << 20;
-inline bool decode_cached_loads(int64_t units, int max_len, int head_dim) {
-    return units * (int64_t)max_len * head_dim * 2 * 2 <= kDecodeCachedBytes;
+inline bool decode_cached_loads(int64_t units, int max_len, int row_bytes) {
+    return units * (int64_t)max_len * row_bytes * 2 <= kDecodeCachedBytes;
 }
 
 // Chunked prefill / full-transaction launch description (one sequence b).
@@ -234,6 +245,41 @@ hipError_t launch_append(const uint16_t* k_rows, const uint16_t* v_rows, const i
                          int l_cap, int l_max, const int32_t* block_table, int page_shift, int max_pages,
                          const Launch& l);
 
+// E4M3 cache of every sequence: codes and one scale byte per row, contiguous or paged (block_table [B][max_pages]) as the
+// bf16 cache; for kv_read of a bf16 cache k and v are its words, k_scale and v_scale nullptr.
+struct Kv8Cache {
+    uint8_t* k;
+    uint8_t* v;
+    uint8_t* k_scale;
+    uint8_t* v_scale;
+    int32_t n_kv_heads, l_cap, l_max;
+    const int32_t* block_table;
+    int32_t page_shift, max_pages;
+};
+struct Kv8WriteArgs {
+    Kv8Cache cache;
+    const uint16_t* k;  // bf16 rows [H_kv][n][D] of sequence b, or [B][H_kv][D] with positions
+    const uint16_t* v;
+    int32_t b, start, n;
+    int64_t n_rows;            // rows of k (and of v)
+    const int32_t* positions;  // [B] rows to write, one per sequence (-1: none), or nullptr
+};
+struct KvReadArgs {
+    Kv8Cache cache;
+    int32_t b, start, n;
+    int64_t out_rows;  // rows per kv head of k and v
+    uint16_t* k;       // [H_kv][out_rows][D] bf16, the first n written
+    uint16_t* v;
+};
+hipError_t launch_kv8_write(int head_dim, const Kv8WriteArgs& a, const Launch& l);
+hipError_t launch_kv_read(int head_dim, const KvReadArgs& a, const Launch& l);
+
+// Decode over an E4M3 cache (DecodeArgs::k_scale): any group of up to 16 heads.
+constexpr int kKv8RoundKeys = 32;  // keys of a wave's round
+bool decode_kv8_supported(int head_dim, int group);
+hipError_t launch_decode_kv8(int head_dim, const DecodeArgs& a, const Launch& l);
+hipError_t launch_decode_kv8_merge(int head_dim, const DecodeArgs& a, const Launch& l);
+
 // Layer input stage of run_layer (sw/attn_driver.py:552-576): RMSNorm of the hidden states
 // and, after the QKV projection GEMM, RoPE plus the head-major scatter of Q and of K/V into
 // the cache.
@@ -288,6 +334,54 @@ struct FewTokensArgs {
 };
 bool few_tokens_supported(const FewTokensArgs& a, int n_cu);
 hipError_t launch_few_tokens(const FewTokensArgs& a, int n_cu, const Launch& l);
+
+// Norms of Q and K heads, RoPE and scatter in one pass (heads.hip): the tokens of one sequence (positions == nullptr) or
+// one token of each.
+struct HeadsArgs {
+    const uint16_t* x;   // [n_tokens][ld] bf16: Q heads, then K heads, then V heads, D columns each
+    int64_t ld;
+    int32_t n_tokens, n_q_heads;
+    const uint16_t* wq;  // [D] bf16 norm weights, nullptr: that side's heads are not normalised
+    const uint16_t* wk;
+    float eps;
+    double log2_base;    // of the rotation's frequencies; 0: no rotation
+    int32_t b, pos_base, k_pos_base, row0;  // one sequence: Q at pos_base + t, K at k_pos_base + t, cache rows row0 + t
+    const int32_t* positions;  // [n_tokens]: token i is sequence i's, at this position (-1: left out)
+    const int32_t* rows;       // [n_tokens] its cache row; nullptr: its position
+    uint16_t* q_out;     // [n_q_heads][n_tokens][D], with positions [n_tokens][n_q_heads][D]
+    Kv8Cache cache;      // bf16 (k_scale == nullptr) or E4M3
+};
+hipError_t launch_qk_norm_rope(int head_dim, const HeadsArgs& a, const Launch& l);
+
+// 4-bit weights (w4.hip): hidden a multiple of `group`, group 32, 64 or 128.
+struct W4PackArgs {
+    const uint8_t* codes;
+    const uint16_t* scales;
+    int32_t rows, hidden, group;
+    uint32_t* packed;
+    uint16_t* packed_scales;
+};
+struct W4UnpackArgs {
+    const uint32_t* packed;
+    const uint16_t* packed_scales;
+    int32_t rows, hidden, group;
+    uint16_t* out;
+};
+struct W4ProjectArgs {
+    const uint16_t* x;      // [n_tokens][hidden] bf16
+    const uint16_t* gamma;  // [hidden], nullptr: no norm
+    const uint32_t* w;      // packed
+    const uint16_t* scales;
+    int32_t n_tokens, hidden, group, rows;
+    float eps;
+    uint16_t* y;            // [n_tokens][ldy] bf16
+    int64_t ldy;
+};
+int64_t w4_packed_bytes(int rows, int hidden);
+int64_t w4_scale_bytes(int rows, int hidden, int group);
+hipError_t launch_w4_pack(const W4PackArgs& a, const Launch& l);
+hipError_t launch_w4_unpack(const W4UnpackArgs& a, const Launch& l);
+hipError_t launch_w4_project(const W4ProjectArgs& a, const Launch& l);
 
 // Streaming-read ceiling probe (probe.hip): reads n_bytes (a multiple of 16) at src with n_wgs
 // 512-thread work-groups, `unroll` (1, 2, 4 or 8) 16-byte nontemporal loads in flight per thread.
