@@ -89,7 +89,7 @@ struct gqa_ctx {
     int prefill_kernel = GQA_PREFILL_KERNEL_AUTO;
     float* pre_ws = nullptr;     // prefill KV-segment partials (O, then (m, l)) of launches with a forced decomposition
     float* auto_ws = nullptr;    // the same of the automatic plan's, which may be in flight beside those
-    uint16_t* zero_row = nullptr;  // one zero K/V row: the prefill source of rows past kv_len
+    uint16_t* zero_row = nullptr;  // one zero K/V row: the prefill source of rows past kv_len (E4M3: a decode round of them)
     size_t pre_ws_floats = 0, auto_ws_floats = 0;
     bool auto_ws_bound = false;    // the stream whose automatically segmented launches use it, and another that
     hipStream_t auto_ws_stream = nullptr;  // has asked for it since (take_auto_ws); only compared: it may be gone
@@ -323,9 +323,9 @@ struct DecodeShape {
 };
 
 DecodeShape plan_decode_shape(int batch, int n_kv_heads, int group, int head_dim, int n_cu, int max_len,
-                              int chunk_opt, int merge_option, bool kv8 = false) {
+                              int chunk_opt, int merge_option) {
     const int64_t units = (int64_t)batch * n_kv_heads;
-    const int round_keys = kv8 ? kKv8RoundKeys : decode_round_keys(group), row_bytes = kv8 ? head_dim : 2 * head_dim;
+    const int round_keys = decode_round_keys(group), row_bytes = 2 * head_dim;
     auto in_chunks = [&](int chunk, int waves) {
         const int splits = decode_split_count(max_len, chunk);
         return DecodeShape{chunk, splits, waves, fuse_merge(merge_option, (int)units, splits, n_cu)};
@@ -353,6 +353,42 @@ DecodeShape plan_decode_shape(int batch, int n_kv_heads, int group, int head_dim
     const bool take = s.fused && s.chunk <= (group > 8 ? kFusedPlanKeysWide : kFusedPlanKeys) &&
                       !(plain.fused && s.chunk <= plain.chunk);
     return take ? s : plain;
+}
+
+// A decode launch over an E4M3 cache: pieces of 2^chunk_log2 keys, a work-group each (splits > 0: at most so many of a
+// (sequence, kv head)) or shared out over `runs` work-groups.
+struct Kv8Shape {
+    int chunk_log2;
+    int splits;
+    int runs;
+    bool fused;  // partials merged in-launch
+};
+
+constexpr int kKv8Partials = 16;  // per CU: two for each run, or one for each piece
+constexpr int kKv8MaxBatch = 65535;  // of a direct launch (its grid)
+
+Kv8Shape plan_kv8(int batch, int n_kv_heads, int head_dim, int n_cu, int max_len, int chunk_opt, int merge_option) {
+    const int64_t units = (int64_t)batch * n_kv_heads;
+    auto log2_up = [](int keys) {
+        int l = 0;
+        while ((1 << l) < keys) ++l;
+        return std::max(l, 8);
+    };
+    static_assert(kKv8Piece == 1 << 8, "the smallest piece");
+    auto direct = [&](int chunk_log2) {
+        const int splits = decode_split_count(max_len, 1 << chunk_log2);
+        return Kv8Shape{chunk_log2, splits, 0,
+                        splits > 1 && (merge_option == GQA_DECODE_MERGE_FUSED ||
+                                       (merge_option == GQA_DECODE_MERGE_AUTO && 2 * units * splits <= n_cu))};
+    };
+    auto fits = [&](const Kv8Shape& s) { return units * s.splits <= (int64_t)kKv8Partials * n_cu && batch <= kKv8MaxBatch; };
+    if (chunk_opt > 0) {
+        const Kv8Shape s = direct(log2_up(chunk_opt));
+        if (fits(s)) return s;
+    }
+    const Kv8Shape s = direct(8);
+    if (fits(s) && units * s.splits <= n_cu) return s;
+    return Kv8Shape{8, 0, 2 * n_cu, false};
 }
 
 constexpr int kProfileLaunches = 512;  // event pairs kept per timer slot
@@ -402,11 +438,7 @@ int plan_decode(gqa_ctx* c, const void* q, const int32_t* lens, const void* k_ne
     if (!(c->kv8 ? decode_kv8_supported(c->cfg.head_dim, c->group) : decode_supported(c->cfg.head_dim, c->group)) ||
         c->numerics != GQA_NUMERICS_EXACT)
         return GQA_ERR_UNSUPPORTED;
-    const DecodeShape shape = plan_decode_shape(c->cfg.batch, c->cfg.n_kv_heads, c->group, c->cfg.head_dim, c->n_cu,
-                                                max_len, c->chunk_opt, c->decode_merge, c->kv8);
-    const int chunk = shape.chunk;
-    const int max_splits = shape.max_splits;
-    if (max_splits > c->max_splits_cap) return GQA_ERR_RANGE;
+    const int64_t units = (int64_t)c->cfg.batch * c->cfg.n_kv_heads;
     DecodeArgs& a = *out;
     a = DecodeArgs{};
     a.q = (const uint16_t*)q;
@@ -420,8 +452,6 @@ int plan_decode(gqa_ctx* c, const void* q, const int32_t* lens, const void* k_ne
     a.n_kv_heads = c->cfg.n_kv_heads;
     a.l_cap = c->l_cap;
     a.l_max = c->cfg.max_seq_len;
-    a.chunk = chunk;
-    a.max_splits = max_splits;
     a.scale_log2 = c->scale * 1.4426950408889634f;
     a.part_o = c->part_o;
     a.part_ml = c->part_ml;
@@ -432,14 +462,30 @@ int plan_decode(gqa_ctx* c, const void* q, const int32_t* lens, const void* k_ne
     a.max_pages = c->max_pages;
     a.zero_row = c->zero_row;
     a.longest_first = c->cfg.batch > 1;
-    a.cached = decode_cached_loads((int64_t)c->cfg.batch * c->cfg.n_kv_heads, max_len, c->cfg.head_dim * kv_value_bytes(c)) ? 1 : 0;
-    a.k_scale = c->k_scale;
-    a.v_scale = c->v_scale;
-    a.group = c->group;
+    a.cached = decode_cached_loads(units, max_len, c->cfg.head_dim * kv_value_bytes(c)) ? 1 : 0;
+    if (c->kv8) {
+        const Kv8Shape shape = plan_kv8(c->cfg.batch, c->cfg.n_kv_heads, c->cfg.head_dim, c->n_cu, max_len, c->chunk_opt,
+                                        c->decode_merge);
+        a.k_scale = c->k_scale;
+        a.v_scale = c->v_scale;
+        a.group = c->group;
+        a.chunk = 1 << shape.chunk_log2;
+        a.chunk_log2 = shape.chunk_log2;
+        a.max_splits = shape.splits;
+        a.runs = shape.runs;
+        a.arrivals = shape.fused ? c->arrivals : nullptr;
+        *combine = !shape.fused && shape.splits != 1;
+        return GQA_OK;
+    }
+    const DecodeShape shape = plan_decode_shape(c->cfg.batch, c->cfg.n_kv_heads, c->group, c->cfg.head_dim, c->n_cu,
+                                                max_len, c->chunk_opt, c->decode_merge);
+    if (shape.max_splits > c->max_splits_cap) return GQA_ERR_RANGE;
+    a.chunk = shape.chunk;
+    a.max_splits = shape.max_splits;
     a.waves = shape.waves;
     a.arrivals = shape.fused ? c->arrivals : nullptr;
-    *combine = max_splits > 1 && a.arrivals == nullptr;
-    a.ticket = (c->cfg.batch > 1 && max_splits == 1) ? c->arrivals + (size_t)c->cfg.batch * c->cfg.n_kv_heads : nullptr;
+    *combine = shape.max_splits > 1 && a.arrivals == nullptr;
+    a.ticket = (c->cfg.batch > 1 && shape.max_splits == 1) ? c->arrivals + units : nullptr;
     return GQA_OK;
 }
 
@@ -1257,8 +1303,9 @@ int create_ctx(const gqa_config* cfg, int32_t page_size, int32_t n_pages, int32_
         alloc((void**)&c->v_scale_pool, kv_rows(c) * (size_t)n_layers);
     }
     point_at_layer(c, 0);
-    alloc((void**)&c->part_o, units * c->max_splits_cap * group * D * sizeof(float));
-    alloc((void**)&c->part_ml, units * c->max_splits_cap * group * 2 * sizeof(float));
+    const size_t partials = (kv8 ? (size_t)kKv8Partials * c->n_cu : units * c->max_splits_cap) * group;
+    alloc((void**)&c->part_o, partials * D * sizeof(float));
+    alloc((void**)&c->part_ml, partials * 2 * sizeof(float));
     alloc((void**)&c->arrivals, (units + 1) * sizeof(int32_t));
     if (prefill_supported(k.head_dim, group)) {
         if (k.max_seq_len > kAutoSegmentKeys) c->auto_ws_floats = prefill_workspace_need(c, c->n_cu);
@@ -1268,7 +1315,8 @@ int create_ctx(const gqa_config* cfg, int32_t page_size, int32_t n_pages, int32_
     alloc((void**)&c->o_dev, c->stage_words * 2);
     alloc((void**)&c->lse_dev, c->lse_words * sizeof(float));
     alloc((void**)&c->lens_dev, (size_t)k.batch * sizeof(int32_t));
-    alloc((void**)&c->zero_row, D * 2);
+    const size_t zero_bytes = kv8 ? kKv8RoundKeys * D : D * 2;
+    alloc((void**)&c->zero_row, zero_bytes);
     alloc((void**)&c->pos_dev, (size_t)k.batch * sizeof(int32_t));
     alloc((void**)&c->rows_dev, 2 * units * D * 2);
     alloc((void**)&c->new_dev, 2 * (size_t)k.n_kv_heads * k.max_q_len * D * 2);
@@ -1287,7 +1335,7 @@ int create_ctx(const gqa_config* cfg, int32_t page_size, int32_t n_pages, int32_
         if (!ok) rc = GQA_ERR_HIP;
     }
     // Zero the caches (every layer's pool) once so rows beyond every sequence's length hold finite words.
-    if (rc == GQA_OK && (hipMemsetAsync(c->zero_row, 0, D * 2, c->stream) != hipSuccess ||
+    if (rc == GQA_OK && (hipMemsetAsync(c->zero_row, 0, zero_bytes, c->stream) != hipSuccess ||
                          hipMemsetAsync(c->arrivals, 0, (units + 1) * sizeof(int32_t), c->stream) != hipSuccess ||
                          hipMemsetAsync(c->k_pool, 0, kv_bytes(c) * (size_t)n_layers, c->stream) != hipSuccess ||
                          hipMemsetAsync(c->v_pool, 0, kv_bytes(c) * (size_t)n_layers, c->stream) != hipSuccess ||

@@ -103,10 +103,14 @@ struct DecodeArgs {
     // same count, so the in-launch merge and the merge launch fold in the same order.
     int32_t waves;
     // E4M3 cache (k_scale != nullptr): kc and vc are rows of codes, k_scale and v_scale their scale bytes, one per row
-    // (kv8_device.h); the rows appended by the launch are quantised.  group: query heads per kv head (E4M3 kernels only).
+    // (kv8_device.h), zero_row is kKv8RoundKeys rows of zeros; the rows appended by the launch are quantised.  group: query heads per kv head (E4M3 kernels only).
     uint8_t* k_scale;
     uint8_t* v_scale;
+    // `chunk` is a power of two here: the keys of a piece.  max_splits > 0: a work-group per piece; 0: the pieces are shared
+    // out over `runs` work-groups (decode_kv8.hip), and part_o and part_ml are [runs][2][G].
     int32_t group;
+    int32_t chunk_log2;
+    int32_t runs;
 };
 constexpr int kDecodeWaves = 8;
 constexpr int kDecodeWavesSmall = 4;
@@ -275,7 +279,8 @@ hipError_t launch_kv8_write(int head_dim, const Kv8WriteArgs& a, const Launch& l
 hipError_t launch_kv_read(int head_dim, const KvReadArgs& a, const Launch& l);
 
 // Decode over an E4M3 cache (DecodeArgs::k_scale): any group of up to 16 heads.
-constexpr int kKv8RoundKeys = 32;  // keys of a wave's round
+constexpr int kKv8RoundKeys = 64;  // keys of a wave's round, at most
+constexpr int kKv8Piece = 256;     // the smallest piece: a round of each wave
 bool decode_kv8_supported(int head_dim, int group);
 hipError_t launch_decode_kv8(int head_dim, const DecodeArgs& a, const Launch& l);
 hipError_t launch_decode_kv8_merge(int head_dim, const DecodeArgs& a, const Launch& l);
