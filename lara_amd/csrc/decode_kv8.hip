@@ -48,7 +48,7 @@ typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kMergeParts = 4;   // a head's partials are summed as s % 4 apart, then these four in order
-constexpr int kMergeBatch8 = 8;  // partials in flight of one part
+constexpr int kPartBatch = 4;  // partials in flight of one part
 
 __device__ __forceinline__ f32x4 mfma_bf16(const u32x4& a, const u32x4& b, const f32x4& c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c,
@@ -166,18 +166,18 @@ struct Partials {
 
 // ---- partials ------------------------------------------------------------------------------------------
 
-// Sums part `part` (partials part, part + 4, ...) of head g: D / 4 lanes, four dims each, at most kMergeBatch8 partials
+// Sums part `part` (partials part, part + 4, ...) of head g: D / 4 lanes, four dims each, at most kPartBatch partials
 // per memory round trip.  (M, L) and O against the part's own maximum.
 template <int D>
 __device__ __forceinline__ void merge_part(const DecodeArgs& a, const Partials& from, int g, int part, float2* ml_out, f32x4* o_out) {
     const int e = threadIdx.x % (D / 4);
     float M = -INFINITY, L = 0.f;
     f32x4 O = {0.f, 0.f, 0.f, 0.f};
-    for (int s0 = part; s0 < from.n; s0 += kMergeParts * kMergeBatch8) {
-        f32x4 o[kMergeBatch8];
-        float2 w[kMergeBatch8];
+    for (int s0 = part; s0 < from.n; s0 += kMergeParts * kPartBatch) {
+        f32x4 o[kPartBatch];
+        float2 w[kPartBatch];
 #pragma unroll
-        for (int j = 0; j < kMergeBatch8; ++j) {
+        for (int j = 0; j < kPartBatch; ++j) {
             const int s = s0 + j * kMergeParts;
             w[j] = make_float2(-INFINITY, 0.f);
             o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -189,13 +189,13 @@ __device__ __forceinline__ void merge_part(const DecodeArgs& a, const Partials& 
         }
         float m = M;
 #pragma unroll
-        for (int j = 0; j < kMergeBatch8; ++j) m = fmaxf(m, w[j].x);
+        for (int j = 0; j < kPartBatch; ++j) m = fmaxf(m, w[j].x);
         if (m == -INFINITY) continue;  // no valid key in these
         const float corr = fast_exp2(M - m);  // 0 while M = -inf
         L *= corr;
         O *= corr;
 #pragma unroll
-        for (int j = 0; j < kMergeBatch8; ++j) {
+        for (int j = 0; j < kPartBatch; ++j) {
             const float f = fast_exp2(w[j].x - m);  // 0 past the last
             L = fmaf(f, w[j].y, L);
 #pragma unroll
@@ -257,7 +257,7 @@ struct Segment {
 constexpr int kv8_waves(bool direct) { return direct ? 8 : 4; }
 
 template <int D, bool DIRECT, bool PAGED, bool CACHED>
-__global__ __launch_bounds__(kv8_waves(DIRECT) * 64, 2) void decode_kv8_kernel(DecodeArgs a) {
+__global__ __launch_bounds__(kv8_waves(DIRECT) * 64, DIRECT ? 4 : 2) void decode_kv8_kernel(DecodeArgs a) {
     constexpr int NW = kv8_waves(DIRECT), RK = kKv8Piece / NW;
     constexpr int CH = D / 64;   // 16-byte chunks of a K row per lane; words of V codes per lane and key in the product
     constexpr int VB = D / 16;   // V codes per lane and key, O tiles

@@ -366,6 +366,8 @@ struct Kv8Shape {
 
 constexpr int kKv8Partials = 16;  // per CU: two for each run, or one for each piece
 constexpr int kKv8MaxBatch = 65535;  // of a direct launch (its grid)
+constexpr double kKv8WholeUnits = 0.5, kKv8DirectUnits = 0.25;  // (sequence, kv head) units per CU
+constexpr int64_t kKv8WholeBytes = 640 << 10;
 
 Kv8Shape plan_kv8(int batch, int n_kv_heads, int head_dim, int n_cu, int max_len, int chunk_opt, int merge_option) {
     const int64_t units = (int64_t)batch * n_kv_heads;
@@ -386,8 +388,16 @@ Kv8Shape plan_kv8(int batch, int n_kv_heads, int head_dim, int n_cu, int max_len
         const Kv8Shape s = direct(log2_up(chunk_opt));
         if (fits(s)) return s;
     }
-    const Kv8Shape s = direct(8);
-    if (fits(s) && units * s.splits <= n_cu) return s;
+    const int64_t unit_bytes = (int64_t)max_len * head_dim * 2;
+    const bool whole = unit_bytes <= (units >= kKv8WholeUnits * n_cu ? kKv8WholeBytes
+                                      : units >= kUnsplitUnits       ? 2 * kDecodeSplitMinBytes
+                                                                     : kDecodeSplitMinBytes);
+    if (whole || units <= kKv8DirectUnits * n_cu) {
+        int l = whole ? log2_up(max_len) : 8;
+        while (!whole && units * decode_split_count(max_len, 1 << l) > n_cu) ++l;
+        const Kv8Shape s = direct(l);
+        if (fits(s)) return s;
+    }
     return Kv8Shape{8, 0, 2 * n_cu, false};
 }
 
