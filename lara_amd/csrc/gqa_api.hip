@@ -2413,7 +2413,7 @@ int gqa_w4_project_device(gqa_ctx* c, const void* x, int32_t n_tokens, int32_t h
     HIP_TRY(device.status);
     const W4ProjectArgs a = {(const uint16_t*)x, (const uint16_t*)rms_weight, (const uint32_t*)w, (const uint16_t*)w_scales,
                              n_tokens, hidden, group, rows, rms_eps, (uint16_t*)y, ldy};
-    HIP_TRY(launch_w4_project(a, timed(c, GQA_TIMER_PROJECTION, pick_stream(c, stream))));
+    HIP_TRY(launch_w4_project(a, c->n_cu, timed(c, GQA_TIMER_PROJECTION, pick_stream(c, stream))));
     return GQA_OK;
 }
 

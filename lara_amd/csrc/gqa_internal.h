@@ -386,7 +386,7 @@ int64_t w4_packed_bytes(int rows, int hidden);
 int64_t w4_scale_bytes(int rows, int hidden, int group);
 hipError_t launch_w4_pack(const W4PackArgs& a, const Launch& l);
 hipError_t launch_w4_unpack(const W4UnpackArgs& a, const Launch& l);
-hipError_t launch_w4_project(const W4ProjectArgs& a, const Launch& l);
+hipError_t launch_w4_project(const W4ProjectArgs& a, int n_cu, const Launch& l);
 
 // Streaming-read ceiling probe (probe.hip): reads n_bytes (a multiple of 16) at src with n_wgs
 // 512-thread work-groups, `unroll` (1, 2, 4 or 8) 16-byte nontemporal loads in flight per thread.

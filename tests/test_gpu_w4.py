@@ -88,6 +88,32 @@ def test_project_against_float64(acc, group, n, rows, hidden):
         assert np.all(got[n:] == 7) and np.all(got[:, rows:] == 7)  # what is not y is as it was
 
 
+@pytest.mark.parametrize("n,rows,hidden,group", [(1, 5200, 256, 32), (16, 5187, 160, 32), (5, 5200, 384, 128), (3, 10250, 128, 64),
+                                                 (16, 10250, 288, 32), (33, 5203, 288, 32), (64, 5200, 192, 64),
+                                                 (47, 5200, 1152, 128), (40, 10241, 96, 32)])
+def test_many_rows_take_several_tiles_a_work_group(acc, n, rows, hidden, group):
+    """Against float64, and a token alone and among others gives the same words."""
+    rng = np.random.default_rng(n + rows + hidden)
+    codes, scales = matrix(rng, rows, hidden, group)
+    w, s = packed(acc, codes, scales, group)
+    x = bf16_normal(rng, (n, hidden))
+    gamma = orc.bf16_rne((1 + 0.2 * rng.standard_normal(hidden)).astype(np.float32))
+    xd, gd = dev(x), dev(gamma)
+    for g in (None, gamma):
+        y = torch.full((n + 1, rows + 1), 7, dtype=torch.int16, device="cuda")
+        gp = gd.data_ptr() if g is not None else None
+        acc.w4_project_device(xd.data_ptr(), n, hidden, w.data_ptr(), s.data_ptr(), group, rows, y.data_ptr(), rms_weight_ptr=gp,
+                              rms_eps=1e-5, ldy=rows + 1)
+        last = torch.zeros(96, dtype=torch.int16, device="cuda")  # (the first 96 rows alone: another form of the kernel)
+        acc.w4_project_device(xd[n - 1 :].data_ptr(), 1, hidden, w.data_ptr(), s.data_ptr(), group, 96, last.data_ptr(),
+                              rms_weight_ptr=gp, rms_eps=1e-5)
+        torch.cuda.synchronize()
+        got = words(y)
+        check(got[:n, :rows], x, g, 1e-5, codes, scales)
+        assert np.all(got[n:] == 7) and np.all(got[:, rows:] == 7)
+        assert torch.equal(last, y[n - 1, :96])
+
+
 @pytest.mark.parametrize("hidden,group", [(160, 32), (96, 32), (192, 64), (2080, 32)])
 def test_hidden_that_ends_inside_a_block(acc, hidden, group):
     rng = np.random.default_rng(hidden)
