@@ -231,6 +231,166 @@ def test_decode_of_a_large_ragged_batch_takes_every_row_once():
             assert np.array_equal(o, first[0]) and np.array_equal(lse, first[1])
 
 
+@pytest.mark.parametrize("hq,hkv,d,L", [(8, 4, 64, 2112), (4, 4, 64, 2112), (64, 4, 64, 2112), (20, 4, 128, 1088), (32, 4, 128, 1088)])
+@pytest.mark.parametrize("page", [None, 64])
+def test_decode_in_equal_runs_against_float64(hq, hkv, d, L, page):
+    """Batches that share their keys out in equal runs: lengths around pieces' and rounds' ends, rows appended at the end,
+    inside and past what is attended, idle slots; repeated steps give the same words."""
+    rng = np.random.default_rng(hq * 100 + d)
+    lens = [0, 1, 2, 63, 64, 65, 255, 256, 257, 320, 321, 384, 511, 513, 576, 577, 800, 1023, L - 1, L]
+    B = len(lens)
+    with engine(batch=B, n_q_heads=hq, n_kv_heads=hkv, head_dim=d, max_seq_len=L, page_size=page) as acc:
+        if page:
+            scatter_reserve(acc, [max(1, n) for n in lens], page)
+        k, v = rows(rng, (B, hkv, L, d)), rows(rng, (B, hkv, L, d))
+        for b, n in enumerate(lens):
+            if n:
+                acc.load_kv(k[b, :, :n], v[b, :, :n], b=b)
+        q = bf16_normal(rng, (B, hq, d))
+        first = acc.decode_step(q, lens, return_lse=True)
+        for b, n in enumerate(lens):
+            close(first[0][b], first[1][b], so.decode(f64(q[b]), so.stored(f64(k[b, :, :n])), so.stored(f64(v[b, :, :n])), acc.scale))
+        for _ in range(3):
+            again = acc.decode_step(q, lens, return_lse=True)
+            assert np.array_equal(again[0], first[0]) and np.array_equal(again[1], first[1])
+        pos, attended = np.array([n - 1 for n in lens], np.int32), list(lens)
+        pos[7], pos[8], pos[16] = 100, -1, 0
+        attended[18] = 700  # (its row, the last of the cache, is stored but not attended)
+        kr, vr = rows(rng, (B, hkv, d), 2.0), rows(rng, (B, hkv, d), 2.0)
+        o, lse = acc.decode_step(q, attended, k_rows=kr, v_rows=vr, positions=pos, return_lse=True)
+        for b, n in enumerate(attended):
+            if pos[b] >= 0:
+                k[b, :, pos[b]], v[b, :, pos[b]] = kr[b], vr[b]
+            close(o[b], lse[b], so.decode(f64(q[b]), so.stored(f64(k[b, :, :n])), so.stored(f64(v[b, :, :n])), acc.scale))
+            if lens[b]:
+                kg, vg = acc.read_kv(b, 0, lens[b])
+                assert np.array_equal(f64(kg), so.stored(f64(k[b, :, : lens[b]])))
+                assert np.array_equal(f64(vg), so.stored(f64(v[b, :, : lens[b]])))
+
+
+@pytest.mark.parametrize("full", [(), (3,), tuple(range(150))])
+def test_decode_in_equal_runs_of_many_sequences(full):
+    """More sequences than a work-group has lanes; next to no work, one long sequence, all of them long."""
+    rng = np.random.default_rng(31)
+    B, L, d = 150, 2624, 128
+    lens = rng.integers(0, 40, B)
+    lens[list(full)] = L if len(full) == 1 else rng.integers(200, 700, len(full))
+    with engine(batch=B, n_q_heads=4, n_kv_heads=1, head_dim=d, max_seq_len=L) as acc:
+        kv = {}
+        for b in range(B):
+            kv[b] = rows(rng, (1, int(lens[b]), d)), rows(rng, (1, int(lens[b]), d))
+            if lens[b]:
+                acc.load_kv(*kv[b], b=b)
+        q = bf16_normal(rng, (B, 4, d))
+        # (the host's step plans for the longest length given, the device's for the cache: both are taken)
+        o, lse = acc.decode_step(q, lens, return_lse=True)
+        qd, ld = dev(q), dev(lens.astype(np.int32))
+        od, lsed = torch.empty((B, 4, d), dtype=torch.int16, device="cuda"), torch.empty((B, 4), device="cuda")
+        call("gqa_decode_device", acc._ctx, ptr(qd), ptr(ld), ptr(od), ptr(lsed), None)
+        torch.cuda.synchronize()
+        for b, n in enumerate(lens):
+            ref = so.decode(f64(q[b]), so.stored(f64(kv[b][0])), so.stored(f64(kv[b][1])), acc.scale)
+            close(o[b], lse[b], ref)
+            close(words(od)[b], lsed.cpu().numpy()[b], ref)
+
+
+@pytest.mark.parametrize("batch,L", [(18, 1 << 18), (2, 2400000)])
+@pytest.mark.parametrize("page", [None, 64])
+def test_rows_past_4_gib_of_a_cache(batch, L, page):
+    """K and V of over 2^32 bytes each: rows of the last sequence, written, read, appended and attended to."""
+    rng = np.random.default_rng(32)
+    hq, hkv, d, n = 16, 8, 128, 1500
+    with engine(batch=batch, n_q_heads=hq, n_kv_heads=hkv, head_dim=d, max_seq_len=L, page_size=page) as acc:
+        if page:
+            for b in range(batch):
+                acc.reserve(b, L if b < batch - 1 else n + 1)
+        b = batch - 1
+        k, v = rows(rng, (hkv, n + 1, d)), rows(rng, (hkv, n + 1, d))
+        acc.load_kv(k[:, :n], v[:, :n], b=b)
+        lens, pos = np.zeros(batch, np.int32), np.full(batch, -1, np.int32)
+        lens[b], pos[b] = n + 1, n
+        q = bf16_normal(rng, (batch, hq, d))
+        kr, vr = rows(rng, (batch, hkv, d)), rows(rng, (batch, hkv, d))
+        kr[b], vr[b] = k[:, n], v[:, n]
+        t = [dev(x) for x in (q, kr, vr, pos, lens)]
+        o, lse = torch.empty((batch, hq, d), dtype=torch.int16, device="cuda"), torch.empty((batch, hq), device="cuda")
+        call("gqa_decode_append_device", acc._ctx, *[ptr(x) for x in t], ptr(o), ptr(lse), None)
+        torch.cuda.synchronize()
+        close(words(o)[b], lse[b].cpu().numpy(), so.decode(f64(q[b]), so.stored(f64(k)), so.stored(f64(v)), acc.scale))
+        kg, vg = acc.read_kv(b, 0, n + 1)
+        assert np.array_equal(f64(kg), so.stored(f64(k))) and np.array_equal(f64(vg), so.stored(f64(v)))
+        assert not np.any(acc.read_kv(0, 0, 300)[0])  # (what the low 32 bits of their places would have hit)
+
+
+@pytest.mark.parametrize("page", [None, 64])
+def test_two_engines_on_two_streams_at_once(page):
+    rng = np.random.default_rng(33)
+    B, L = 24, 1600
+    kw = dict(batch=B, n_q_heads=16, n_kv_heads=4, head_dim=128, max_seq_len=L, page_size=page)
+    with engine(**kw) as x, engine(**kw) as y:
+        sides = []
+        for eng in (x, y):
+            lens = rng.integers(1, L, B)
+            if page:
+                scatter_reserve(eng, list(lens), page)
+            for b in range(B):
+                eng.load_kv(rows(rng, (4, lens[b], 128)), rows(rng, (4, lens[b], 128)), b=b)
+            q, n = dev(bf16_normal(rng, (B, 16, 128))), dev(lens.astype(np.int32))
+            o = [torch.zeros((B, 16, 128), dtype=torch.int16, device="cuda") for _ in range(9)]
+            call("gqa_decode_device", eng._ctx, ptr(q), ptr(n), ptr(o[8]), None, None)
+            sides.append((eng, q, n, o, torch.cuda.Stream()))
+        torch.cuda.synchronize()
+        for i in range(8):
+            for eng, q, n, o, stream in sides:
+                call("gqa_decode_device", eng._ctx, ptr(q), ptr(n), ptr(o[i]), None, ctypes.c_void_p(stream.cuda_stream))
+        torch.cuda.synchronize()
+        for _, _, _, o, _ in sides:
+            assert torch.count_nonzero(o[8]) and all(torch.equal(t, o[8]) for t in o[:8])
+
+
+def test_equal_runs_in_a_captured_graph():
+    """Lengths, positions and rows that change between replays; every replay against the eager step."""
+    rng = np.random.default_rng(34)
+    B, hkv, L, d = 20, 4, 1600, 128
+    kw = dict(batch=B, n_q_heads=16, n_kv_heads=hkv, head_dim=d, max_seq_len=L)
+    with engine(**kw) as a, engine(**kw) as e:
+        start = rng.integers(0, 1500, B)
+        for b in range(B):
+            if start[b]:
+                k, v = rows(rng, (hkv, start[b], d)), rows(rng, (hkv, start[b], d))
+                a.load_kv(k, v, b=b)
+                e.load_kv(k, v, b=b)
+        lens = dev(start.astype(np.int32))
+        buf = [dict(q=torch.zeros((B, 16, d), dtype=torch.int16, device="cuda"), k=torch.zeros((B, hkv, d), dtype=torch.int16, device="cuda"),
+                    v=torch.zeros((B, hkv, d), dtype=torch.int16, device="cuda"), pos=lens - 1, lens=lens.clone(),
+                    o=torch.zeros((B, 16, d), dtype=torch.int16, device="cuda"), lse=torch.zeros((B, 16), device="cuda")) for _ in range(2)]
+
+        def args(t):
+            return [ptr(t[n]) for n in ("q", "k", "v", "pos", "lens", "o", "lse")]
+
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            call("gqa_decode_append_device", a._ctx, *args(buf[0]), ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+        for step in range(6):
+            for name, t in (("q", bf16_normal(rng, (B, 16, d))), ("k", rows(rng, (B, hkv, d))), ("v", rows(rng, (B, hkv, d)))):
+                for t_buf in buf:
+                    t_buf[name].copy_(dev(t))
+            idle = int(rng.integers(0, B))
+            for t_buf in buf:
+                t_buf["pos"] += 1
+                t_buf["lens"] += 1
+                t_buf["lens"][idle] = 0
+                t_buf["pos"][idle] = -1
+            _ = torch.randn(256, 256, device="cuda") @ torch.randn(256, 256, device="cuda")
+            torch.cuda.synchronize()
+            graph.replay()
+            call("gqa_decode_append_device", e._ctx, *args(buf[1]), None)
+            torch.cuda.synchronize()
+            assert torch.equal(buf[0]["o"], buf[1]["o"]) and torch.equal(buf[0]["lse"], buf[1]["lse"])
+            assert torch.all(torch.isneginf(buf[0]["lse"][idle])) and not torch.any(buf[0]["o"][idle])
+
+
 def test_decode_extremes():
     """A dominating key, equal keys, values of very different scales, NaN in rows that are not attended, a key whose scale
     byte is the smallest."""
