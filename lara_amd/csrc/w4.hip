@@ -123,11 +123,11 @@ __device__ __forceinline__ float w4_row_add(float v) {
 // A block's turn: the tokens' columns, loaded a turn ahead as whole lines (a lane has 8 columns of every fourth token), take
 // gamma and go to LDS as operand B; nobody else reads these columns, so no barrier.  Straight from memory, operand B
 // would be 16 rows at a stride a load and gamma the same 4 loads again, each multiplied in all 16 columns however few
-// tokens there are: 13 tokens x 4096 -> 6144 took 10.5 us for 8.8, one token 9.1 for 6.6.  Codes and scales come
+// tokens there are: 13 tokens x 4096 -> 6144 took 10.5 us for 8.8, one token 9.1 for 7.0.  Codes and scales come
 // straight from memory, also a turn ahead.  (Tokens that stay in LDS for the whole launch, work-groups going from tile to
 // tile: 6.9 us for one token, 14.4 for 13, where every work-group's copy of the tokens is what it waits for.)
 //
-// What bounds it: at one token the weights' latency (4096 -> 6144, group 128, 13 MB: 6.6 us alone, 4.0 with other launches
+// What bounds it: at one token the weights' latency (4096 -> 6144, group 128, 13 MB: 7.0 us alone, 4.0 with other launches
 // beside it, of which about 2.7 are the launch; 1.9 us at the copy rate).  From 16 tokens on the unpacking of codes (7
 // vector instructions for 8 codes a lane, used for 16 NT tokens) and the tokens' own way to every work-group.
 //
@@ -168,7 +168,7 @@ __global__ __launch_bounds__(kW4Waves * 64, NT * RT <= 2 && SPG == 4 ? 4 : 2) vo
         const int token = 4 * u + quarter;
         x[u] = (uint32_t)(token < tokens ? token : tokens - 1) * a.hidden;
     }
-    // Blocks past the last are the last one again, not used; columns past the matrix are the first, as zeros.
+    // Blocks past the last are the last one again, not used; for columns past the matrix stand the first (scale 0).
     auto load_x = [&](Tokens& b, int i) __attribute__((always_inline)) {
         const int kb = wave + kW4Waves * i, k = (kb < blocks ? kb : blocks - 1) * 128 + 8 * col, from = k < a.hidden ? k : 0;
 #pragma unroll
@@ -207,16 +207,19 @@ __global__ __launch_bounds__(kW4Waves * 64, NT * RT <= 2 && SPG == 4 ? 4 : 2) vo
 #pragma unroll
         for (int u = 0; u < 4 * NT; ++u) {
             if (4 * u >= tokens) break;
-            u32x4 v = inside ? b.x[u] : u32x4{};
+            u32x4 v = b.x[u];
             if constexpr (NORM) {
+                float sum = squares[u];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
+                    const bf16x2_t two = __builtin_bit_cast(bf16x2_t, (uint32_t)v[j]);
+                    sum = __builtin_amdgcn_fdot2_f32_bf16(two, two, sum, false);
                     const float lo = __uint_as_float(v[j] << 16), hi = __uint_as_float(v[j] & 0xFFFF0000u);
-                    squares[u] = fmaf(hi, hi, fmaf(lo, lo, squares[u]));
                     const bf16x2_t pair = {(__bf16)(lo * __uint_as_float(b.gamma[j] << 16)),
                                            (__bf16)(hi * __uint_as_float(b.gamma[j] & 0xFFFF0000u))};
                     v[j] = __builtin_bit_cast(uint32_t, pair);
                 }
+                squares[u] = inside ? sum : squares[u];
             }
             xw[4 * u * kXRow] = v;
         }

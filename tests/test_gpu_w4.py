@@ -127,6 +127,22 @@ def test_hidden_that_ends_inside_a_block(acc, hidden, group):
     check(words(y), x, None, 0.0, codes, scales)
 
 
+def test_norm_of_small_and_large_tokens(acc):
+    """Tokens whose squares leave the normal range of fp32: their mean is subnormal (2^-21 of it at 2^-128), or near the top.
+    x * gamma is 2^-64 and 2^60 here, so the products and their sums stay normal."""
+    rng = np.random.default_rng(7)
+    codes, scales = matrix(rng, 48, 256, 64)
+    w, s = packed(acc, codes, scales, 64)
+    x = orc.bf16_rne((f64(bf16_normal(rng, (6, 256))) * np.array([2.0**-64, 2.0**60, 1, 2.0**-40, 2.0**-64, 2.0**-63])[:, None]).astype(np.float32))
+    gamma = orc.bf16_rne(2.0 ** rng.integers(-3, 4, 256).astype(np.float32))
+    xd, gd = dev(x), dev(gamma)
+    for n in (6, 1):
+        y = torch.zeros((n, 48), dtype=torch.int16, device="cuda")
+        acc.w4_project_device(xd.data_ptr(), n, 256, w.data_ptr(), s.data_ptr(), 64, 48, y.data_ptr(), rms_weight_ptr=gd.data_ptr(), rms_eps=0.0)
+        torch.cuda.synchronize()
+        check(words(y), x[:n], gamma, 0.0, codes, scales, exact_gamma=True)
+
+
 def test_unpacked_matrix_is_exactly_rounded(acc):
     rng = np.random.default_rng(5)
     for rows, hidden, group in ((33, 288, 32), (64, 256, 128), (7, 64, 64)):
