@@ -53,13 +53,14 @@ extern "C" {
 #define GQA_STATUS_ERROR       (1u << 3)
 
 /* Per-kernel timer slots reported by gqa_kernel_times. */
-#define GQA_TIMER_APPEND  0
+#define GQA_TIMER_APPEND  0 /* rows into the cache; E4M3: also its rows read back (gqa_read_kv, prefill) */
 #define GQA_TIMER_DECODE  1
 #define GQA_TIMER_COMBINE 2 /* log-sum-exp merge launch of split-KV decode or segmented prefill */
 #define GQA_TIMER_PREFILL 3
 #define GQA_TIMER_NORM    4 /* layer stage: RMSNorm (gqa_layer_qkv_device) */
-#define GQA_TIMER_PROJECTION 5 /* layer stage: the QKV projection's hipBLASLt kernels, between two recorded events */
-#define GQA_TIMER_ROPE    6 /* layer stage: RoPE + scatter */
+#define GQA_TIMER_PROJECTION 5 /* layer stage: the QKV projection's hipBLASLt kernels, between two recorded events;
+                                  gqa_w4_project_device */
+#define GQA_TIMER_ROPE    6 /* layer stage: RoPE + scatter; gqa_qk_norm_rope_device, _step_device */
 #define GQA_TIMER_COUNT   7
 
 /* Tunables for gqa_set_option. */
@@ -71,7 +72,13 @@ extern "C" {
                                   The automatic plan does not split a (sequence, kv head) whose K/V take
                                   at most 128 KiB (256 KiB from 32 of them on).  Work-groups have 8 waves, or
                                   4 when the 8-wave plan has at most 8 work-groups (the automatic chunk is
-                                  then planned for 4) */
+                                  then planned for 4).
+                                  E4M3 contexts: rounded up to a power of two of at least 256 keys, and no split
+                                  where that gives more than 16 pieces per CU (the pieces are then shared out in
+                                  equal runs, two per CU).  0: one work-group for a (sequence, kv head) whose K/V
+                                  take at most 128 KiB (256 KiB from 32 of them on, 640 KiB from half as many as
+                                  CUs on); else pieces for up to one work-group per CU while there are at most a
+                                  quarter as many as CUs, else equal runs */
 #define GQA_OPT_PROFILE      2 /* 1 = time every kernel launch with a HIP event pair bound to the launch
                                   (hipExtLaunchKernel; restarts the record).  Binding adds no GPU work
                                   between launches, but each timed launch costs the host several us,
@@ -118,7 +125,8 @@ extern "C" {
  * but slows the streaming of larger grids more than a launch costs -- else LAUNCH.  An automatic plan of the
  * shortest splits (one round of every wave) that would need the merge launch takes splits twice as long
  * where that lets AUTO fuse.
- * Both fold the splits in the same order (the same output words). */
+ * Both fold the splits in the same order (the same output words).  E4M3 contexts: equal runs always take LAUNCH, and
+ * AUTO fuses while the split grid is at most half the GPU's CU count. */
 #define GQA_DECODE_MERGE_AUTO   0
 #define GQA_DECODE_MERGE_LAUNCH 1
 #define GQA_DECODE_MERGE_FUSED  2
@@ -330,7 +338,7 @@ int gqa_load_kv_device(gqa_ctx* ctx, int32_t b, int32_t start_pos, int32_t n,
 /* gqa_read_kv_device: gqa_read_kv into device memory (k, v are [H_kv][n][D] bf16 in HBM, 16-byte aligned), from a bf16 or
  * an E4M3 cache. */
 int gqa_read_kv_device(gqa_ctx* ctx, int32_t b, int32_t start_pos, int32_t n, void* k, void* v, void* stream);
-/* Device addresses of the K and V caches ([B][H_kv][L_cap][D] bf16) and L_cap. */
+/* Device addresses of the K and V caches ([B][H_kv][L_cap][D] bf16, or E4M3 codes) and L_cap. */
 int gqa_cache_pointers(gqa_ctx* ctx, void** k_cache, void** v_cache, int32_t* l_cap);
 
 /* ---- decode without allocation ------------------------------------------------------

@@ -9,11 +9,16 @@
 //
 // Direct launches (a small grid): the keys of every (sequence, kv head) are cut into pieces of `chunk` keys, a work-group
 // each.
-// Shares (the others): the keys of every (sequence, kv head) are cut into pieces of `chunk` keys, and all pieces, in order, into one
-// run per work-group, of equal cost to within a piece whatever the lengths are.  A run is a few segments: the end of one
-// (sequence, kv head), whole ones, the beginning of another.  Whole ones are written as they end; the others leave fp32
-// partials (O, m, l), at most two a work-group, that meet with log-sum-exp weights in a second launch -- those of a direct
-// launch in the launch itself where it is small (by the last work-group of a (sequence, kv head) to arrive).  Every K/V byte is read once for all heads of the group.
+// Shares (the others): the pieces of all (sequence, kv head)s, in order, are cut into one run per work-group, of equal
+// cost to within a piece whatever the lengths are.  A run is a few segments: the end of one (sequence, kv head), whole
+// ones, the beginning of another.  Whole ones are written as they end; the others leave fp32 partials (O, m, l), at most
+// two a work-group, that meet with log-sum-exp weights in a second launch -- those of a direct launch in the launch itself
+// where it is small (by the last work-group of a (sequence, kv head) to arrive).  Every K/V byte is read once for all
+// heads of the group.
+//
+// What bounds it: memory.  64 x 8192 keys, 8 kv heads of 128 (1.08 GB): 155 us, 6.98 TB/s (a read of 1 GiB: 7.02); 64
+// sequences of 1000 .. 16000 keys over 64-row pages (549 MB): 90 us beside other launches, 6.1 TB/s, 112 alone; one of
+// 4097 keys (8.5 MB): 5.2 / 10.4, the latency of the launch, one round of loads and the merge.
 //
 // Inside a segment the waves take rounds of keys in turn (four waves 64, eight 32: small launches, which are one latency
 // chain), the next round's K being loaded once the scores are

@@ -364,6 +364,19 @@ struct Kv8Shape {
     bool fused;  // partials merged in-launch
 };
 
+// Both sides measured (us, one launch after the other / beside other launches; all lengths equal, 256 CUs):
+//                                              direct                        shared
+//   1 x 4097 keys, 8 kv heads, D 128          10.4 /  5.2                   15.0 /  6.4
+//   8 x 4000 (64 units: a quarter per CU)     19.2 / 13.3                   24.9 / 14.8
+//   9 x 4000 (72)                             36.0 / 19.4 (unsplit)         26.1 / 16.2
+//   16 x 1300 (128 units of 325 KiB)          16.6 /  9.3 (unsplit)         23.2 / 12.8
+//   16 x 2500 (625 KiB)                       26.6 / 15.6                   27.5 / 18.1
+//   64 x 2400 (512 units of 600 KiB)          53.4 / 49.5                   59.4 / 49.6
+//   64 x 4000 (1000 KiB)                      85.4 / 79.7                   88.8 / 78.9
+//   12 x 1900, D 64 (96 units of 237 KiB)     10.6 /  4.7                   14.1 /  6.6
+//   64 sequences of 1000 .. 16000 keys        163 / 94                      112 / 90
+// The shared runs' merge launch and their search for a start cost about 8 us alone, and lengths that differ cost the
+// unsplit ones the longest of them, which is why units stay whole only while the longest is short.
 constexpr int kKv8Partials = 16;  // per CU: two for each run, or one for each piece
 constexpr int kKv8MaxBatch = 65535;  // of a direct launch (its grid)
 constexpr double kKv8WholeUnits = 0.5, kKv8DirectUnits = 0.25;  // (sequence, kv head) units per CU
