@@ -3,7 +3,7 @@
 // Both are one pass over memory: a write moves 2 D bytes in and D + 1 out per row, a read the reverse; D / 8 lanes hold
 // a row, so the row's maximum is three or four lane exchanges and no LDS.
 //
-// Bound by memory: 8192 tokens of 8 kv heads of 128 read back (50 MB) in 7.5 us beside other launches, 6.7 TB/s (9.3 alone,
+// Bound by memory: 8192 tokens of 8 kv heads of 128 read back (50 MB) in 7.5 us beside other launches, 6.7 TB/s (8.7 alone,
 // 2.7 of them the launch); 2048 written (12.6 MB) in 3.6 / 4.8, where a launch is most of it.  One 16-byte load a side and
 // thread: rows are independent, so the grid is the depth.
 #include "kv8_device.h"
@@ -50,14 +50,16 @@ __global__ __launch_bounds__(kKv8Threads) void kv8_write_kernel(Kv8WriteArgs a) 
 }
 
 // Rows start .. start + n - 1 of sequence b to [H_kv][out_rows][D] bf16 (rows of an unmapped page: zeros).  E4M3: from
-// codes and scales; otherwise from a bf16 cache (the words as they are).
+// codes and scales; otherwise from a bf16 cache (the words as they are).  Work-groups take the heads in turn, as those of the
+// row-block prefill do that reads the rows next: with 8 heads on the same XCD, out of its L2 (256 rows after 7936: 64.4 -> 62.5 us alone, and 9.5 -> 8.7 for this launch; stores past
+// the L2: 73.6).
 template <int D, bool E4M3>
 __global__ __launch_bounds__(kKv8Threads) void kv_read_kernel(KvReadArgs a) {
     constexpr int LANES = D / 8;
-    const int64_t i = ((int64_t)blockIdx.x * kKv8Threads + threadIdx.x) / LANES;
-    const int part = threadIdx.x % LANES;
-    if (i >= (int64_t)a.cache.n_kv_heads * a.n) return;
-    const int h = (int)(i / a.n), t = (int)(i - (int64_t)h * a.n);
+    const int h = blockIdx.x % a.cache.n_kv_heads, part = threadIdx.x % LANES;
+    const int64_t at = (int64_t)(blockIdx.x / a.cache.n_kv_heads) * (kKv8Threads / LANES) + threadIdx.x / LANES;
+    if (at >= a.n) return;
+    const int t = (int)at;
     const int64_t row = kv8_row(a.cache, a.b, h, a.start + t);
     const int64_t to = ((int64_t)h * a.out_rows + t) * LANES + part;
     const uint8_t* const codes[2] = {a.cache.k, a.cache.v};
@@ -100,7 +102,7 @@ hipError_t launch_kv8_write(int head_dim, const Kv8WriteArgs& a, const Launch& l
 
 hipError_t launch_kv_read(int head_dim, const KvReadArgs& a, const Launch& l) {
     if (a.n < 1) return hipSuccess;
-    const int64_t threads = (int64_t)a.cache.n_kv_heads * a.n * (head_dim / 8), wgs = (threads + kKv8Threads - 1) / kKv8Threads;
+    const int64_t rows = kKv8Threads / (head_dim / 8), wgs = (a.n + rows - 1) / rows * a.cache.n_kv_heads;
     if (wgs > 0x7FFFFFFF) return hipErrorInvalidValue;
     const dim3 grid((uint32_t)wgs), block(kKv8Threads);
     const bool e4m3 = a.cache.k_scale != nullptr;
