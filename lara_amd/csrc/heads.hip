@@ -6,13 +6,15 @@
 // by 2^-25 of itself: 0.03 rad at position 10^6).
 //
 // D / 8 lanes hold a head row, so its sum of squares (and an E4M3 row's maximum) is three or four lane exchanges, and a
-// lane's four pairs are the same in every head that it takes.  A work-group is a token, so an angle is made once for all
-// of its heads.
+// lane's four pairs are the same in every head that it takes.  A work-group is a token (two of a prompt at D 64, as many
+// rows), so an angle is made once for all of its heads; three rows a thread are on their way at once, the first ones and
+// the weights while the angles are computed.
 //
-// Bound by memory for prompts: 2048 tokens of 32 + 16 heads of 128 (50 MB) in 8.9 us beside other launches, 5.7 TB/s (11.9
-// alone); a step of 64 sequences (1.4 MB) is a launch, 4.0 / 5.0.  (Loads ahead of the angles: 14.1 us alone for those 2048,
-// the waves that had waited for angles while others streamed all waiting for memory at once; sine and cosine in fp32: 0.1
-// less.)
+// Bound by memory for long prompts: 8192 tokens of 32 + 16 heads of 128 (185 MB) in 28.3 us beside other launches, 6.5 TB/s
+// (32 alone; a load and a weight at a time 37); 2048 (50 MB) 9.3 / 12.2, one wave of work-groups whose vector
+// instructions and loads take turns; 4000 of 48 heads of 64 11.5 alone, 13.4 with a token a work-group.  Two tokens a
+// work-group at D 128: 14.2 at 2048, 36 at 8192.  Registers for 8 work-groups a CU matter: with 80 (weights and angles kept
+// as fp32) 2048 take 14.6.  A step of 64 sequences (1.4 MB) is a launch: 4.5 alone, 5.1 without the loads ahead.
 #include "kv8_device.h"
 
 #include <math.h>
@@ -21,6 +23,7 @@ namespace lara {
 namespace {
 
 constexpr int kHeadsThreads = 256;
+constexpr int kHeadsBatch = 3;
 
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 
@@ -38,49 +41,64 @@ __device__ __forceinline__ float row_sum(float v) {
     return v;
 }
 
-// One work-group per token.
-template <int D, bool E4M3>
+// TOKENS tokens a work-group (one of the step form); a thread keeps its token and its place in a row.
+template <int D, bool E4M3, int TOKENS>
 __global__ __launch_bounds__(kHeadsThreads) void qk_norm_rope_kernel(HeadsArgs a) {
     constexpr int LANES = D / 8, PAIRS = D / 2;
-    const int token = blockIdx.x;
+    const int token0 = blockIdx.x * TOKENS, tokens = TOKENS == 1 || a.n_tokens - token0 >= TOKENS ? TOKENS : a.n_tokens - token0;
     const int part = threadIdx.x % LANES;
-    int b = a.b, pos = a.pos_base + token, k_pos = a.k_pos_base + token, t = a.row0 + token;
-    if (a.positions != nullptr) {  // one token of each sequence
-        b = token;
-        pos = k_pos = a.positions[token];
-        t = a.rows != nullptr ? a.rows[token] : pos;
-        if (pos < 0 || t < 0 || t >= a.cache.l_max) return;  // (the whole work-group) nothing of this sequence is written
+    int b = a.b, pos0 = a.pos_base + token0, k_pos0 = a.k_pos_base + token0, t0 = a.row0 + token0;
+    if (TOKENS == 1 && a.positions != nullptr) {  // one token of each sequence
+        b = token0;
+        pos0 = k_pos0 = a.positions[token0];
+        t0 = a.rows != nullptr ? a.rows[token0] : pos0;
+        if (pos0 < 0 || t0 < 0 || t0 >= a.cache.l_max) return;  // (the whole work-group) nothing of this sequence is written
     }
-    __shared__ float2 turn[2][PAIRS];
+    const int heads = a.n_q_heads + 2 * a.cache.n_kv_heads, chunks = heads * TOKENS * LANES;
+    // A batch of values is loaded at once, the first ahead of the angles.
+    u32x4 in[kHeadsBatch];
+    auto load = [&](int from) __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = 0; k < kHeadsBatch; ++k) {
+            const int i = from + k * kHeadsThreads, of = i / LANES % TOKENS;
+            if (i < chunks && of < tokens)
+                in[k] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(a.x + (size_t)(token0 + of) * a.ld) +
+                                                   i / (LANES * TOKENS) * LANES + part);
+        }
+    };
+    load(threadIdx.x);
+    u32x4 wq = {}, wk = {};
+    if (a.wq != nullptr) wq = reinterpret_cast<const u32x4*>(a.wq)[part];
+    if (a.wk != nullptr) wk = reinterpret_cast<const u32x4*>(a.wk)[part];
+    __shared__ float2 turn[2][TOKENS][PAIRS];
     if (a.log2_base > 0.0) {
-        const int sets = k_pos != pos ? 2 : 1;
-        for (int i = threadIdx.x; i < sets * PAIRS; i += kHeadsThreads) {
-            const int p = i % PAIRS;
+        const int sets = k_pos0 != pos0 ? 2 : 1;
+        for (int i = threadIdx.x; i < sets * TOKENS * PAIRS; i += kHeadsThreads) {
+            const int p = i % PAIRS, of = i / PAIRS % TOKENS, set = i / (PAIRS * TOKENS);
             double sd, cd;
-            sincos((double)(i < PAIRS ? pos : k_pos) * exp2(-2.0 * p / D * a.log2_base), &sd, &cd);
-            turn[i / PAIRS][p] = make_float2((float)cd, (float)sd);
+            sincos((double)((set ? k_pos0 : pos0) + of) * exp2(-2.0 * p / D * a.log2_base), &sd, &cd);
+            turn[set][of][p] = make_float2((float)cd, (float)sd);
         }
         __syncthreads();
     }
-    const int heads = a.n_q_heads + 2 * a.cache.n_kv_heads;
-    const u32x4* const src = reinterpret_cast<const u32x4*>(a.x + (size_t)token * a.ld);
-    for (int i = threadIdx.x; i < heads * LANES; i += kHeadsThreads) {  // (a row's lanes stay together)
-        const int head = i / LANES;
+    auto process = [&](int i, const u32x4& words) __attribute__((always_inline)) {  // (a row's lanes stay together)
+        const int of = i / LANES % TOKENS, token = token0 + of;
+        if (i >= chunks || of >= tokens) return;
+        const int head = i / (LANES * TOKENS);
         const bool is_q = head < a.n_q_heads, is_k = !is_q && head < a.n_q_heads + a.cache.n_kv_heads;
         float x[8];
-        unpack_bf16x8(__builtin_nontemporal_load(src + i), x);
-        const uint16_t* const weight = is_q ? a.wq : is_k ? a.wk : nullptr;
-        if (weight != nullptr) {
+        unpack_bf16x8(words, x);
+        if (is_q ? a.wq != nullptr : is_k && a.wk != nullptr) {
             float w[8], sum = 0.f;
-            unpack_bf16x8(reinterpret_cast<const u32x4*>(weight)[part], w);
+            unpack_bf16x8(is_q ? wq : wk, w);
 #pragma unroll
             for (int j = 0; j < 8; ++j) sum = fmaf(x[j], x[j], sum);
-            const float inv = 1.0f / sqrtf(row_sum<LANES>(sum) / (float)D + a.eps);
+            const float inv = rsqrtf(row_sum<LANES>(sum) * (1.0f / D) + a.eps);
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[j] = x[j] * inv * w[j];
         }
         if (a.log2_base > 0.0 && (is_q || is_k)) {
-            const float2* const cs = turn[is_k && k_pos != pos ? 1 : 0] + 4 * part;
+            const float2* const cs = turn[is_k && k_pos0 != pos0 ? 1 : 0][of] + 4 * part;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const float c = cs[j].x, s = cs[j].y, x0 = x[2 * j], x1 = x[2 * j + 1];
@@ -99,11 +117,11 @@ __global__ __launch_bounds__(kHeadsThreads) void qk_norm_rope_kernel(HeadsArgs a
         if (is_q) {
             const size_t row = a.positions != nullptr ? (size_t)token * a.n_q_heads + head : (size_t)head * a.n_tokens + token;
             reinterpret_cast<u32x4*>(a.q_out)[row * LANES + part] = o;
-            continue;
+            return;
         }
         const int h = head - a.n_q_heads - (is_k ? 0 : a.cache.n_kv_heads);
-        const int64_t row = kv8_row(a.cache, b, h, t);
-        if (row < 0) continue;  // unmapped page: nothing to write
+        const int64_t row = kv8_row(a.cache, b, h, t0 + of);
+        if (row < 0) return;  // unmapped page: nothing to write
         uint8_t* const to = is_k ? a.cache.k : a.cache.v;
         if constexpr (E4M3) {
             uint32_t byte;
@@ -113,21 +131,27 @@ __global__ __launch_bounds__(kHeadsThreads) void qk_norm_rope_kernel(HeadsArgs a
         } else {
             reinterpret_cast<u32x4*>(to)[row * LANES + part] = o;
         }
+    };
+    for (int i = threadIdx.x; i < chunks; i += kHeadsBatch * kHeadsThreads) {
+#pragma unroll
+        for (int k = 0; k < kHeadsBatch; ++k) process(i + k * kHeadsThreads, in[k]);
+        load(i + kHeadsBatch * kHeadsThreads);
     }
 }
 
 }  // namespace
 
+template <int D, int TOKENS>
+static hipError_t launch_tokens(const HeadsArgs& a, const Launch& l) {
+    const dim3 grid((a.n_tokens + TOKENS - 1) / TOKENS), block(kHeadsThreads);
+    return a.cache.k_scale != nullptr ? launch_kernel(qk_norm_rope_kernel<D, true, TOKENS>, grid, block, l, a)
+                                      : launch_kernel(qk_norm_rope_kernel<D, false, TOKENS>, grid, block, l, a);
+}
+
 hipError_t launch_qk_norm_rope(int head_dim, const HeadsArgs& a, const Launch& l) {
     if (a.n_tokens < 1) return hipSuccess;
-    const dim3 grid(a.n_tokens), block(kHeadsThreads);
-    const bool e4m3 = a.cache.k_scale != nullptr;
-    if (head_dim == 128)
-        return e4m3 ? launch_kernel(qk_norm_rope_kernel<128, true>, grid, block, l, a)
-                    : launch_kernel(qk_norm_rope_kernel<128, false>, grid, block, l, a);
-    if (head_dim == 64)
-        return e4m3 ? launch_kernel(qk_norm_rope_kernel<64, true>, grid, block, l, a)
-                    : launch_kernel(qk_norm_rope_kernel<64, false>, grid, block, l, a);
+    if (head_dim == 128) return launch_tokens<128, 1>(a, l);
+    if (head_dim == 64) return a.positions == nullptr ? launch_tokens<64, 2>(a, l) : launch_tokens<64, 1>(a, l);
     return hipErrorInvalidValue;
 }
 

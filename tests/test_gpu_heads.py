@@ -176,3 +176,25 @@ def test_refusals():
         assert prompt(x=k) == R and prompt(x=v) == R  # the rows it writes
         assert prompt() == step() == _lib.GQA_OK
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_rows_whose_squares_are_subnormal_or_zero(d):
+    """Mean squares near 2^-128 (2^-21 of it a step of the sum: 2^-19 of a value with the bound above), eps 0; a row of zeros
+    with an eps stays zero."""
+    rng = np.random.default_rng(41)
+    hq, hkv, n = 4, 2, 5
+    scale = np.array([2.0**-64, 1.0, 2.0**-63, 2.0**-40, 2.0**-64])
+    x = orc.bf16_rne((rng.standard_normal((n, (hq + 2 * hkv) * d)) * scale[:, None]).astype(np.float32))
+    zero = np.zeros_like(x)
+    with AttentionAccelerator(n_q_heads=hq, n_kv_heads=hkv, head_dim=d, max_seq_len=64) as acc:
+        one = dev(orc.bf16_rne(np.ones(d, np.float32)))
+        for words_in, eps in ((x, 0.0), (zero, 1e-6)):
+            xd, q = dev(words_in), torch.empty((hq, n, d), dtype=torch.int16, device="cuda")
+            acc.qk_norm_rope_device(xd.data_ptr(), words_in.shape[1], n, one.data_ptr(), one.data_ptr(), q.data_ptr(), eps=eps, rope_base=0.0)
+            torch.cuda.synchronize()
+            qh, kh, _ = split(words_in, hq, hkv, d)
+            k = acc.read_kv(0, 0, n)[0]
+            for got, h in ((words(q), qh), (k, kh)):
+                want = h / np.sqrt((h * h).mean(-1, keepdims=True) + eps)
+                assert np.all(np.abs(f64(got) - want) <= (2.0**-8 + 2 * FP32) * np.abs(want))
