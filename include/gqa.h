@@ -236,6 +236,8 @@ int gqa_paged_layers(gqa_ctx* ctx, int32_t* n_layers, int32_t* layer);
  *     several streams follow each other, and these calls return GQA_ERR_UNSUPPORTED under a stream capture.  Decode,
  *     append, load, read and the heads' entry points below need no workspace.
  *   - KV260 numerics and gqa_decode_append_noalloc are for bf16 caches.
+ * Decode launches of one context share its split partials, as on a bf16 cache: the caller orders them, replays of captured
+ * ones among them.
  * gqa_cache_pointers returns the codes' pools; gqa_kv8_scales the active layer's scale bytes ([B][H_kv][L_cap], paged
  * [n_pages][H_kv][page_size]; GQA_ERR_UNSUPPORTED on a bf16 context). */
 int gqa_create_kv8(const gqa_config* cfg, int32_t page_size, int32_t n_pages, int32_t n_layers, gqa_ctx** out_ctx);
@@ -336,7 +338,7 @@ int gqa_prefill_append_device(gqa_ctx* ctx, int32_t b, const void* q, const void
 int gqa_load_kv_device(gqa_ctx* ctx, int32_t b, int32_t start_pos, int32_t n,
                        const void* k, const void* v, void* stream);
 /* gqa_read_kv_device: gqa_read_kv into device memory (k, v are [H_kv][n][D] bf16 in HBM, 16-byte aligned), from a bf16 or
- * an E4M3 cache. */
+ * an E4M3 cache.  They must overlap neither each other nor the cache (GQA_ERR_RANGE). */
 int gqa_read_kv_device(gqa_ctx* ctx, int32_t b, int32_t start_pos, int32_t n, void* k, void* v, void* stream);
 /* Device addresses of the K and V caches ([B][H_kv][L_cap][D] bf16, or E4M3 codes) and L_cap. */
 int gqa_cache_pointers(gqa_ctx* ctx, void** k_cache, void** v_cache, int32_t* l_cap);
@@ -418,7 +420,8 @@ int gqa_layer_times(gqa_ctx* ctx, float* out_us, int32_t n);
  * memory, rows NULL for rows = positions; q_out is [B][H_q][D].  A sequence with a negative position, or a row outside
  * 0 .. max_seq_len - 1, is left out: neither its Q nor its cache is written.  Positions of sequences that are not left
  * out stay below 2^30.
- * qkv must not overlap q_out or the cache, and all operands are 16-byte aligned (else GQA_ERR_RANGE). */
+ * ld is a multiple of 8 below 2^31.  qkv, q_out and the cache must not overlap, nor the weights and q_out, and all
+ * operands are 16-byte aligned (positions and rows 4-byte), else GQA_ERR_RANGE. */
 int gqa_qk_norm_rope_device(gqa_ctx* ctx, int32_t b, const void* qkv, int64_t ld, int32_t n_tokens, const void* q_weight,
                             const void* k_weight, float eps, int32_t q_pos_base, int32_t kv_pos_base, int32_t kv_row0,
                             double rope_base, void* q_out, void* stream);
@@ -434,7 +437,7 @@ int gqa_qk_norm_rope_step_device(gqa_ctx* ctx, const void* qkv, int64_t ld, cons
  * [rows][hidden / group] out for the products, once; gqa_w4_bytes gives the sizes of the two results.
  * gqa_w4_project_device: y [n_tokens][ldy] bf16 (the first `rows` of each row) = norm(x) W^T for x [n_tokens][hidden] bf16,
  * norm(x) = x / sqrt(mean(x^2) + rms_eps) * rms_weight, or x with rms_weight NULL.  x * rms_weight is rounded to bf16,
- * sums are fp32.  n_tokens up to GQA_W4_MAX_TOKENS; a token's result does not depend on the others of the call.
+ * sums are fp32.  n_tokens up to GQA_W4_MAX_TOKENS, ldy below 2^31; a token's result does not depend on the others of the call.
  * gqa_w4_unpack_device: the packed matrix as bf16 [rows][hidden], for long prompts (gqa_layer_qkv_device).
  * The context gives device and stream.  Operands are 16-byte aligned (codes any, scales and y 2-byte) and outputs must
  * not overlap inputs, else GQA_ERR_RANGE.  None of these calls allocates or synchronises. */

@@ -221,6 +221,27 @@ inline bool overlaps(const void* a, size_t na, const void* b, size_t nb) {
     return na > 0 && nb > 0 && x < y + nb && y < x + na;
 }
 
+// The context's device for the length of a call; the caller's is put back.
+struct DeviceScope {
+    int before = -1;
+    hipError_t status;
+    explicit DeviceScope(int device) {
+        status = hipGetDevice(&before);
+        if (status == hipSuccess && before != device) status = hipSetDevice(device);
+        else before = -1;
+    }
+    ~DeviceScope() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+};
+
+// Whether n bytes at p reach into what the context's active layer keeps.
+inline bool overlaps_cache(const gqa_ctx* c, const void* p, size_t n) {
+    const size_t scales = c->kv8 ? kv_rows(c) : 0;
+    return overlaps(p, n, c->k_cache, kv_bytes(c)) || overlaps(p, n, c->v_cache, kv_bytes(c)) ||
+           overlaps(p, n, c->k_scale, scales) || overlaps(p, n, c->v_scale, scales);
+}
+
 // Device operands the kernels move in 16-byte vectors (Q, appended K/V rows, prefill output)
 // must be 16-byte aligned; nullptr passes (optional operands are checked for presence apart).
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -1901,6 +1922,10 @@ int gqa_read_kv_device(gqa_ctx* c, int32_t b, int32_t start_pos, int32_t n, void
     if (!aligned16(k) || !aligned16(v)) return GQA_ERR_RANGE;
     if (n == 0) return GQA_OK;
     if (!rows_backed(c, b, start_pos, n)) return GQA_ERR_RANGE;
+    const size_t bytes = (size_t)c->cfg.n_kv_heads * n * c->cfg.head_dim * 2;
+    if (overlaps(k, bytes, v, bytes) || overlaps_cache(c, k, bytes) || overlaps_cache(c, v, bytes)) return GQA_ERR_RANGE;
+    const DeviceScope device(c->cfg.device);
+    HIP_TRY(device.status);
     HIP_TRY(read_rows(c, b, start_pos, n, n, k, v, pick_stream(c, stream)));
     return GQA_OK;
 }
@@ -2282,32 +2307,20 @@ int gqa_layer_times(gqa_ctx* c, float* out_us, int32_t n) {
 
 namespace {
 
-// The context's device for the length of a call; the caller's is put back.
-struct DeviceScope {
-    int before = -1;
-    hipError_t status;
-    explicit DeviceScope(int device) {
-        status = hipGetDevice(&before);
-        if (status == hipSuccess && before != device) status = hipSetDevice(device);
-        else before = -1;
-    }
-    ~DeviceScope() {
-        if (before >= 0) (void)hipSetDevice(before);
-    }
-};
-
 constexpr int kHeadsMaxPosition = 1 << 30;
 
 int run_heads(gqa_ctx* c, HeadsArgs& a, const void* qkv, int64_t ld, const void* q_weight, const void* k_weight, float eps,
               double rope_base, void* q_out, hipStream_t s) {
     const int64_t width = (int64_t)(c->cfg.n_q_heads + 2 * c->cfg.n_kv_heads) * c->cfg.head_dim;
-    if (ld < width || ld % 8 != 0 || !aligned16(qkv) || !aligned16(q_weight) || !aligned16(k_weight) || !aligned16(q_out))
+    if (ld < width || ld > INT32_MAX || ld % 8 != 0 || !aligned16(qkv) || !aligned16(q_weight) || !aligned16(k_weight) || !aligned16(q_out))
         return GQA_ERR_RANGE;
     if (!(eps >= 0.f) || !isfinite(eps)) return GQA_ERR_RANGE;
     if (!(rope_base == 0.0 || rope_base > 1.0) || !isfinite(rope_base)) return GQA_ERR_RANGE;
-    // The kernel reads the rows while it writes Q and the cache.
+    // The kernel reads the rows and the weights while it writes Q and the cache.
+    const size_t weight = (size_t)c->cfg.head_dim * 2;
     const size_t in = ((size_t)(a.n_tokens - 1) * ld + width) * 2, out = (size_t)a.n_tokens * c->cfg.n_q_heads * c->cfg.head_dim * 2;
-    if (overlaps(qkv, in, q_out, out) || overlaps(qkv, in, c->k_cache, kv_bytes(c)) || overlaps(qkv, in, c->v_cache, kv_bytes(c)))
+    if (overlaps(qkv, in, q_out, out) || overlaps(q_weight, weight, q_out, q_weight ? out : 0) ||
+        overlaps(k_weight, weight, q_out, k_weight ? out : 0) || overlaps_cache(c, qkv, in) || overlaps_cache(c, q_out, out))
         return GQA_ERR_RANGE;
     a.x = (const uint16_t*)qkv;
     a.ld = ld;
@@ -2357,6 +2370,7 @@ int gqa_qk_norm_rope_device(gqa_ctx* c, int32_t b, const void* qkv, int64_t ld, 
 int gqa_qk_norm_rope_step_device(gqa_ctx* c, const void* qkv, int64_t ld, const void* q_weight, const void* k_weight, float eps,
                                  const int32_t* positions, const int32_t* rows, double rope_base, void* q_out, void* stream) {
     if (!c || !qkv || !positions || !q_out) return GQA_ERR_NULL;
+    if ((reinterpret_cast<uintptr_t>(positions) | reinterpret_cast<uintptr_t>(rows)) & 3) return GQA_ERR_RANGE;
     HeadsArgs a{};
     a.n_tokens = c->cfg.batch;
     a.positions = positions;
@@ -2412,7 +2426,7 @@ int gqa_w4_project_device(gqa_ctx* c, const void* x, int32_t n_tokens, int32_t h
     if (!c || !x || !w || !w_scales || !y) return GQA_ERR_NULL;
     const int rc = check_w4(rows, hidden, group);
     if (rc != GQA_OK) return rc;
-    if (n_tokens < 1 || n_tokens > GQA_W4_MAX_TOKENS || ldy < rows) return GQA_ERR_RANGE;
+    if (n_tokens < 1 || n_tokens > GQA_W4_MAX_TOKENS || ldy < rows || ldy > INT32_MAX) return GQA_ERR_RANGE;
     if (!(rms_eps >= 0.f) || !isfinite(rms_eps)) return GQA_ERR_RANGE;
     if (!aligned16(x) || !aligned16(rms_weight) || !aligned16(w) || !aligned16(w_scales) || (reinterpret_cast<uintptr_t>(y) & 1))
         return GQA_ERR_RANGE;

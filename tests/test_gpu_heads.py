@@ -198,3 +198,31 @@ def test_rows_whose_squares_are_subnormal_or_zero(d):
             for got, h in ((words(q), qh), (k, kh)):
                 want = h / np.sqrt((h * h).mean(-1, keepdims=True) + eps)
                 assert np.all(np.abs(f64(got) - want) <= (2.0**-8 + 2 * FP32) * np.abs(want))
+
+
+def test_refuses_outputs_in_the_cache_or_over_the_weights():
+    t = torch.zeros(1 << 16, dtype=torch.int16, device="cuda")
+    u = torch.zeros(1 << 16, dtype=torch.int16, device="cuda")
+    pos = torch.zeros(4, dtype=torch.int32, device="cuda")
+    lib, R = _lib.lib(), _lib.GQA_ERR_RANGE
+    with AttentionAccelerator(n_q_heads=8, n_kv_heads=2, head_dim=64, max_seq_len=64, kv_format="e4m3") as acc:
+        c, width = acc._ctx, 12 * 64
+        k, v, ks, vs = (ctypes.c_void_p() for _ in range(4))
+        cap = ctypes.c_int32()
+        call("gqa_cache_pointers", c, ctypes.byref(k), ctypes.byref(v), ctypes.byref(cap))
+        call("gqa_kv8_scales", c, ctypes.byref(ks), ctypes.byref(vs))
+
+        def prompt(x=ptr(t), ld=width, wq=None, q=ptr(u)):
+            return lib.gqa_qk_norm_rope_device(c, 0, x, ld, 4, wq, None, 1e-5, 0, 0, 0, 1e4, q, None)
+
+        for inside in (k, v, ks, vs):
+            assert prompt(q=inside) == R and prompt(x=inside) == R
+            assert lib.gqa_read_kv_device(c, 0, 0, 4, inside, ptr(t), None) == R
+            assert lib.gqa_read_kv_device(c, 0, 0, 4, ptr(t), inside, None) == R
+        assert lib.gqa_read_kv_device(c, 0, 0, 4, ptr(t), ptr(t), None) == R
+        assert prompt(wq=ptr(u)) == R and prompt(ld=1 << 31) == R
+        odd = ctypes.c_void_p(pos.data_ptr() + 2)
+        for p, r in ((odd, None), (ptr(pos), odd)):
+            assert lib.gqa_qk_norm_rope_step_device(c, ptr(t), width, None, None, 1e-5, p, r, 1e4, ptr(u), None) == R
+        assert prompt() == _lib.GQA_OK
+        torch.cuda.synchronize()

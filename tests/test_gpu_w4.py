@@ -205,6 +205,12 @@ def test_refusals(acc):
     torch.cuda.synchronize()
 
 
+def test_refuses_a_stride_past_31_bits(acc):
+    t = torch.zeros(1 << 14, dtype=torch.int16, device="cuda")
+    at = [ptr(t[1024 * i :]) for i in range(4)]
+    assert _lib.lib().gqa_w4_project_device(acc._ctx, at[0], 1, 64, at[1], at[2], 64, 16, None, 0.0, at[3], 1 << 31, None) == _lib.GQA_ERR_RANGE
+
+
 def test_a_decode_step_of_all_operators():
     """Projection with 4-bit weights, norms with RoPE into a paged E4M3 cache, attention: two layers' caches, four steps,
     each operator checked on what the one before it gave; then the same steps from a captured graph, word for word."""
