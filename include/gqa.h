@@ -437,7 +437,8 @@ int gqa_qk_norm_rope_step_device(gqa_ctx* ctx, const void* qkv, int64_t ld, cons
  * [rows][hidden / group] out for the products, once; gqa_w4_bytes gives the sizes of the two results.
  * gqa_w4_project_device: y [n_tokens][ldy] bf16 (the first `rows` of each row) = norm(x) W^T for x [n_tokens][hidden] bf16,
  * norm(x) = x / sqrt(mean(x^2) + rms_eps) * rms_weight, or x with rms_weight NULL.  x * rms_weight is rounded to bf16,
- * sums are fp32.  n_tokens up to GQA_W4_MAX_TOKENS, ldy below 2^31; a token's result does not depend on the others of the call.
+ * sums are fp32, of (128 + c) x and -136 x before the scale: a token whose |x * rms_weight| passes 2^112, or that is
+ * not finite, may give NaN in every row.  n_tokens up to GQA_W4_MAX_TOKENS, ldy below 2^31; a token's result does not depend on the others of the call.
  * gqa_w4_unpack_device: the packed matrix as bf16 [rows][hidden], for long prompts (gqa_layer_qkv_device).
  * The context gives device and stream.  Operands are 16-byte aligned (codes any, scales and y 2-byte) and outputs must
  * not overlap inputs, else GQA_ERR_RANGE.  None of these calls allocates or synchronises. */

@@ -11,9 +11,8 @@
 // Rows past the matrix have code 8 and scale 0, columns past it scale 0.
 //
 // The constant 136 = 128 + 8 leaves through a product of its own, with operand A = -136 everywhere: it is the same for
-// all rows, and a group's accumulators of every row tile start from it.  Products are exact and
-// summed in fp32, a group at a time, then scaled in fp32.
-// x * gamma is rounded to bf16 (operand B; half a step of 2^-8, as the normalised rows of the bf16 stage are).
+// all rows, and a group's accumulators of every row tile start from it.  Products are exact and summed in fp32, a group at a
+// time, then scaled in fp32.  x * gamma is rounded to bf16 (operand B; half a step of 2^-8, as the normalised rows of the bf16 stage are).
 #include "gqa_internal.h"
 
 #include <math.h>
@@ -128,7 +127,7 @@ __device__ __forceinline__ float w4_row_add(float v) {
 // tile: 6.9 us for one token, 14.4 for 13, where every work-group's copy of the tokens is what it waits for.)
 //
 // What bounds it: at one token the weights' latency (4096 -> 6144, group 128, 13 MB: 7.0 us alone, 4.0 with other launches
-// beside it, of which about 2.7 are the launch; 1.9 us at the copy rate).  From 16 tokens on the unpacking of codes (7
+// beside it, of which about 2.7 are the launch; 1.9 us at the read rate).  From 16 tokens on the unpacking of codes (7
 // vector instructions for 8 codes a lane, used for 16 NT tokens) and the tokens' own way to every work-group.
 //
 // A token's sum is the same in every form: each wave adds its groups in order, the waves are added in order.
