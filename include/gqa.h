@@ -235,6 +235,8 @@ int gqa_paged_layers(gqa_ctx* ctx, int32_t* n_layers, int32_t* layer);
  *     kv_len seen (a call that grows it synchronises the device), and the layer stage passes through it: uses of it on
  *     several streams follow each other, and these calls return GQA_ERR_UNSUPPORTED under a stream capture.  Decode,
  *     append, load, read and the heads' entry points below need no workspace.
+ *   - decode plans for batch * n_kv_heads * max_seq_len up to 2^36 keys (in the host forms, times the longest length);
+ *     GQA_ERR_UNSUPPORTED above (a paged context may be sized so without having the rows).
  *   - KV260 numerics and gqa_decode_append_noalloc are for bf16 caches.
  * Decode launches of one context share its split partials, as on a bf16 cache: the caller orders them, replays of captured
  * ones among them.
@@ -438,7 +440,8 @@ int gqa_qk_norm_rope_step_device(gqa_ctx* ctx, const void* qkv, int64_t ld, cons
  * gqa_w4_project_device: y [n_tokens][ldy] bf16 (the first `rows` of each row) = norm(x) W^T for x [n_tokens][hidden] bf16,
  * norm(x) = x / sqrt(mean(x^2) + rms_eps) * rms_weight, or x with rms_weight NULL.  x * rms_weight is rounded to bf16,
  * sums are fp32, of (128 + c) x and -136 x before the scale: a token whose |x * rms_weight| passes 2^112, or that is
- * not finite, may give NaN in every row.  n_tokens up to GQA_W4_MAX_TOKENS, ldy below 2^31; a token's result does not depend on the others of the call.
+ * not finite, may give NaN in every row.  n_tokens up to GQA_W4_MAX_TOKENS, ldy below 2^31; a token's result does not
+ * depend on the others of the call.
  * gqa_w4_unpack_device: the packed matrix as bf16 [rows][hidden], for long prompts (gqa_layer_qkv_device).
  * The context gives device and stream.  Operands are 16-byte aligned (codes any, scales and y 2-byte) and outputs must
  * not overlap inputs, else GQA_ERR_RANGE.  None of these calls allocates or synchronises. */

@@ -400,6 +400,7 @@ struct Kv8Shape {
 // unsplit ones the longest of them, which is why units stay whole only while the longest is short.
 constexpr int kKv8Partials = 16;  // per CU: two for each run, or one for each piece
 constexpr int kKv8MaxBatch = 65535;  // of a direct launch (its grid)
+constexpr int64_t kKv8MaxCost = 1 << 30;
 constexpr double kKv8WholeUnits = 0.5, kKv8DirectUnits = 0.25;  // (sequence, kv head) units per CU
 constexpr int64_t kKv8WholeBytes = 640 << 10;
 
@@ -510,6 +511,9 @@ int plan_decode(gqa_ctx* c, const void* q, const int32_t* lens, const void* k_ne
     if (c->kv8) {
         const Kv8Shape shape = plan_kv8(c->cfg.batch, c->cfg.n_kv_heads, c->cfg.head_dim, c->n_cu, max_len, c->chunk_opt,
                                         c->decode_merge);
+        // (Runs count the batch's cost in 32 bits, whatever lengths the device holds.)
+        if (shape.runs > 0 && units * (4 * (((int64_t)max_len + kKv8Piece - 1) / kKv8Piece) + 4) > kKv8MaxCost)
+            return GQA_ERR_UNSUPPORTED;
         a.k_scale = c->k_scale;
         a.v_scale = c->v_scale;
         a.group = c->group;

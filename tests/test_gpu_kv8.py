@@ -569,6 +569,24 @@ def test_refusals():
         assert e.value.code == _lib.GQA_ERR_UNSUPPORTED
 
 
+def test_decode_refuses_more_keys_than_its_runs_count():
+    """A paged context sized for 2^39 keys with one page of rows: the device form plans for all of them and is refused, the
+    host form plans for the lengths."""
+    rng = np.random.default_rng(43)
+    B, hkv, d, page = 512, 8, 64, 1 << 12
+    with engine(batch=B, n_q_heads=8, n_kv_heads=hkv, head_dim=d, max_seq_len=1 << 27, max_q_len=16, page_size=page,
+                n_pages=1) as acc:
+        acc.reserve(3, 40)
+        k, v, q = rows(rng, (hkv, 40, d)), rows(rng, (hkv, 40, d)), bf16_normal(rng, (B, 8, d))
+        acc.load_kv(k, v, b=3)
+        lens = np.zeros(B, np.int32)
+        lens[3] = 40
+        t, n, o = dev(q), dev(lens), torch.zeros((B, 8, d), dtype=torch.int16, device="cuda")
+        assert _lib.lib().gqa_decode_device(acc._ctx, ptr(t), ptr(n), ptr(o), None, None) == _lib.GQA_ERR_UNSUPPORTED
+        got, lse = acc.decode_step(q, lens, return_lse=True)
+        close(got[3], lse[3], so.decode(f64(q[3]), so.stored(f64(k)), so.stored(f64(v)), acc.scale))
+
+
 def test_unmapped_pages_read_as_zeros_on_the_device():
     """Device lengths past the mapped rows: keys and values of zero, nothing written."""
     rng = np.random.default_rng(17)
