@@ -5,6 +5,7 @@
 #include "gqa_internal.h"
 
 #include <limits.h>
+#include <math.h>
 
 namespace lara {
 namespace {
@@ -24,6 +25,14 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
 }
 
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Sums (m, l, O) of a softmax are joined at the largest m.  Where that is -inf, no score was above it: l and O are 0 (no
+// key) or NaN (scores of NaN, which a maximum passes over), and both come through weights of 0.
+__device__ __forceinline__ float softmax_base(float m) { return m == -INFINITY ? 0.f : m; }
+// A row and its natural-log sum: 0 and -inf without keys (l is 1 at least where there is a score that is a number), NaN
+// with a score of NaN.
+__device__ __forceinline__ float softmax_out(float o, float l) { return l == 0.f ? 0.f : o / l; }
+__device__ __forceinline__ float softmax_lse(float m, float l) { return l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2; }
 
 __device__ __forceinline__ int clamp_len(int len, int l_max) {
     return len < 0 ? 0 : (len > l_max ? l_max : len);

@@ -34,8 +34,8 @@
 //     plain read of 1 GiB); then lanes m and m + 8 exchange halves, so that m < 8 has the first D / 16 dims of both keys,
 //     m >= 8 the others.  Byte t of them belongs to row m of tile t, dim D/16 * (2 (m % 8) + m / 8) + t.  v_perm_b32 pairs
 //     the bytes of two keys, the conversion makes them a word of operand A.
-// A row of length 0 writes zeros and -inf.  Rows past a sequence's end are cleared (a stale code may be NaN, and 0 * NaN
-// is NaN) and their scores masked.
+// A row of length 0 writes zeros and -inf, one with a score of NaN writes NaN.  Rows past a sequence's end are cleared (a
+// stale code may be NaN, and 0 * NaN is NaN) and their scores masked.
 //
 // The row appended by the launch: the wave whose round holds it quantises it for itself, puts it into the round's
 // registers and writes it to the cache, so no wave waits for another.
@@ -195,13 +195,13 @@ __device__ __forceinline__ void merge_part(const DecodeArgs& a, const Partials& 
         float m = M;
 #pragma unroll
         for (int j = 0; j < kPartBatch; ++j) m = fmaxf(m, w[j].x);
-        if (m == -INFINITY) continue;  // no valid key in these
-        const float corr = fast_exp2(M - m);  // 0 while M = -inf
+        const float base = softmax_base(m);
+        const float corr = fast_exp2(M - base);  // 0 while M = -inf
         L *= corr;
         O *= corr;
 #pragma unroll
         for (int j = 0; j < kPartBatch; ++j) {
-            const float f = fast_exp2(w[j].x - m);  // 0 past the last
+            const float f = fast_exp2(w[j].x - base);  // 0 past the last
             L = fmaf(f, w[j].y, L);
 #pragma unroll
             for (int i = 0; i < 4; ++i) O[i] = fmaf(f, o[j][i], O[i]);
@@ -230,18 +230,17 @@ __device__ __forceinline__ void merge_heads(const DecodeArgs& a, const Partials&
         const int g = idx / D, d = idx - g * D;
         const float2* const ml = lds_ml + g * kMergeParts;
         const float M = fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x));
+        const float base = softmax_base(M);
         float O = 0.f, L = 0.f;
-        if (M != -INFINITY) {
 #pragma unroll
-            for (int p = 0; p < kMergeParts; ++p) {
-                const float f = fast_exp2(ml[p].x - M);  // 0 for an empty part
-                O = fmaf(f, lds_o[(g * kMergeParts + p) * D + d], O);
-                L = fmaf(f, ml[p].y, L);
-            }
+        for (int p = 0; p < kMergeParts; ++p) {
+            const float f = fast_exp2(ml[p].x - base);  // 0 for an empty part
+            O = fmaf(f, lds_o[(g * kMergeParts + p) * D + d], O);
+            L = fmaf(f, ml[p].y, L);
         }
         const size_t row = (size_t)b * H_q + h * a.group + g0 + g;
-        a.out[row * D + d] = f32_to_bf16_rne(L > 0.f ? O / L : 0.f);
-        if (d == 0 && a.lse != nullptr) a.lse[row] = L > 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
+        a.out[row * D + d] = f32_to_bf16_rne(softmax_out(O, L));
+        if (d == 0 && a.lse != nullptr) a.lse[row] = softmax_lse(M, L);
     }
 }
 
@@ -623,20 +622,19 @@ __global__ __launch_bounds__(kv8_waves(DIRECT) * 64, DIRECT ? 4 : 2) void decode
             float M = -INFINITY;
 #pragma unroll
             for (int w = 0; w < NW; ++w) M = fmaxf(M, lds_ml[w * G + g].x);
+            const float base = softmax_base(M);
             float O = 0.f, Ls = 0.f;
-            if (M != -INFINITY) {
 #pragma unroll
-                for (int w = 0; w < NW; ++w) {
-                    const float2 ml = lds_ml[w * G + g];
-                    const float f = fast_exp2(ml.x - M);  // 0 for a wave without rounds
-                    O = fmaf(f, lds_o[(w * G + g) * OS + d], O);
-                    Ls = fmaf(f, ml.y, Ls);
-                }
+            for (int w = 0; w < NW; ++w) {
+                const float2 ml = lds_ml[w * G + g];
+                const float f = fast_exp2(ml.x - base);  // 0 for a wave without rounds
+                O = fmaf(f, lds_o[(w * G + g) * OS + d], O);
+                Ls = fmaf(f, ml.y, Ls);
             }
             if (whole) {
                 const size_t to = (size_t)seg.b * H_q + seg.h * G + g;
-                a.out[to * D + d] = f32_to_bf16_rne(Ls > 0.f ? O / Ls : 0.f);
-                if (d == 0 && a.lse != nullptr) a.lse[to] = Ls > 0.f ? (M + log2f(Ls)) * kLn2 : -INFINITY;
+                a.out[to * D + d] = f32_to_bf16_rne(softmax_out(O, Ls));
+                if (d == 0 && a.lse != nullptr) a.lse[to] = softmax_lse(M, Ls);
             } else {
                 const size_t to = slot + g;
                 if (DIRECT && a.arrivals != nullptr) {  // agent-scope stores: seen across the XCDs without an L2 write-back
