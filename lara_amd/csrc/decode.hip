@@ -151,14 +151,14 @@ __device__ __forceinline__ void merge_splits_parallel(const DecodeArgs& a, int u
             float bm = M[k];
 #pragma unroll
             for (int j = 0; j < kMergeBatch; ++j) bm = fmaxf(bm, ml[j].x);
-            if (bm == -INFINITY) continue;  // no valid key in these splits yet
-            const float corr = fast_exp2(M[k] - bm);  // 0 while M = -inf
+            const float from = softmax_base(bm);
+            const float corr = fast_exp2(M[k] - from);  // 0 while M = -inf
             L[k] *= corr;
 #pragma unroll
             for (int i = 0; i < 8; ++i) O[k][i] *= corr;
 #pragma unroll
             for (int j = 0; j < kMergeBatch; ++j) {
-                const float w = fast_exp2(ml[j].x - bm);  // 0 for a split past n_splits
+                const float w = fast_exp2(ml[j].x - from);  // 0 for a split past n_splits
                 L[k] = fmaf(w, ml[j].y, L[k]);
                 O[k][0] = fmaf(w, lo[j].x, O[k][0]);
                 O[k][1] = fmaf(w, lo[j].y, O[k][1]);
@@ -191,18 +191,17 @@ __device__ __forceinline__ void merge_splits_parallel(const DecodeArgs& a, int u
         float Mx = -INFINITY;
 #pragma unroll
         for (int w = 0; w < NW; ++w) Mx = fmaxf(Mx, lds_m[w][gl]);
+        const float from = softmax_base(Mx);
         float Ov = 0.f, Ls = 0.f;
-        if (Mx != -INFINITY) {
 #pragma unroll
-            for (int w = 0; w < NW; ++w) {
-                const float sc = fast_exp2(lds_m[w][gl] - Mx);  // 0 for a wave without splits
-                Ov = fmaf(sc, lds_o[w][gl][d], Ov);
-                Ls = fmaf(sc, lds_l[w][gl], Ls);
-            }
+        for (int w = 0; w < NW; ++w) {
+            const float sc = fast_exp2(lds_m[w][gl] - from);  // 0 for a wave without splits
+            Ov = fmaf(sc, lds_o[w][gl][d], Ov);
+            Ls = fmaf(sc, lds_l[w][gl], Ls);
         }
         const size_t row = (size_t)b * H_q + h * G + g0 + gl;
-        a.out[row * D + d] = f32_to_bf16_rne(Ls > 0.f ? Ov / Ls : 0.f);
-        if (d == 0 && a.lse != nullptr) a.lse[row] = Ls > 0.f ? (Mx + log2f(Ls)) * kLn2 : -INFINITY;
+        a.out[row * D + d] = f32_to_bf16_rne(softmax_out(Ov, Ls));
+        if (d == 0 && a.lse != nullptr) a.lse[row] = softmax_lse(Mx, Ls);
     }
 }
 
@@ -454,19 +453,18 @@ __global__ __launch_bounds__(NW * 64) void decode_split_kernel(DecodeArgs a) {
         float M = -INFINITY;
 #pragma unroll
         for (int w = 0; w < NW; ++w) M = fmaxf(M, lds_m[w][g]);
+        const float from = softmax_base(M);
         float O = 0.f, Ls = 0.f;
-        if (M != -INFINITY) {
 #pragma unroll
-            for (int w = 0; w < NW; ++w) {
-                const float sc = fast_exp2(lds_m[w][g] - M);
-                O = fmaf(sc, lds_o[w][g][d], O);
-                Ls = fmaf(sc, lds_l[w][g], Ls);
-            }
+        for (int w = 0; w < NW; ++w) {
+            const float sc = fast_exp2(lds_m[w][g] - from);  // 0 for a wave without rounds
+            O = fmaf(sc, lds_o[w][g][d], O);
+            Ls = fmaf(sc, lds_l[w][g], Ls);
         }
         if (single) {
             const size_t row = (size_t)b * H_q + h * G + g;
-            a.out[row * D + d] = f32_to_bf16_rne(Ls > 0.f ? O / Ls : 0.f);
-            if (d == 0 && a.lse != nullptr) a.lse[row] = Ls > 0.f ? (M + log2f(Ls)) * kLn2 : -INFINITY;
+            a.out[row * D + d] = f32_to_bf16_rne(softmax_out(O, Ls));
+            if (d == 0 && a.lse != nullptr) a.lse[row] = softmax_lse(M, Ls);
         } else {
             const size_t pidx = ((size_t)unit * a.max_splits + split) * G + g;
             if (fused_merge) {

@@ -79,3 +79,8 @@ def decode_non_finite(kv_format, plan):
 @pytest.mark.parametrize("plan", DECODE_PLANS)
 def test_e4m3_decode(plan):
     decode_non_finite("e4m3", plan)
+
+
+@pytest.mark.parametrize("plan", DECODE_PLANS)
+def test_bf16_decode(plan):
+    decode_non_finite("bf16", plan)
