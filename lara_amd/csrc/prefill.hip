@@ -55,6 +55,11 @@ constexpr int kWaves = 8;   // waves per work-group: (row block, head) tasks, he
 constexpr int kStages = 3;  // LDS ring depth: two blocks in flight behind the one computed
 constexpr float kLn2 = 0.693147180559945309f;
 
+// 1 / l of a row's softmax sum l, and its natural-log sum: 0 and -inf without keys (l is 1 at least where there is a score
+// that is a number), NaN with a score of NaN.
+__device__ __forceinline__ float row_inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
+__device__ __forceinline__ float row_lse(float m, float l) { return l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2; }
+
 __device__ __forceinline__ f32x16 mfma32(const u32x4& a, const u32x4& b, const f32x16& c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b),
                                                    c, 0, 0, 0);
@@ -626,8 +631,8 @@ __global__ __launch_bounds__(kWaves * 64) void prefill_kernel(PrefillArgs a) {
     float lse_s = -INFINITY;  // PAIR: S's log-sum-exp (lanes of the first half-wave)
     auto leave_s = [&]() __attribute__((always_inline)) {
         const float l_row = l_lane + half_swap(l_lane, half);
-        const float inv = l_row > 0.f ? 1.f / l_row : 0.f;
-        lse_s = l_row > 0.f ? (m_run + log2f(l_row)) * kLn2 : -INFINITY;
+        const float inv = row_inverse(l_row);
+        lse_s = row_lse(m_run, l_row);
         const int q4 = wave & 3;
         // L's Q^T first: the stash below takes its place.
 #pragma unroll
@@ -758,7 +763,7 @@ __global__ __launch_bounds__(kWaves * 64) void prefill_kernel(PrefillArgs a) {
             const float l_sum = fmaf(l_row, wa, mlb.y * wb);
             // Every lane stages its row (rows past q_len too: the stores skip them), since the row
             // stores below take each lane to other rows.
-            const float inv = l_sum > 0.f ? 1.f / l_sum : 0.f;
+            const float inv = row_inverse(l_sum);
             // L's rows are staged in ring stage 3 (the partials and their (m, l) fill stages 0-2).
             uint2* stash = reinterpret_cast<uint2*>(q4 < 2 ? &lds_k[NST - 1][0] : &lds_v[NST - 1][0]) +
                            (q4 & 1) * (kRows * NCH * 2);
@@ -778,7 +783,7 @@ __global__ __launch_bounds__(kWaves * 64) void prefill_kernel(PrefillArgs a) {
                 }
             stash_store_rows<D, 1>(stash, a.out + (size_t)hq * a.q_len * D, rb * kRows, a.q_len, lane);
             if (row_ok && half == 0 && a.lse != nullptr)
-                a.lse[(size_t)hq * a.q_len + row] = l_sum > 0.f ? (M + log2f(l_sum)) * kLn2 : -INFINITY;
+                a.lse[(size_t)hq * a.q_len + row] = row_lse(M, l_sum);
         } else if (has_s) {
             // S's output rows from the stash leave_s filled.
             stash_store_rows<D, 1>(reinterpret_cast<const uint2*>(&lds_q[q4][0][0]), a.out + (size_t)hq * a.q_len * D,
@@ -813,7 +818,7 @@ __global__ __launch_bounds__(kWaves * 64) void prefill_kernel(PrefillArgs a) {
     // lane of the wave stages its row (rows past q_len too: the stores skip them).
     const int f = (n_blocks + (wave >> 2)) % NST;
     uint2* stash = reinterpret_cast<uint2*>((wave & 2) ? &lds_v[f][0] : &lds_k[f][0]) + (wave & 1) * (kRows * NCH * 2);
-    const float inv = l_row > 0.f ? 1.f / l_row : 0.f;
+    const float inv = row_inverse(l_row);
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -825,7 +830,7 @@ __global__ __launch_bounds__(kWaves * 64) void prefill_kernel(PrefillArgs a) {
         }
     stash_store_rows<D, G>(stash, a.out + (size_t)h * G * a.q_len * D, task * kRows, a.q_len, lane);
     if (row_ok && half == 0 && a.lse != nullptr)
-        a.lse[(size_t)hq * a.q_len + row] = l_row > 0.f ? (m_run + log2f(l_row)) * kLn2 : -INFINITY;
+        a.lse[(size_t)hq * a.q_len + row] = row_lse(m_run, l_row);
 }
 
 // ---- Row-block prefill for launches too small to fill the GPU ------------------------------
@@ -1257,7 +1262,7 @@ __global__ __launch_bounds__(NW * 64) void prefill_rows_kernel(PrefillArgs a) {
             wt[w] = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - M);
             L = fmaf(wt[w], lds_ml[n][w][1][r], L);
         }
-        const float inv = L > 0.f ? 1.f / L : 0.f;
+        const float inv = row_inverse(L);
         uint16_t* orow = a.out + ((size_t)(hq + n) * a.q_len + out_row) * D + dg * DPT;
 #pragma unroll
         for (int d8 = 0; d8 < DPT; d8 += 8) {
@@ -1287,7 +1292,7 @@ __global__ __launch_bounds__(NW * 64) void prefill_rows_kernel(PrefillArgs a) {
             *reinterpret_cast<uint4*>(orow + d8) = wv;
         }
         if (dg == 0 && a.lse != nullptr)
-            a.lse[(size_t)(hq + n) * a.q_len + out_row] = L > 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
+            a.lse[(size_t)(hq + n) * a.q_len + out_row] = row_lse(M, L);
     }
 }
 
@@ -1357,14 +1362,14 @@ __global__ __launch_bounds__(kMergeRows * D / 8) void prefill_combine_kernel(Pre
             }
         }
     }
-    const float inv = L > 0.f ? 1.f / L : 0.f;
+    const float inv = row_inverse(L);
     uint4 w;
     w.x = (uint32_t)f32_to_bf16_rne(O[0] * inv) | ((uint32_t)f32_to_bf16_rne(O[1] * inv) << 16);
     w.y = (uint32_t)f32_to_bf16_rne(O[2] * inv) | ((uint32_t)f32_to_bf16_rne(O[3] * inv) << 16);
     w.z = (uint32_t)f32_to_bf16_rne(O[4] * inv) | ((uint32_t)f32_to_bf16_rne(O[5] * inv) << 16);
     w.w = (uint32_t)f32_to_bf16_rne(O[6] * inv) | ((uint32_t)f32_to_bf16_rne(O[7] * inv) << 16);
     *reinterpret_cast<uint4*>(a.out + prow * D + 8 * d8) = w;
-    if (d8 == 0 && a.lse != nullptr) a.lse[prow] = L > 0.f ? (M + log2f(L)) * kLn2 : -INFINITY;
+    if (d8 == 0 && a.lse != nullptr) a.lse[prow] = row_lse(M, L);
 }
 
 // Tasks of a kv head: 32 (query row, head) pairs each.

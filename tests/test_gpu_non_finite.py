@@ -84,3 +84,50 @@ def test_e4m3_decode(plan):
 @pytest.mark.parametrize("plan", DECODE_PLANS)
 def test_bf16_decode(plan):
     decode_non_finite("bf16", plan)
+
+
+PREFILL_KERNELS = {"rows": _lib.GQA_PREFILL_KERNEL_ROWS, "shared": _lib.GQA_PREFILL_KERNEL_SHARED,
+                   "paired": _lib.GQA_PREFILL_KERNEL_PAIRED, "segments": _lib.GQA_PREFILL_KERNEL_SHARED}
+
+
+@pytest.mark.parametrize("kv_format", ["bf16", "e4m3"])
+@pytest.mark.parametrize("kernel", PREFILL_KERNELS)
+def test_prefill(kernel, kv_format):
+    """Causal blocks: some query rows of NaN (one of them without keys), then a key of NaN, which the rows before it do not
+    see."""
+    rng = np.random.default_rng(29)
+    hq, hkv, d, n, history, kv_pos = 8, 2, 64, 70, 90, 100
+    kv_len = history + n
+    q, k, v = (bf16_normal(rng, (h, m, d)) for h, m in ((hq, n), (hkv, kv_len), (hkv, kv_len)))
+    with AttentionAccelerator(n_q_heads=hq, n_kv_heads=hkv, head_dim=d, max_seq_len=kv_len, max_q_len=n,
+                              kv_format=kv_format) as acc:
+        call("gqa_set_option", acc._ctx, _lib.GQA_OPT_PREFILL_KERNEL, PREFILL_KERNELS[kernel])
+        if kernel == "segments":
+            call("gqa_set_option", acc._ctx, _lib.GQA_OPT_PREFILL_WGS, 64)
+
+        def block(q, k, q_pos_base):
+            acc.load_kv(k, v)
+            o, lse = acc.prefill_chunk(q, q_pos_base=q_pos_base, kv_len=kv_len, kv_pos_base=kv_pos, causal=True, return_lse=True)
+            return orc.bf16_u16_to_fp32(o), lse
+
+        def check(got, clean, want):
+            want_o = np.repeat(want[..., None], d, -1)
+            assert np.array_equal(np.isnan(got[0]), want_o) and np.array_equal(np.isnan(got[1]), want)
+            assert np.array_equal(got[0][~want_o], clean[0][~want_o]) and np.array_equal(got[1][~want], clean[1][~want])
+
+        bad = q.copy()
+        want = np.zeros((hq, n), bool)
+        bad[0, 0, 3] = bad[2, 31, 0] = bad[5, 64, 63] = bad[7, n - 1, 9] = NAN
+        want[2, 31] = want[5, 64] = want[7, n - 1] = True
+        q_pos = kv_pos - 1  # row 0 is before the first key: no scores, so no NaN either
+        clean = block(q, k, q_pos)
+        assert not clean[0][:, 0].any() and np.all(clean[1][:, 0] == -np.inf)
+        check(block(bad, k, q_pos), clean, want)
+        q_pos = kv_pos + history  # the rows follow the keys
+        want[0, 0] = True
+        check(block(bad, k, q_pos), block(q, k, q_pos), want)
+        bad = k.copy()
+        bad[1, history + 40, 11] = NAN
+        want = np.zeros((hq, n), bool)
+        want[hq // hkv:, 40:] = True
+        check(block(q, bad, q_pos), block(q, k, q_pos), want)
