@@ -1855,6 +1855,8 @@ int gqa_load_kv_device(gqa_ctx* c, int32_t b, int32_t start_pos, int32_t n, cons
     if (b < 0 || b >= c->cfg.batch) return GQA_ERR_STREAM_DEST;
     if (n < 0 || start_pos < 0 || (int64_t)start_pos + n > c->cfg.max_seq_len) return GQA_ERR_RANGE;
     if (n == 0) return GQA_OK;
+    const DeviceScope device(c->cfg.device);
+    HIP_TRY(device.status);
     hipStream_t s = pick_stream(c, stream);
     if (c->kv8) {
         if (!aligned16(k) || !aligned16(v) || !rows_backed(c, b, start_pos, n)) return GQA_ERR_RANGE;
@@ -1957,6 +1959,8 @@ int gqa_append_kv(gqa_ctx* c, const uint16_t* k_rows, const uint16_t* v_rows, co
 int gqa_append_kv_device(gqa_ctx* c, const void* k_rows, const void* v_rows, const int32_t* positions,
                          void* stream) {
     if (!c || !k_rows || !v_rows || !positions) return GQA_ERR_NULL;
+    const DeviceScope device(c->cfg.device);
+    HIP_TRY(device.status);
     hipStream_t s = pick_stream(c, stream);
     if (c->kv8) {
         if (!aligned16(k_rows) || !aligned16(v_rows)) return GQA_ERR_RANGE;
@@ -2008,6 +2012,8 @@ int gqa_decode(gqa_ctx* c, const uint16_t* q, const int32_t* ctx_lens, uint16_t*
 int gqa_decode_device(gqa_ctx* c, const void* q, const int32_t* ctx_lens, void* o, float* lse, void* stream) {
     if (!c || !q || !ctx_lens || !o) return GQA_ERR_NULL;
     if (!aligned16(q)) return GQA_ERR_RANGE;
+    const DeviceScope device(c->cfg.device);
+    HIP_TRY(device.status);
     return run_decode(c, q, ctx_lens, nullptr, nullptr, nullptr, o, lse, pick_stream(c, stream), c->cfg.max_seq_len);
 }
 
@@ -2051,6 +2057,8 @@ int gqa_decode_append_device(gqa_ctx* c, const void* q, const void* k_rows, cons
                              const int32_t* positions, const int32_t* ctx_lens, void* o, float* lse, void* stream) {
     if (!c || !q || !k_rows || !v_rows || !positions || !ctx_lens || !o) return GQA_ERR_NULL;
     if (!aligned16(q) || !aligned16(k_rows) || !aligned16(v_rows)) return GQA_ERR_RANGE;
+    const DeviceScope device(c->cfg.device);
+    HIP_TRY(device.status);
     return run_decode(c, q, ctx_lens, k_rows, v_rows, positions, o, lse, pick_stream(c, stream),
                       c->cfg.max_seq_len);
 }
@@ -2180,6 +2188,8 @@ int gqa_prefill_append_device(gqa_ctx* c, int32_t b, const void* q, const void* 
     if (rc != GQA_OK) return rc;
     if (!rows_backed(c, b, 0, kv_len)) return GQA_ERR_RANGE;
     if (n_new < 1 || n_new > kv_len) return GQA_ERR_RANGE;
+    const DeviceScope device(c->cfg.device);
+    HIP_TRY(device.status);
     return run_prefill(c, b, q, q_len, q_pos_base, kv_len, kv_pos_base, causal, o, lse, pick_stream(c, stream),
                        k_rows, v_rows, n_new);
 }
@@ -2191,6 +2201,8 @@ int gqa_prefill_device(gqa_ctx* c, int32_t b, const void* q, int32_t q_len, int3
     int rc = check_prefill_args(c, b, q_len, q_pos_base, kv_len, kv_pos_base);
     if (rc != GQA_OK) return rc;
     if (!rows_backed(c, b, 0, kv_len)) return GQA_ERR_RANGE;
+    const DeviceScope device(c->cfg.device);
+    HIP_TRY(device.status);
     return run_prefill(c, b, q, q_len, q_pos_base, kv_len, kv_pos_base, causal, o, lse, pick_stream(c, stream));
 }
 

@@ -1,0 +1,113 @@
+"""The engine's host code against a HIP runtime that runs nothing (tests/hip_stub.cpp): which device is current where
+something is launched or allocated, what follows a failed allocation or launch, and whether launches keep to the
+runtime's limits.  On the CPU; every scenario is a process of its own.
+"""
+import ctypes
+import shutil
+import subprocess
+import sys
+from pathlib import Path
+
+import pytest
+
+ROOT = Path(__file__).resolve().parents[1]
+P = ctypes.c_void_p
+
+
+class Engine:
+    """libgqa.so over the stub, and an E4M3 context on device 1 while device 0 is current."""
+
+    def __init__(self, stub, kv8=True, page=0, **cfg):
+        sys.path.insert(0, str(ROOT))
+        self.stub = ctypes.CDLL(stub, mode=ctypes.RTLD_GLOBAL)
+        self.stub.stub_take_log.restype = ctypes.c_char_p
+        self.stub.stub_fail_malloc_above.argtypes = [ctypes.c_size_t]
+        from lara_amd import _lib
+
+        self._lib, self.lib = _lib, _lib.lib()
+        kw = dict(batch=2, n_q_heads=8, n_kv_heads=2, head_dim=64, max_seq_len=300, max_q_len=64, scale=0.0, device=1)
+        kw.update(cfg)
+        self.cfg = kw
+        c, self.ctx = _lib.GqaConfig(**kw), P()
+        if kv8:
+            n_pages = kw["batch"] * -(-kw["max_seq_len"] // page) if page else 0
+            self.ok("gqa_create_kv8", ctypes.byref(c), page, n_pages, 1, ctypes.byref(self.ctx))
+        else:
+            self.ok("gqa_create", ctypes.byref(c), ctypes.byref(self.ctx))
+        self.stub.hipSetDevice(0)
+        self.log()
+
+    def call(self, name, *args):
+        return getattr(self.lib, name)(*args)
+
+    def ok(self, name, *args):
+        rc = self.call(name, *args)
+        assert rc == 0, (name, rc)
+
+    def log(self):
+        return [line.split() for line in self.stub.stub_take_log().decode().splitlines()]
+
+
+DEV = P(0x10000)  # a device operand: the stub's kernels read nothing
+OUT = P(0x90000000)
+
+
+def kernels(log):
+    return [line[2] for line in log if line[1] == "launch"]
+
+
+# ---- scenarios -------------------------------------------------------------------------------------------
+
+def device_of_calls(stub):
+    """Device entry points of an E4M3 context work on its device whichever is current, and leave that one current."""
+    e = Engine(stub)
+    c = e.ctx
+    calls = [
+        ("gqa_load_kv_device", c, 0, 0, 100, DEV, DEV, None),
+        ("gqa_append_kv_device", c, DEV, DEV, DEV, None),
+        ("gqa_read_kv_device", c, 0, 0, 100, DEV, OUT, None),
+        ("gqa_decode_device", c, DEV, DEV, OUT, None, None),
+        ("gqa_decode_append_device", c, DEV, DEV, DEV, DEV, DEV, OUT, None, None),
+        ("gqa_prefill_device", c, 0, DEV, 20, 80, 100, 0, 1, OUT, None, None),
+        ("gqa_prefill_append_device", c, 0, DEV, DEV, DEV, 20, 20, 80, 100, 0, 1, OUT, None, None),
+        ("gqa_qk_norm_rope_device", c, 0, DEV, 768, 4, None, None, 1e-6, 0, 0, 0, 1e4, OUT, None),
+        ("gqa_qk_norm_rope_step_device", c, DEV, 768, None, None, 1e-6, DEV, None, 1e4, OUT, None),
+    ]
+    for name, *args in calls:
+        e.ok(name, *args)
+        log = e.log()
+        assert kernels(log), name
+        assert all(line[0] == "1" for line in log), (name, log)
+        assert e.stub.stub_device() == 0, name
+    # a longer history grows the workspace: what it frees and waits for is on that device too
+    e = Engine(stub, max_seq_len=1 << 15)
+    for kv_len in (100, 1 << 15):
+        e.ok("gqa_prefill_device", e.ctx, 0, DEV, 20, kv_len - 20, kv_len, 0, 1, OUT, None, None)
+        log = e.log()
+        assert any(line[1] == "hipMalloc" for line in log) and all(line[0] == "1" for line in log), log
+        assert e.stub.stub_device() == 0
+    assert {"hipDeviceSynchronize", "hipFree"} <= {line[1] for line in log}
+
+
+SCENARIOS = {f.__name__: f for f in (device_of_calls,)}
+
+
+@pytest.fixture(scope="module")
+def stub(tmp_path_factory):
+    if shutil.which("g++") is None:
+        pytest.skip("needs g++")
+    so = tmp_path_factory.mktemp("hip_stub") / "libhip_stub.so"
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-shared", "-fPIC", "-D__HIP_PLATFORM_AMD__",
+                    "-I/opt/rocm/include", str(ROOT / "tests" / "hip_stub.cpp"), "-o", str(so)], check=True, timeout=120)
+    return so
+
+
+@pytest.mark.parametrize("name", SCENARIOS)
+def test_scenario(stub, name):
+    run = subprocess.run([sys.executable, str(Path(__file__).resolve()), str(stub), name], capture_output=True, text=True,
+                         timeout=60)
+    assert run.returncode == 0, run.stdout + run.stderr
+
+
+if __name__ == "__main__":
+    SCENARIOS[sys.argv[2]](sys.argv[1])
