@@ -943,6 +943,7 @@ int ensure_buffer(uint8_t** buf, size_t* cap, size_t bytes) {
         *cap = 0;
     }
     if (hipMalloc(buf, bytes) != hipSuccess) {
+        (void)hipGetLastError();  // else the next launch reports it
         *buf = nullptr;
         return GQA_ERR_OOM;
     }
@@ -1342,7 +1343,9 @@ int create_ctx(const gqa_config* cfg, int32_t page_size, int32_t n_pages, int32_
     int rc = GQA_OK;
     auto alloc = [&](void** p, size_t bytes) {
         if (rc != GQA_OK) return;
-        if (hipMalloc(p, bytes) != hipSuccess) rc = GQA_ERR_OOM;
+        if (hipMalloc(p, bytes) == hipSuccess) return;
+        (void)hipGetLastError();  // else the next launch, of another context, reports it
+        rc = GQA_ERR_OOM;
     };
     alloc((void**)&c->k_pool, kv_bytes(c) * (size_t)n_layers);
     alloc((void**)&c->v_pool, kv_bytes(c) * (size_t)n_layers);
@@ -1369,7 +1372,10 @@ int create_ctx(const gqa_config* cfg, int32_t page_size, int32_t n_pages, int32_
     alloc((void**)&c->rows_dev, 2 * units * D * 2);
     alloc((void**)&c->new_dev, 2 * (size_t)k.n_kv_heads * k.max_q_len * D * 2);
     if (c->paged) alloc((void**)&c->table_dev, (size_t)k.batch * c->max_pages * sizeof(int32_t));
-    if (rc == GQA_OK && hipHostMalloc((void**)&c->o_pinned, c->stage_words * 2, 0) != hipSuccess) rc = GQA_ERR_OOM;
+    if (rc == GQA_OK && hipHostMalloc((void**)&c->o_pinned, c->stage_words * 2, 0) != hipSuccess) {
+        (void)hipGetLastError();
+        rc = GQA_ERR_OOM;
+    }
     // A blocking stream: ordered both ways with the legacy default stream, so a caller that
     // passes NULL (for instance PyTorch's default stream, whose handle is 0) sees its own
     // earlier default-stream work finish before the library reads it, and vice versa.

@@ -89,7 +89,33 @@ def device_of_calls(stub):
     assert {"hipDeviceSynchronize", "hipFree"} <= {line[1] for line in log}
 
 
-SCENARIOS = {f.__name__: f for f in (device_of_calls,)}
+def workspace_of_the_exact_size(stub):
+    """Where the workspace rounded up cannot be had, calls go on with one of the size they need, and the failed allocation
+    is not reported by a launch behind it."""
+    e = Engine(stub, max_seq_len=1 << 16, max_q_len=1000)
+    rows = 40000  # K and V in bf16: 2 heads * 64 values * 2 * 2 bytes a row, 20.5 MB; rounded up 32 MiB
+    e.stub.stub_fail_malloc_above(24 << 20)
+    e.ok("gqa_prefill_device", e.ctx, 0, DEV, 20, rows - 20, rows, 0, 1, OUT, None, None)
+    log = e.log()
+    assert [int(line[2]) for line in log if line[1] == "hipMalloc"] == [32 << 20, rows * 512] and len(kernels(log)) >= 2
+    # nothing to be had at all: the call says so, and the next one that needs no more than is there runs
+    e.stub.stub_fail_malloc_above(0)
+    assert e.call("gqa_prefill_device", e.ctx, 0, DEV, 20, 60000, 60020, 0, 1, OUT, None, None) == e._lib.GQA_ERR_OOM
+    e.ok("gqa_decode_device", e.ctx, DEV, DEV, OUT, None, None)
+    e.stub.stub_fail_malloc_above(1 << 40)
+    e.ok("gqa_prefill_device", e.ctx, 0, DEV, 20, 60000, 60020, 0, 1, OUT, None, None)
+    # the layer stage's buffer of projected rows likewise
+    e.stub.stub_fail_malloc_above(0)
+    assert e.call("gqa_layer_qkv_device", e.ctx, 0, DEV, 1000, 512, DEV, DEV, DEV, None, 1e-5, 0, 0, 0, 1, OUT, None) == e._lib.GQA_ERR_OOM
+    e.ok("gqa_decode_device", e.ctx, DEV, DEV, OUT, None, None)
+    # a context that cannot be had leaves the others as they are
+    cfg, other = e._lib.GqaConfig(**e.cfg), P()
+    e.stub.stub_fail_malloc_above(1 << 20)
+    assert e.call("gqa_create_kv8", ctypes.byref(cfg), 0, 0, 1, ctypes.byref(other)) == e._lib.GQA_ERR_OOM and not other
+    e.ok("gqa_decode_device", e.ctx, DEV, DEV, OUT, None, None)
+
+
+SCENARIOS = {f.__name__: f for f in (device_of_calls, workspace_of_the_exact_size)}
 
 
 @pytest.fixture(scope="module")
