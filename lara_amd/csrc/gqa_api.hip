@@ -809,28 +809,46 @@ int run_prefill_rows(gqa_ctx* c, int32_t b, const PrefillRows& from, const void*
 
 int ensure_buffer(uint8_t** buf, size_t* cap, size_t bytes);
 
-// The E4M3 context's bf16 workspace for a use on s, at least `bytes` of it; done_kv8_ws ends the use.  There is one: a use
-// waits for the one before it wherever that was (uses on one stream follow each other anyway), so streams that take
-// turns are ordered by it.  Not under a capture: a graph replays beside uses that it knows nothing of.
-int take_kv8_ws(gqa_ctx* c, size_t bytes, hipStream_t s) {
-    if (stream_capturing(s)) return GQA_ERR_UNSUPPORTED;
-    if (bytes > c->kv8_ws_bytes) {  // in powers of two: a growing history does not allocate at each step
-        size_t grown = 1 << 20;
-        while (grown < bytes) grown *= 2;
-        int rc = ensure_buffer(&c->kv8_ws, &c->kv8_ws_bytes, grown);
-        if (rc == GQA_ERR_OOM) rc = ensure_buffer(&c->kv8_ws, &c->kv8_ws_bytes, bytes);
-        if (rc != GQA_OK) return rc;
+// A use of the E4M3 context's bf16 workspace on s, at least `bytes` of it, to the end of the object's life: whatever a
+// call has launched by then, after an error too.  There is one workspace: a use waits for the one before it wherever that
+// was (uses on one stream follow each other anyway), so streams that take turns are ordered by it.  Not under a capture: a
+// graph replays beside uses that it knows nothing of.
+class Kv8Workspace {
+  public:
+    Kv8Workspace(gqa_ctx* c, size_t bytes, hipStream_t s) : c_(c), s_(s), status_(take(bytes)) {}
+    ~Kv8Workspace() {
+        if (status_ != GQA_OK) return;
+        if (hipEventRecord(c_->ev_kv8_ws, s_) != hipSuccess) {  // (no mark to wait for: wait here)
+            (void)hipGetLastError();
+            (void)hipStreamSynchronize(s_);
+        }
+        c_->kv8_ws_stream = s_;
+        c_->kv8_ws_used = true;
     }
-    // (A caller's handle does not name a stream for good, so only the context's own stream goes without the wait.)
-    if (c->kv8_ws_used && !(s == c->stream && c->kv8_ws_stream == s)) HIP_TRY(hipStreamWaitEvent(s, c->ev_kv8_ws, 0));
-    return GQA_OK;
-}
-int done_kv8_ws(gqa_ctx* c, hipStream_t s) {
-    HIP_TRY(hipEventRecord(c->ev_kv8_ws, s));
-    c->kv8_ws_stream = s;
-    c->kv8_ws_used = true;
-    return GQA_OK;
-}
+    Kv8Workspace(const Kv8Workspace&) = delete;
+    Kv8Workspace& operator=(const Kv8Workspace&) = delete;
+    int status() const { return status_; }
+    uint16_t* rows() const { return (uint16_t*)c_->kv8_ws; }
+
+  private:
+    int take(size_t bytes) {
+        if (stream_capturing(s_)) return GQA_ERR_UNSUPPORTED;
+        if (bytes > c_->kv8_ws_bytes) {  // in powers of two: a growing history does not allocate at each step
+            size_t grown = 1 << 20;
+            while (grown < bytes) grown *= 2;
+            int rc = ensure_buffer(&c_->kv8_ws, &c_->kv8_ws_bytes, grown);
+            if (rc == GQA_ERR_OOM) rc = ensure_buffer(&c_->kv8_ws, &c_->kv8_ws_bytes, bytes);
+            if (rc != GQA_OK) return rc;
+        }
+        // (A caller's handle does not name a stream for good, so only the context's own stream goes without the wait.)
+        if (c_->kv8_ws_used && !(s_ == c_->stream && c_->kv8_ws_stream == s_))
+            HIP_TRY(hipStreamWaitEvent(s_, c_->ev_kv8_ws, 0));
+        return GQA_OK;
+    }
+    gqa_ctx* const c_;
+    const hipStream_t s_;
+    const int status_;
+};
 
 // Quantises bf16 rows [H_kv][n][D] into rows start .. of sequence b.
 hipError_t write_kv8(gqa_ctx* c, int b, int start, int n, const void* k, const void* v, hipStream_t s) {
@@ -874,15 +892,13 @@ int run_prefill(gqa_ctx* c, int32_t b, const void* q, int32_t q_len, int32_t q_p
     if (!prefill_supported(c->cfg.head_dim, c->group)) return GQA_ERR_UNSUPPORTED;
     const int cap = std::max(64, (kv_len + 63) / 64 * 64);
     const size_t side = (size_t)c->cfg.n_kv_heads * cap * D;
-    int rc = take_kv8_ws(c, 2 * side * 2, s);
-    if (rc != GQA_OK) return rc;
-    uint16_t* const k = (uint16_t*)c->kv8_ws;
+    const Kv8Workspace ws(c, 2 * side * 2, s);
+    if (ws.status() != GQA_OK) return ws.status();
+    uint16_t* const k = ws.rows();
     if (n_new > 0) HIP_TRY(write_kv8(c, b, kv_len - n_new, n_new, k_new, v_new, s));
     HIP_TRY(read_rows(c, b, 0, kv_len, cap, k, k + side, s));
-    rc = run_prefill_rows(c, b, PrefillRows{k, k + side, cap, nullptr}, q, q_len, q_pos_base, kv_len, kv_pos_base, causal, o,
-                          lse, s, nullptr, nullptr, 0);
-    const int done = done_kv8_ws(c, s);
-    return rc != GQA_OK ? rc : done;
+    return run_prefill_rows(c, b, PrefillRows{k, k + side, cap, nullptr}, q, q_len, q_pos_base, kv_len, kv_pos_base, causal, o,
+                            lse, s, nullptr, nullptr, 0);
 }
 
 int finish_sync(gqa_ctx* c) {
@@ -1220,25 +1236,17 @@ int run_layer_qkv(gqa_ctx* c, int32_t b, const void* x, int32_t n_tokens, int32_
 int run_layer_stage(gqa_ctx* c, int32_t b, const void* x, int32_t n_tokens, int32_t hidden, const void* wq, const void* wk,
                     const void* wv, const void* gamma, float eps, int32_t q_pos_base, int32_t kv_pos_base, int32_t row0,
                     int32_t rope, void* q_out, hipStream_t s, bool stage_events) {
-    uint16_t* rows = nullptr;
+    if (!c->kv8)
+        return run_layer_qkv(c, b, x, n_tokens, hidden, wq, wk, wv, gamma, eps, q_pos_base, kv_pos_base, row0, rope, q_out, s,
+                             stage_events);
     const size_t side = (size_t)n_tokens * c->cfg.n_kv_heads * c->cfg.head_dim;
-    if (c->kv8) {
-        const int rc = take_kv8_ws(c, 2 * side * 2, s);
-        if (rc != GQA_OK) return rc;
-        rows = (uint16_t*)c->kv8_ws;
-    }
-    int rc = run_layer_qkv(c, b, x, n_tokens, hidden, wq, wk, wv, gamma, eps, q_pos_base, kv_pos_base, row0, rope, q_out, s,
-                           stage_events, rows);
-    if (!c->kv8) return rc;
-    if (rc == GQA_OK) {
-        const hipError_t e = write_kv8(c, b, row0, n_tokens, rows, rows + side, s);
-        if (e != hipSuccess) {
-            last_hip_error(e, "quantising the layer's K/V rows");
-            rc = GQA_ERR_HIP;
-        }
-    }
-    const int done = done_kv8_ws(c, s);
-    return rc != GQA_OK ? rc : done;
+    const Kv8Workspace ws(c, 2 * side * 2, s);
+    if (ws.status() != GQA_OK) return ws.status();
+    const int rc = run_layer_qkv(c, b, x, n_tokens, hidden, wq, wk, wv, gamma, eps, q_pos_base, kv_pos_base, row0, rope, q_out,
+                                 s, stage_events, ws.rows());
+    if (rc != GQA_OK) return rc;
+    HIP_TRY(write_kv8(c, b, row0, n_tokens, ws.rows(), ws.rows() + side, s));
+    return GQA_OK;
 }
 
 int layer_times(gqa_ctx* c) {
@@ -1801,15 +1809,14 @@ int gqa_load_kv(gqa_ctx* c, int32_t b, int32_t start_pos, int32_t n, const uint1
         if (!rows_backed(c, b, start_pos, n)) return GQA_ERR_RANGE;
         if (c->paged) c->pages.touch(b);
         const size_t side = (size_t)c->cfg.n_kv_heads * n * c->cfg.head_dim;
-        rc = take_kv8_ws(c, 2 * side * 2, c->stream);
-        if (rc != GQA_OK) return rc;
-        uint16_t* const rows = (uint16_t*)c->kv8_ws;
+        const Kv8Workspace ws(c, 2 * side * 2, c->stream);
+        if (ws.status() != GQA_OK) return ws.status();
+        uint16_t* const rows = ws.rows();
         HIP_TRY(hipEventRecord(c->ev_begin, c->stream));
         HIP_TRY(hipMemcpyAsync(rows, k, side * 2, hipMemcpyHostToDevice, c->stream));
         HIP_TRY(hipMemcpyAsync(rows + side, v, side * 2, hipMemcpyHostToDevice, c->stream));
         HIP_TRY(write_kv8(c, b, start_pos, n, rows, rows + side, c->stream));
-        rc = done_kv8_ws(c, c->stream);
-        return rc != GQA_OK ? rc : finish_sync(c);
+        return finish_sync(c);
     }
     if (c->paged) {
         if (!rows_backed(c, b, start_pos, n)) return GQA_ERR_RANGE;
@@ -1898,14 +1905,12 @@ int gqa_read_kv(gqa_ctx* c, int32_t b, int32_t start_pos, int32_t n, uint16_t* k
     if (c->kv8) {
         if (!rows_backed(c, b, start_pos, n)) return GQA_ERR_RANGE;
         const size_t side = (size_t)c->cfg.n_kv_heads * n * c->cfg.head_dim;
-        rc = take_kv8_ws(c, 2 * side * 2, c->stream);
-        if (rc != GQA_OK) return rc;
-        uint16_t* const rows = (uint16_t*)c->kv8_ws;
+        const Kv8Workspace ws(c, 2 * side * 2, c->stream);
+        if (ws.status() != GQA_OK) return ws.status();
+        uint16_t* const rows = ws.rows();
         HIP_TRY(read_rows(c, b, start_pos, n, n, rows, rows + side, c->stream));
         HIP_TRY(hipMemcpyAsync(k, rows, side * 2, hipMemcpyDeviceToHost, c->stream));
         HIP_TRY(hipMemcpyAsync(v, rows + side, side * 2, hipMemcpyDeviceToHost, c->stream));
-        rc = done_kv8_ws(c, c->stream);
-        if (rc != GQA_OK) return rc;
         HIP_TRY(hipStreamSynchronize(c->stream));
         return GQA_OK;
     }

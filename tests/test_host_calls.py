@@ -115,7 +115,39 @@ def workspace_of_the_exact_size(stub):
     e.ok("gqa_decode_device", e.ctx, DEV, DEV, OUT, None, None)
 
 
-SCENARIOS = {f.__name__: f for f in (device_of_calls, workspace_of_the_exact_size)}
+def workspace_after_a_failed_launch(stub):
+    """Whichever launch of a call fails, the next use of the workspace on another stream waits for what the call had
+    launched before."""
+    e = Engine(stub)
+    host = (ctypes.c_uint16 * (2 * 300 * 64))()
+    other = P(0x777000)
+    calls = [
+        ("gqa_prefill_device", e.ctx, 0, DEV, 20, 80, 100, 0, 1, OUT, None, None),
+        ("gqa_prefill_append_device", e.ctx, 0, DEV, DEV, DEV, 20, 20, 80, 100, 0, 1, OUT, None, None),
+        ("gqa_layer_qkv_device", e.ctx, 0, DEV, 4, 1024, DEV, DEV, DEV, None, 1e-5, 0, 0, 0, 1, OUT, None),
+        ("gqa_load_kv", e.ctx, 0, 0, 300, host, host),
+        ("gqa_read_kv", e.ctx, 0, 0, 300, host, host),
+    ]
+    for name, *args in calls:
+        e.log()
+        e.ok(name, *args)
+        launches = len(kernels(e.log()))
+        assert launches >= 1, name
+        for at in range(launches):
+            e.stub.stub_fail_launch(at)
+            assert e.call(name, *args) == e._lib.GQA_ERR_HIP, (name, at)
+            log = e.log()
+            assert len(kernels(log)) == at + 1
+            failed = max(i for i, line in enumerate(log) if line[1] == "launch")
+            marks = [line[2] for line in log[failed:] if line[1] == "hipEventRecord"]
+            e.ok("gqa_prefill_device", e.ctx, 0, DEV, 20, 80, 100, 0, 1, OUT, None, other)
+            log = e.log()
+            first = min(i for i, line in enumerate(log) if line[1] == "launch")
+            waited = [line[2] for line in log[:first] if line[1] == "hipStreamWaitEvent"]
+            assert len(waited) == 1 and waited[0] in marks, (name, at, marks, waited)
+
+
+SCENARIOS = {f.__name__: f for f in (device_of_calls, workspace_of_the_exact_size, workspace_after_a_failed_launch)}
 
 
 @pytest.fixture(scope="module")
