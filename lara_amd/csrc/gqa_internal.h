@@ -5,6 +5,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 namespace lara {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -55,6 +57,14 @@ template <typename... KArgs, typename... Args>
 inline hipError_t launch_kernel(void (*kernel)(KArgs...), dim3 grid, dim3 block, const Launch& l, Args... args) {
     return launch_kernel_lds(kernel, grid, block, 0, l, args...);
 }
+
+// A grid of `wgs` work-groups (at most 2^31) and few more, in rows of up to 2^20: the runtime takes at most 2^32 - 1
+// work-items a dimension, 2^24 work-groups of 256.  wide_block() is a work-group's place in it.
+inline dim3 wide_grid(int64_t wgs) {
+    const int64_t rows = std::max<int64_t>(1, (wgs + (1 << 20) - 1) >> 20);
+    return dim3((uint32_t)((wgs + rows - 1) / rows), (uint32_t)rows);
+}
+__device__ __forceinline__ uint32_t wide_block() { return blockIdx.y * gridDim.x + blockIdx.x; }
 
 // Split-KV decode launch description.  All pointers are device pointers.
 struct DecodeArgs {

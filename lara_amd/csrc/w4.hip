@@ -32,7 +32,7 @@ __host__ __device__ inline int w4_groups(int hidden, int group) { return w4_bloc
 
 // codes [rows][hidden / 2] (the even column in the low half of a byte), scales [rows][hidden / group] bf16.
 __global__ __launch_bounds__(kW4Threads) void w4_pack_kernel(W4PackArgs a) {
-    const int64_t i = (int64_t)blockIdx.x * kW4Threads + threadIdx.x;  // a dword of the packed codes
+    const int64_t i = (int64_t)wide_block() * kW4Threads + threadIdx.x;  // a dword of the packed codes
     const int blocks = w4_blocks(a.hidden), tiles = (a.rows + 15) / 16;
     const int64_t dwords = (int64_t)tiles * blocks * 256;
     if (i < dwords) {
@@ -64,7 +64,7 @@ __global__ __launch_bounds__(kW4Threads) void w4_pack_kernel(W4PackArgs a) {
 
 // The packed matrix as bf16 [rows][hidden]: (c - 8) * s, one rounding.
 __global__ __launch_bounds__(kW4Threads) void w4_unpack_kernel(W4UnpackArgs a) {
-    const int64_t i = (int64_t)blockIdx.x * kW4Threads + threadIdx.x;
+    const int64_t i = (int64_t)wide_block() * kW4Threads + threadIdx.x;
     const int blocks = w4_blocks(a.hidden), tiles = (a.rows + 15) / 16;
     if (i >= (int64_t)tiles * blocks * 256) return;
     const int s = (int)(i & 3), lane = (int)(i >> 2) & 63;
@@ -315,7 +315,7 @@ int64_t w4_packed_bytes(int rows, int hidden) { return (int64_t)((rows + 15) / 1
 int64_t w4_scale_bytes(int rows, int hidden, int group) { return (int64_t)((rows + 15) / 16) * w4_groups(hidden, group) * 32; }
 
 static dim3 w4_grid(int rows, int hidden) {
-    return dim3((uint32_t)((w4_packed_bytes(rows, hidden) / 4 + kW4Threads - 1) / kW4Threads));
+    return wide_grid((w4_packed_bytes(rows, hidden) / 4 + kW4Threads - 1) / kW4Threads);
 }
 hipError_t launch_w4_pack(const W4PackArgs& a, const Launch& l) {
     return launch_kernel(w4_pack_kernel, w4_grid(a.rows, a.hidden), dim3(kW4Threads), l, a);

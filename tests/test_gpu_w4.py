@@ -292,3 +292,22 @@ def test_a_decode_step_of_all_operators():
                     ref, _, avg = so.decode(f64(q[b]).reshape(hq, d), caches[layer][0][b], caches[layer][1][b], eager.scale)
                     got_o = f64(o[b]).reshape(hq, d)
                     assert np.all(np.abs(got_o - ref) <= 2.0**-8 * np.abs(ref) + (2.0**-8 + 2.0**-13) * avg)
+
+
+@pytest.mark.parametrize("rows,hidden,group", [((1 << 15) + 7, 1 << 16, 32), (1 << 19, 1 << 12, 128)])
+def test_matrices_of_about_2_20_work_groups(acc, rows, hidden, group):
+    """Packed and unpacked again: every value of the matrix, rounded once."""
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    codes = torch.randint(0, 256, (rows, hidden // 2), dtype=torch.uint8, device="cuda", generator=gen)
+    scales = (0.01 * torch.randn((rows, hidden // group), device="cuda", generator=gen)).bfloat16()
+    wb, sb = w4.packed_bytes(rows, hidden, group)
+    w, s = torch.empty(wb, dtype=torch.uint8, device="cuda"), torch.empty(sb, dtype=torch.uint8, device="cuda")
+    out = torch.full((rows, hidden), float("nan"), dtype=torch.bfloat16, device="cuda")
+    acc.w4_pack_device(codes.data_ptr(), scales.data_ptr(), rows, hidden, group, w.data_ptr(), s.data_ptr())
+    acc.w4_unpack_device(w.data_ptr(), s.data_ptr(), rows, hidden, group, out.data_ptr())
+    torch.cuda.synchronize()
+    for at in range(0, rows, 4096):
+        two = codes[at:at + 4096]
+        c = torch.stack((two & 15, two >> 4), -1).view(two.shape[0], -1).float() - 8  # (8 codes times a bf16: exact in fp32)
+        want = (c.view(two.shape[0], -1, group) * scales[at:at + 4096].float()[..., None]).view(two.shape[0], -1).bfloat16()
+        assert torch.equal(out[at:at + 4096], want), at

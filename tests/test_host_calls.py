@@ -147,7 +147,22 @@ def workspace_after_a_failed_launch(stub):
             assert len(waited) == 1 and waited[0] in marks, (name, at, marks, waited)
 
 
-SCENARIOS = {f.__name__: f for f in (device_of_calls, workspace_of_the_exact_size, workspace_after_a_failed_launch)}
+def launches_of_the_largest_matrices(stub):
+    """Packing and unpacking 4-bit matrices up to the documented sizes keeps to the runtime's limit of 2^32 - 1 work-items a
+    dimension, with a work-item for every 8 codes."""
+    e = Engine(stub)
+    far = [P(i << 40) for i in range(1, 5)]
+    for rows, hidden, group in ((1 << 20, 1 << 16, 128), (1 << 20, 1 << 16, 32), ((1 << 19) + 1, 1 << 16, 64), (1, 32, 32), (1000, 4096, 128)):
+        threads = -(-rows // 16) * -(-hidden // 128) * 256
+        e.ok("gqa_w4_pack_device", e.ctx, far[0], far[1], rows, hidden, group, far[2], far[3], None)
+        e.ok("gqa_w4_unpack_device", e.ctx, far[2], far[3], rows, hidden, group, far[0], None)
+        for line in e.log():
+            x, y, _, block = (int(n) for n in line[4:8])
+            assert threads <= x * y * block < threads + 2 * block * y
+
+
+SCENARIOS = {f.__name__: f for f in (device_of_calls, workspace_of_the_exact_size, workspace_after_a_failed_launch,
+                                     launches_of_the_largest_matrices)}
 
 
 @pytest.fixture(scope="module")
