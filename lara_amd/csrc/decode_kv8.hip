@@ -680,8 +680,9 @@ __global__ __launch_bounds__(kv8_waves(DIRECT) * 64, DIRECT ? 4 : 2) void decode
 // The merge launch: a work-group per (sequence, kv head, head of the group).
 template <int D>
 __global__ __launch_bounds__(kMergeParts * D / 4) void decode_kv8_merge_kernel(DecodeArgs a) {
-    const int unit = blockIdx.x / a.group, g = blockIdx.x - unit * a.group;
+    const int block = wide_block(), unit = block / a.group, g = block - unit * a.group;
     const int b = unit / a.n_kv_heads, h = unit - b * a.n_kv_heads;
+    if (b >= a.batch) return;
     Partials from;
     if (a.max_splits > 0) {
         from = Partials::direct(a, unit, pieces_of(a, clamp_len(a.lens[b], a.l_max)));
@@ -727,7 +728,7 @@ hipError_t launch_decode_kv8(int head_dim, const DecodeArgs& a, const Launch& l)
 }
 
 hipError_t launch_decode_kv8_merge(int head_dim, const DecodeArgs& a, const Launch& l) {
-    const dim3 grid(a.batch * a.n_kv_heads * a.group), block(kMergeParts * head_dim / 4);
+    const dim3 grid = wide_grid((int64_t)a.batch * a.n_kv_heads * a.group), block(kMergeParts * head_dim / 4);
     if (head_dim == 128) return launch_kernel(decode_kv8_merge_kernel<128>, grid, block, l, a);
     if (head_dim == 64) return launch_kernel(decode_kv8_merge_kernel<64>, grid, block, l, a);
     return hipErrorInvalidValue;

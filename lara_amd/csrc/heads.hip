@@ -45,7 +45,9 @@ __device__ __forceinline__ float row_sum(float v) {
 template <int D, bool E4M3, int TOKENS>
 __global__ __launch_bounds__(kHeadsThreads) void qk_norm_rope_kernel(HeadsArgs a) {
     constexpr int LANES = D / 8, PAIRS = D / 2;
-    const int token0 = blockIdx.x * TOKENS, tokens = TOKENS == 1 || a.n_tokens - token0 >= TOKENS ? TOKENS : a.n_tokens - token0;
+    const int token0 = wide_block() * TOKENS;
+    if (token0 >= a.n_tokens) return;  // (the whole work-group)
+    const int tokens = TOKENS == 1 || a.n_tokens - token0 >= TOKENS ? TOKENS : a.n_tokens - token0;
     const int part = threadIdx.x % LANES;
     int b = a.b, pos0 = a.pos_base + token0, k_pos0 = a.k_pos_base + token0, t0 = a.row0 + token0;
     if (TOKENS == 1 && a.positions != nullptr) {  // one token of each sequence
@@ -143,7 +145,7 @@ __global__ __launch_bounds__(kHeadsThreads) void qk_norm_rope_kernel(HeadsArgs a
 
 template <int D, int TOKENS>
 static hipError_t launch_tokens(const HeadsArgs& a, const Launch& l) {
-    const dim3 grid((a.n_tokens + TOKENS - 1) / TOKENS), block(kHeadsThreads);
+    const dim3 grid = wide_grid((a.n_tokens + TOKENS - 1) / TOKENS), block(kHeadsThreads);
     return a.cache.k_scale != nullptr ? launch_kernel(qk_norm_rope_kernel<D, true, TOKENS>, grid, block, l, a)
                                       : launch_kernel(qk_norm_rope_kernel<D, false, TOKENS>, grid, block, l, a);
 }

@@ -18,7 +18,7 @@ constexpr int kKv8Threads = 256;
 template <int D>
 __global__ __launch_bounds__(kKv8Threads) void kv8_write_kernel(Kv8WriteArgs a) {
     constexpr int LANES = D / 8;
-    const int64_t i = ((int64_t)blockIdx.x * kKv8Threads + threadIdx.x) / LANES;
+    const int64_t i = ((int64_t)wide_block() * kKv8Threads + threadIdx.x) / LANES;
     const int part = threadIdx.x % LANES;
     if (i >= a.n_rows) return;  // (a row's lanes leave together)
     int b = a.b, t;
@@ -56,8 +56,9 @@ __global__ __launch_bounds__(kKv8Threads) void kv8_write_kernel(Kv8WriteArgs a) 
 template <int D, bool E4M3>
 __global__ __launch_bounds__(kKv8Threads) void kv_read_kernel(KvReadArgs a) {
     constexpr int LANES = D / 8;
-    const int h = blockIdx.x % a.cache.n_kv_heads, part = threadIdx.x % LANES;
-    const int64_t at = (int64_t)(blockIdx.x / a.cache.n_kv_heads) * (kKv8Threads / LANES) + threadIdx.x / LANES;
+    const uint32_t block = wide_block();
+    const int h = block % a.cache.n_kv_heads, part = threadIdx.x % LANES;
+    const int64_t at = (int64_t)(block / a.cache.n_kv_heads) * (kKv8Threads / LANES) + threadIdx.x / LANES;
     if (at >= a.n) return;
     const int t = (int)at;
     const int64_t row = kv8_row(a.cache, a.b, h, a.start + t);
@@ -94,7 +95,7 @@ hipError_t launch_kv8_write(int head_dim, const Kv8WriteArgs& a, const Launch& l
     if (a.n_rows < 1) return hipSuccess;
     const int64_t threads = a.n_rows * (head_dim / 8), wgs = (threads + kKv8Threads - 1) / kKv8Threads;
     if (wgs > 0x7FFFFFFF) return hipErrorInvalidValue;
-    const dim3 grid((uint32_t)wgs), block(kKv8Threads);
+    const dim3 grid = wide_grid(wgs), block(kKv8Threads);
     if (head_dim == 128) return launch_kernel(kv8_write_kernel<128>, grid, block, l, a);
     if (head_dim == 64) return launch_kernel(kv8_write_kernel<64>, grid, block, l, a);
     return hipErrorInvalidValue;
@@ -104,7 +105,7 @@ hipError_t launch_kv_read(int head_dim, const KvReadArgs& a, const Launch& l) {
     if (a.n < 1) return hipSuccess;
     const int64_t rows = kKv8Threads / (head_dim / 8), wgs = (a.n + rows - 1) / rows * a.cache.n_kv_heads;
     if (wgs > 0x7FFFFFFF) return hipErrorInvalidValue;
-    const dim3 grid((uint32_t)wgs), block(kKv8Threads);
+    const dim3 grid = wide_grid(wgs), block(kKv8Threads);
     const bool e4m3 = a.cache.k_scale != nullptr;
     if (head_dim == 128)
         return e4m3 ? launch_kernel(kv_read_kernel<128, true>, grid, block, l, a)

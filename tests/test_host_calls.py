@@ -158,11 +158,40 @@ def launches_of_the_largest_matrices(stub):
         e.ok("gqa_w4_unpack_device", e.ctx, far[2], far[3], rows, hidden, group, far[0], None)
         for line in e.log():
             x, y, _, block = (int(n) for n in line[4:8])
-            assert threads <= x * y * block < threads + 2 * block * y
+            assert threads <= x * y * block < threads + (block if y == 1 else block << 16)
+
+
+def launches_of_the_longest_caches(stub):
+    """Rows written and read back, heads and the decode merge at sizes whose work-items pass 2^32."""
+    n = 1 << 28
+    e = Engine(stub, batch=1, max_seq_len=n)
+    far = [P((1 << 56) + (i << 48)) for i in range(4)]
+
+    def blocks(kernel, least):
+        (line,) = [line for line in e.log() if line[1] == "launch" and kernel in line[2]]
+        x, y = int(line[4]), int(line[5])
+        assert least <= x * y < least + (1 << 16), line
+
+    e.ok("gqa_load_kv_device", e.ctx, 0, 0, n, far[0], far[1], None)
+    blocks("kv8_write", 2 * n * 8 // 256)
+    e.ok("gqa_read_kv_device", e.ctx, 0, 0, n, far[0], far[1], None)
+    blocks("kv_read", 2 * n * 8 // 256)
+    e.ok("gqa_prefill_device", e.ctx, 0, far[0], 20, n - 20, n, 0, 1, far[2], None, None)
+    blocks("kv_read", 2 * n * 8 // 256)
+    e.ok("gqa_qk_norm_rope_device", e.ctx, 0, far[0], 768, n, None, None, 1e-6, 0, 0, 0, 1e4, far[2], None)
+    blocks("qk_norm_rope", n // 2)  # (two tokens a work-group)
+    bf16 = Engine(stub, kv8=False, batch=1, n_q_heads=1, n_kv_heads=1, head_dim=128, max_seq_len=1 << 24)
+    bf16.ok("gqa_read_kv_device", bf16.ctx, 0, 0, 1 << 24, far[0], far[1], None)
+    bf16.ok("gqa_qk_norm_rope_device", bf16.ctx, 0, far[0], 384, 1 << 24, None, None, 1e-6, 0, 0, 0, 1e4, far[2], None)
+    many = Engine(stub, batch=1 << 20, n_q_heads=64, n_kv_heads=4, max_seq_len=64, max_q_len=1)
+    many.ok("gqa_decode_device", many.ctx, far[0], far[1], far[2], None, None)
+    assert "merge" in kernels(many.log())[-1]
+    many.ok("gqa_qk_norm_rope_step_device", many.ctx, far[0], 72 * 64, None, None, 1e-6, far[1], None, 1e4, far[2], None)
+    many.ok("gqa_append_kv_device", many.ctx, far[0], far[1], far[2], None)
 
 
 SCENARIOS = {f.__name__: f for f in (device_of_calls, workspace_of_the_exact_size, workspace_after_a_failed_launch,
-                                     launches_of_the_largest_matrices)}
+                                     launches_of_the_largest_matrices, launches_of_the_longest_caches)}
 
 
 @pytest.fixture(scope="module")
