@@ -73,7 +73,7 @@ extern "C" {
                                   at most 128 KiB (256 KiB from 32 of them on).  Work-groups have 8 waves, or
                                   4 when the 8-wave plan has at most 8 work-groups (the automatic chunk is
                                   then planned for 4).
-                                  E4M3 contexts: rounded up to a power of two of at least 256 keys, and no split
+                                  E4M3 contexts: rounded up to a power of two of 256 .. 2^30 keys, and no split
                                   where that gives more than 16 pieces per CU (the pieces are then shared out in
                                   equal runs, two per CU).  0: one work-group for a (sequence, kv head) whose K/V
                                   take at most 128 KiB (256 KiB from 32 of them on, 640 KiB from half as many as

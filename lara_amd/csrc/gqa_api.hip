@@ -406,12 +406,12 @@ constexpr int64_t kKv8WholeBytes = 640 << 10;
 
 Kv8Shape plan_kv8(int batch, int n_kv_heads, int head_dim, int n_cu, int max_len, int chunk_opt, int merge_option) {
     const int64_t units = (int64_t)batch * n_kv_heads;
-    auto log2_up = [](int keys) {
-        int l = 0;
-        while ((1 << l) < keys) ++l;
-        return std::max(l, 8);
+    auto log2_up = [](int keys) {  // (2^30, which holds every row of a context, at most)
+        int l = 8;
+        while (l < 30 && (1 << l) < keys) ++l;
+        return l;
     };
-    static_assert(kKv8Piece == 1 << 8, "the smallest piece");
+    static_assert(kKv8Piece == 1 << 8 && kMaxRows == 1 << 30, "the smallest piece and the largest");
     auto direct = [&](int chunk_log2) {
         const int splits = decode_split_count(max_len, 1 << chunk_log2);
         return Kv8Shape{chunk_log2, splits, 0,

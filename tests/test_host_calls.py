@@ -190,8 +190,20 @@ def launches_of_the_longest_caches(stub):
     many.ok("gqa_append_kv_device", many.ctx, far[0], far[1], far[2], None)
 
 
+def decode_pieces_of_the_longest_caches(stub):
+    """GQA_OPT_DECODE_CHUNK up to its largest value in a context of 2^30 rows: a piece of 2^30 keys holds them all."""
+    e = Engine(stub, page=1 << 16, batch=1, max_seq_len=1 << 30, max_q_len=1)
+    e.lib.gqa_set_option.argtypes = [P, ctypes.c_int32, ctypes.c_int64]
+    for chunk, grid in ((1 << 30, 1), ((1 << 30) + 64, 1), ((1 << 29) + 64, 1), (1 << 29, 2), ((1 << 28) + 64, 2)):
+        e.ok("gqa_set_option", e.ctx, e._lib.GQA_OPT_DECODE_CHUNK, chunk)
+        e.ok("gqa_decode_device", e.ctx, DEV, DEV, OUT, None, None)
+        (line, *_) = [line for line in e.log() if line[1] == "launch"]
+        assert "decode_kv8_kernel" in line[2] and int(line[4]) == grid, (chunk, line)
+
+
 SCENARIOS = {f.__name__: f for f in (device_of_calls, workspace_of_the_exact_size, workspace_after_a_failed_launch,
-                                     launches_of_the_largest_matrices, launches_of_the_longest_caches)}
+                                     launches_of_the_largest_matrices, launches_of_the_longest_caches,
+                                     decode_pieces_of_the_longest_caches)}
 
 
 @pytest.fixture(scope="module")
