@@ -37,7 +37,7 @@ extern "C" {
 #define GQA_ERR_STREAM_DEST    0x11 /* ERR_STREAM_DEST attn_pkg.sv:284: bad destination/index */
 #define GQA_ERR_RESULT_LEN     0x12 /* ERR_RESULT_LEN attn_pkg.sv:285: output size mismatch */
 #define GQA_ERR_HIP            0x20 /* a HIP runtime call failed */
-#define GQA_ERR_OOM            0x21 /* device or pinned allocation failed */
+#define GQA_ERR_OOM            0x21 /* device, pinned or host allocation failed, or sizes past any memory */
 #define GQA_ERR_NO_DEVICE      0x22 /* no usable gfx950 device */
 #define GQA_ERR_NULL           0x23 /* required pointer argument is NULL */
 #define GQA_ERR_RANGE          0x24 /* length / position outside the configured capacity */

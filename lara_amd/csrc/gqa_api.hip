@@ -8,6 +8,7 @@
 #include <hipblaslt/hipblaslt.h>
 
 #include <algorithm>
+#include <exception>
 #include <mutex>
 #include <stdio.h>
 #include <stdlib.h>
@@ -1295,6 +1296,18 @@ int grow_forced_workspace(gqa_ctx* c, int target_wgs) {
     return GQA_OK;
 }
 
+// Whether a context's sizes are past any memory: more (sequence, kv head)s than 31 bits hold (their decode rows alone are
+// 512 GiB), or pools, staging, split partials or block tables of more than 2^48 bytes.  Below that no size here passes 64
+// bits.
+bool past_any_memory(const gqa_config& k, int page_size, int n_pages, int n_layers, bool kv8) {
+    const double units = (double)k.batch * k.n_kv_heads, D = k.head_dim, most = (double)(1ll << 48);
+    const double rows = page_size > 0 ? (double)n_pages * page_size * k.n_kv_heads : units * (k.max_seq_len + 64.0);
+    const double staged = (double)k.n_q_heads * D * 2 * std::max(k.batch, k.max_q_len);
+    const double table = page_size > 0 ? 4.0 * k.batch * (k.max_seq_len / page_size + 1.0) : 0.0;
+    const double partials = kv8 ? 0.0 : units * (k.max_seq_len / kMinSplitCap + 1.0) * (k.n_q_heads / k.n_kv_heads) * D * 4;
+    return units > INT32_MAX || rows * D * 2 * n_layers > most || staged > most || table > most || partials > most;
+}
+
 int create_ctx(const gqa_config* cfg, int32_t page_size, int32_t n_pages, int32_t n_layers, gqa_ctx** out_ctx,
                bool kv8 = false) {
     if (!cfg || !out_ctx) return GQA_ERR_NULL;
@@ -1308,6 +1321,7 @@ int create_ctx(const gqa_config* cfg, int32_t page_size, int32_t n_pages, int32_
     if (!(kv8 ? decode_kv8_supported(k.head_dim, group) : decode_supported(k.head_dim, group)) &&
         !prefill_supported(k.head_dim, group))
         return GQA_ERR_UNSUPPORTED;
+    if (past_any_memory(k, page_size, n_pages, n_layers, kv8)) return GQA_ERR_OOM;
 
     int n = 0;
     if (hipGetDeviceCount(&n) != hipSuccess || n < 1) return GQA_ERR_NO_DEVICE;
@@ -1340,7 +1354,12 @@ int create_ctx(const gqa_config* cfg, int32_t page_size, int32_t n_pages, int32_
         while ((1 << c->page_shift) < page_size) ++c->page_shift;
         c->n_pages = n_pages;
         c->max_pages = (k.max_seq_len + page_size - 1) / page_size;
-        c->pages = PageTable(k.batch, c->max_pages, n_pages);
+        try {
+            c->pages = PageTable(k.batch, c->max_pages, n_pages);
+        } catch (const std::exception&) {  // (no host memory for the tables)
+            delete c;
+            return GQA_ERR_OOM;
+        }
     }
     c->n_layers = n_layers;
     const size_t D = (size_t)k.head_dim;

@@ -201,9 +201,27 @@ def decode_pieces_of_the_longest_caches(stub):
         assert "decode_kv8_kernel" in line[2] and int(line[4]) == grid, (chunk, line)
 
 
+def contexts_past_any_memory(stub):
+    """Sizes whose tables or pools no machine holds, or whose bytes pass 64 bits, are refused as out of memory; neither an
+    exception nor a small allocation comes of them."""
+    e = Engine(stub)
+    tables = dict(e.cfg, batch=1 << 16, max_seq_len=1 << 30)
+    pools = dict(e.cfg, batch=1 << 21, n_q_heads=1 << 13, n_kv_heads=1 << 13, max_seq_len=1 << 30)  # 2^64 rows
+    cfg, ctx = e._lib.GqaConfig(**tables), P()
+    for create, *args in (("gqa_create_kv8", 64, 100, 1), ("gqa_create_paged", 64, 100), ("gqa_create_paged_layers", 64, 100, 2)):
+        assert e.call(create, ctypes.byref(cfg), *args, ctypes.byref(ctx)) == e._lib.GQA_ERR_OOM and not ctx, create
+    cfg = e._lib.GqaConfig(**pools)
+    for create, *args in (("gqa_create_kv8", 0, 0, 1), ("gqa_create",), ("gqa_create_kv8", 64, (1 << 31) - 1, 1024)):
+        assert e.call(create, ctypes.byref(cfg), *args, ctypes.byref(ctx)) == e._lib.GQA_ERR_OOM and not ctx, create
+    cfg = e._lib.GqaConfig(**dict(e.cfg, batch=1 << 21, n_q_heads=1 << 13, n_kv_heads=1 << 9, max_seq_len=1 << 30))  # 2^64 bytes of partials
+    assert e.call("gqa_create_paged", ctypes.byref(cfg), 1 << 16, 100, ctypes.byref(ctx)) == e._lib.GQA_ERR_OOM and not ctx
+    assert not any(line[1] == "hipMalloc" and int(line[2]) < 1 << 20 for line in e.log())
+    e.ok("gqa_decode_device", e.ctx, DEV, DEV, OUT, None, None)
+
+
 SCENARIOS = {f.__name__: f for f in (device_of_calls, workspace_of_the_exact_size, workspace_after_a_failed_launch,
                                      launches_of_the_largest_matrices, launches_of_the_longest_caches,
-                                     decode_pieces_of_the_longest_caches)}
+                                     decode_pieces_of_the_longest_caches, contexts_past_any_memory)}
 
 
 @pytest.fixture(scope="module")
