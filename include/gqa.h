@@ -78,7 +78,9 @@ extern "C" {
                                   equal runs, two per CU).  0: one work-group for a (sequence, kv head) whose K/V
                                   take at most 128 KiB (256 KiB from 32 of them on, 640 KiB from half as many as
                                   CUs on); else pieces for up to one work-group per CU while there are at most a
-                                  quarter as many as CUs, else equal runs */
+                                  quarter as many as CUs, else equal runs.  The device forms and prepared steps plan
+                                  with max_seq_len for the length: a few short sequences in a large context take
+                                  longer than in one of their own size (decode_kv8.hip has figures) */
 #define GQA_OPT_PROFILE      2 /* 1 = time every kernel launch with a HIP event pair bound to the launch
                                   (hipExtLaunchKernel; restarts the record).  Binding adds no GPU work
                                   between launches, but each timed launch costs the host several us,
@@ -227,16 +229,20 @@ int gqa_paged_layers(gqa_ctx* ctx, int32_t* n_layers, int32_t* layer);
  * Every entry point works as on a bf16 context, with bf16 rows crossing the boundary: the rows given to gqa_load_kv,
  * gqa_append_kv, gqa_decode_append, gqa_prefill_append and the layer stage are quantised as they are written (in the
  * same launch for the decode step), attention sees the stored values (those of rows appended by the call too), and
- * gqa_read_kv returns them as bf16, which holds them exactly.  Device operands are 16-byte aligned, in
+ * gqa_read_kv returns them as bf16, which holds them exactly (but below 2^-133, where only the heads' entry points write).  Device operands are 16-byte aligned, in
  * gqa_load_kv_device and gqa_append_kv_device too.  Differences:
  *   - decode takes every group of 1 .. 16 query heads per kv head; prefill the bf16 kernels' groups.  Decode's error
  *     against exact attention over the stored values is as of the bf16 cache.
- *   - prefill (and transactions) read the attended rows back into a bf16 workspace first, which grows to the longest
- *     kv_len seen (a call that grows it synchronises the device), and the layer stage passes through it: uses of it on
- *     several streams follow each other, and these calls return GQA_ERR_UNSUPPORTED under a stream capture.  Decode,
- *     append, load, read and the heads' entry points below need no workspace.
- *   - decode plans for batch * n_kv_heads * max_seq_len up to 2^36 keys (in the host forms, times the longest length);
- *     GQA_ERR_UNSUPPORTED above (a paged context may be sized so without having the rows).
+ *   - prefill (and transactions) read all kv_len rows back into a bf16 workspace first, however few query rows there are
+ *     (16 after 7900 keys of 8 kv heads of 128: 17.5 us, 9.7 over a bf16 cache); the layer stage and the host forms of
+ *     load and read pass through it too.  It holds 4 * H_kv * D bytes for each row of the largest such call, rounded up to
+ *     a power of two where that can be had; a call that grows it synchronises the device.  Uses of it on several
+ *     streams follow each other, and prefill and the layer stage return GQA_ERR_UNSUPPORTED under a stream capture.
+ *     Append, decode, the device forms of load and read and the heads' entry points below need no workspace.
+ *   - decode in equal runs plans for batch * n_kv_heads * (ceil(max_seq_len / 256) + 1) up to 2^28 (in the host forms, with
+ *     the longest length); GQA_ERR_UNSUPPORTED above (a paged context may be sized so without having the rows).
+ *   - V rows whose largest magnitude lies outside 2^-100 .. 2^96 may lose accuracy or pass fp32 on their way through
+ *     decode's sums (a weight is at most 2^8 before the division, times the row's scale).
  *   - KV260 numerics and gqa_decode_append_noalloc are for bf16 caches.
  * Decode launches of one context share its split partials, as on a bf16 cache: the caller orders them, replays of captured
  * ones among them.
@@ -281,7 +287,9 @@ int gqa_decode_append(gqa_ctx* ctx, const uint16_t* q, const uint16_t* k_rows, c
  * against cache rows 0..kv_len-1: q and o are host head-major [H_q][q_len][D]
  * (attn_driver.py:487-488, 464).  Query i sits at absolute position q_pos_base + i,
  * key j at kv_pos_base + j; with causal != 0 key j is valid iff its position <= the
- * query's (softmax_engine.sv:865-871).  Rows with no valid key output zeros. */
+ * query's (softmax_engine.sv:865-871).  Rows with no valid key output zeros, and -inf for lse; a score of NaN (a NaN in
+ * the query or in a key that it sees) makes the row and its lse NaN, here and in decode.  A V row that holds an infinity
+ * or NaN reaches rows of its 32-row block that the causal mask hides it from, too (their weight of 0 times it). */
 int gqa_prefill(gqa_ctx* ctx, int32_t b, const uint16_t* q, int32_t q_len,
                 int32_t q_pos_base, int32_t kv_len, int32_t kv_pos_base, int32_t causal,
                 uint16_t* o, float* lse);
@@ -422,6 +430,7 @@ int gqa_layer_times(gqa_ctx* ctx, float* out_us, int32_t n);
  * memory, rows NULL for rows = positions; q_out is [B][H_q][D].  A sequence with a negative position, or a row outside
  * 0 .. max_seq_len - 1, is left out: neither its Q nor its cache is written.  Positions of sequences that are not left
  * out stay below 2^30.
+ * Sums of squares are fp32: a head with a magnitude above 2^60 may come out as zeros where it is normalised.
  * ld is a multiple of 8 below 2^31.  qkv, q_out and the cache must not overlap, nor the weights and q_out, and all
  * operands are 16-byte aligned (positions and rows 4-byte), else GQA_ERR_RANGE. */
 int gqa_qk_norm_rope_device(gqa_ctx* ctx, int32_t b, const void* qkv, int64_t ld, int32_t n_tokens, const void* q_weight,
@@ -440,7 +449,7 @@ int gqa_qk_norm_rope_step_device(gqa_ctx* ctx, const void* qkv, int64_t ld, cons
  * gqa_w4_project_device: y [n_tokens][ldy] bf16 (the first `rows` of each row) = norm(x) W^T for x [n_tokens][hidden] bf16,
  * norm(x) = x / sqrt(mean(x^2) + rms_eps) * rms_weight, or x with rms_weight NULL.  x * rms_weight is rounded to bf16,
  * sums are fp32, of (128 + c) x and -136 x before the scale: a token whose |x * rms_weight| passes 2^112, or that is
- * not finite, may give NaN in every row.  n_tokens up to GQA_W4_MAX_TOKENS, ldy below 2^31; a token's result does not
+ * not finite, may give NaN in every row, and one with |x| above 2^55 zeros where it is normalised.  n_tokens up to GQA_W4_MAX_TOKENS, ldy below 2^31; a token's result does not
  * depend on the others of the call.
  * gqa_w4_unpack_device: the packed matrix as bf16 [rows][hidden], for long prompts (gqa_layer_qkv_device).
  * The context gives device and stream.  Operands are 16-byte aligned (codes any, scales and y 2-byte) and outputs must

@@ -16,9 +16,11 @@
 // where it is small (by the last work-group of a (sequence, kv head) to arrive).  Every K/V byte is read once for all
 // heads of the group.
 //
-// What bounds it: memory.  64 x 8192 keys, 8 kv heads of 128 (1.08 GB): 155 us, 6.98 TB/s (a read of 1 GiB: 7.02); 64
-// sequences of 1000 .. 16000 keys over 64-row pages (549 MB): 90 us beside other launches, 6.1 TB/s, 112 alone; one of
-// 4097 keys (8.5 MB): 5.2 / 10.4, the latency of the launch, one round of loads and the merge.
+// What bounds it: memory.  64 x 8192 keys, 8 kv heads of 128 (1.08 GB): 155 us, 6.98 TB/s (a read of 1 GiB: 7.02); 61
+// sequences of 512 .. 8192 keys over 64-row pages and three idle slots (549 MB): 90 us beside other launches, 6.1 TB/s, 100
+// .. 112 alone; one of 4097 keys in a cache of as many (8.5 MB): 4.7 / 10.4, the latency of the launch, one round of loads and the
+// merge.  Pieces of a direct launch follow from the cache's rows, not from the lengths, so a short sequence in a large
+// cache has few: the same 4097 keys in 8192 rows 6.6 / 11.1, in 32768 9.8 / 16.2, in 131072 12.1 / 35.4.
 //
 // Inside a segment the waves take rounds of keys in turn (four waves 64, eight 32: small launches, which are one latency
 // chain), the next round's K being loaded once the scores are

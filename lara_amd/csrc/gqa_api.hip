@@ -386,7 +386,8 @@ struct Kv8Shape {
     bool fused;  // partials merged in-launch
 };
 
-// Both sides measured (us, one launch after the other / beside other launches; all lengths equal, 256 CUs):
+// Both sides measured (us, one launch after the other / beside other launches; 256 CUs; all lengths equal but in the last
+// row, and the cache's rows as many: shorter sequences in a larger cache have fewer pieces, decode_kv8.hip):
 //                                              direct                        shared
 //   1 x 4097 keys, 8 kv heads, D 128          10.4 /  5.2                   15.0 /  6.4
 //   8 x 4000 (64 units: a quarter per CU)     19.2 / 13.3                   24.9 / 14.8
@@ -396,7 +397,7 @@ struct Kv8Shape {
 //   64 x 2400 (512 units of 600 KiB)          53.4 / 49.5                   59.4 / 49.6
 //   64 x 4000 (1000 KiB)                      85.4 / 79.7                   88.8 / 78.9
 //   12 x 1900, D 64 (96 units of 237 KiB)     10.6 /  4.7                   14.1 /  6.6
-//   64 sequences of 1000 .. 16000 keys        163 / 94                      112 / 90
+//   61 of 512 .. 8192 keys and 3 idle         134 / 92 (unsplit)            100 / 90
 // The shared runs' merge launch and their search for a start cost about 8 us alone, and lengths that differ cost the
 // unsplit ones the longest of them, which is why units stay whole only while the longest is short.
 constexpr int kKv8Partials = 16;  // per CU: two for each run, or one for each piece
