@@ -2112,7 +2112,8 @@ int gqa_decode_append_noalloc(const gqa_config* cfg, void* k_cache, void* v_cach
     int n_dev = 0;
     if (hipGetDeviceCount(&n_dev) != hipSuccess || k.device < 0 || k.device >= n_dev || k.device >= kNoAllocDevices)
         return GQA_ERR_NO_DEVICE;
-    HIP_TRY(hipSetDevice(k.device));
+    const DeviceScope device(k.device);
+    HIP_TRY(device.status);
     NoAllocDevice* dev = nullptr;
     int rc = noalloc_setup(k.device, (hipStream_t)stream, &dev);
     if (rc != GQA_OK) return rc;
@@ -2286,7 +2287,8 @@ int gqa_layer_qkv_device(gqa_ctx* c, int32_t b, const void* x, int32_t n_tokens,
     if (rc != GQA_OK) return rc;
     if (!rows_backed(c, b, kv_row0, n_tokens)) return GQA_ERR_RANGE;
     if (!(rms_eps >= 0.f) || !isfinite(rms_eps)) return GQA_ERR_RANGE;
-    HIP_TRY(hipSetDevice(c->cfg.device));
+    const DeviceScope device(c->cfg.device);
+    HIP_TRY(device.status);
     return run_layer_stage(c, b, x, n_tokens, hidden, wq, wk, wv, rms_weight, rms_eps, q_pos_base, kv_pos_base, kv_row0,
                            rope, q_out, pick_stream(c, stream), false);
 }
@@ -2518,7 +2520,8 @@ int gqa_graph_capture_decode_append(gqa_ctx* c, const void* q, const void* k_row
 int gqa_graph_launch(gqa_graph* g, void* stream) {
     if (!g || !g->ctx) return GQA_ERR_NULL;
     gqa_ctx* c = g->ctx;
-    HIP_TRY(hipSetDevice(c->cfg.device));
+    const DeviceScope device(c->cfg.device);
+    HIP_TRY(device.status);
     Launch l;
     l.stream = pick_stream(c, stream);
     HIP_TRY(launch_step(c->cfg.head_dim, c->group, g->args, l));

@@ -61,7 +61,9 @@ def kernels(log):
 def device_of_calls(stub):
     """Device entry points of an E4M3 context work on its device whichever is current, and leave that one current."""
     e = Engine(stub)
-    c = e.ctx
+    c, graph, cfg = e.ctx, P(), e._lib.GqaConfig(**e.cfg)
+    e.ok("gqa_graph_capture_decode_append", c, DEV, DEV, DEV, DEV, DEV, OUT, None, ctypes.byref(graph))
+    assert e.stub.stub_device() == 0
     calls = [
         ("gqa_load_kv_device", c, 0, 0, 100, DEV, DEV, None),
         ("gqa_append_kv_device", c, DEV, DEV, DEV, None),
@@ -72,6 +74,12 @@ def device_of_calls(stub):
         ("gqa_prefill_append_device", c, 0, DEV, DEV, DEV, 20, 20, 80, 100, 0, 1, OUT, None, None),
         ("gqa_qk_norm_rope_device", c, 0, DEV, 768, 4, None, None, 1e-6, 0, 0, 0, 1e4, OUT, None),
         ("gqa_qk_norm_rope_step_device", c, DEV, 768, None, None, 1e-6, DEV, None, 1e4, OUT, None),
+        ("gqa_layer_qkv_device", c, 0, DEV, 4, 1024, DEV, DEV, DEV, None, 1e-5, 0, 0, 0, 1, OUT, None),
+        ("gqa_w4_pack_device", c, DEV, DEV, 16, 128, 128, OUT, P(0xA0000000), None),
+        ("gqa_w4_unpack_device", c, DEV, DEV, 16, 128, 128, OUT, None),
+        ("gqa_w4_project_device", c, DEV, 3, 128, DEV, DEV, 128, 16, None, 1e-5, OUT, 16, None),
+        ("gqa_graph_launch", graph, None),
+        ("gqa_decode_append_noalloc", ctypes.byref(cfg), DEV, DEV, 320, DEV, DEV, DEV, DEV, DEV, OUT, None, None),
     ]
     for name, *args in calls:
         e.ok(name, *args)
