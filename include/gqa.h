@@ -55,13 +55,17 @@ extern "C" {
 /* Per-kernel timer slots reported by gqa_kernel_times. */
 #define GQA_TIMER_APPEND  0 /* rows into the cache; E4M3: also its rows read back (gqa_read_kv, prefill) */
 #define GQA_TIMER_DECODE  1
-#define GQA_TIMER_COMBINE 2 /* log-sum-exp merge launch of split-KV decode or segmented prefill */
+#define GQA_TIMER_COMBINE 2 /* log-sum-exp merge launch of split-KV decode, of a shared prefix or of segmented prefill;
+                               the sum of gqa_attention_mass_device's row shares */
 #define GQA_TIMER_PREFILL 3
 #define GQA_TIMER_NORM    4 /* layer stage: RMSNorm (gqa_layer_qkv_device) */
 #define GQA_TIMER_PROJECTION 5 /* layer stage: the QKV projection's hipBLASLt kernels, between two recorded events;
                                   gqa_w4_project_device */
-#define GQA_TIMER_ROPE    6 /* layer stage: RoPE + scatter; gqa_qk_norm_rope_device, _step_device */
-#define GQA_TIMER_COUNT   7
+#define GQA_TIMER_ROPE    6 /* layer stage: RoPE + scatter; gqa_qk_norm_rope_device, gqa_qk_norm_rotary_device and their step
+                               forms */
+#define GQA_TIMER_MASS    7 /* gqa_attention_mass_device, _step_device */
+#define GQA_TIMER_EVICT   8 /* gqa_evict_device: selection and move, a launch each */
+#define GQA_TIMER_COUNT   9
 
 /* Tunables for gqa_set_option. */
 #define GQA_OPT_DECODE_CHUNK 1 /* keys per split-KV work-group (a multiple of 64 giving at most max(l_cap / 256,
@@ -439,6 +443,92 @@ int gqa_qk_norm_rope_device(gqa_ctx* ctx, int32_t b, const void* qkv, int64_t ld
 int gqa_qk_norm_rope_step_device(gqa_ctx* ctx, const void* qkv, int64_t ld, const void* q_weight, const void* k_weight,
                                  float eps, const int32_t* positions, const int32_t* rows, double rope_base, void* q_out,
                                  void* stream);
+
+/* ---- heads: other rotary forms ----------------------------------------------------------
+ * The same two calls for models that turn their heads another way (the board turns pairs side by side, all of a head, with
+ * plain frequencies).  The first R = rotary_dim dims of a head turn (0: all; a multiple of 8), the others stay:
+ *   layout  GQA_ROPE_PAIRS: dims (2p, 2p + 1); GQA_ROPE_HALVES: dims (p, p + R / 2), p < R / 2
+ *   (a, b) becomes (a c - b s, a s + b c), c and s the cosine and sine of position * f_p, times `magnitude`
+ * with f_p = base^(-2p/R), and for contexts longer than the original_len that a model was trained on:
+ *   GQA_ROPE_PLAIN   f_p
+ *   GQA_ROPE_LINEAR  f_p / factor
+ *   GQA_ROPE_BANDS   f_p w + f_p / factor (1 - w), w = (T_p - low) / (high - low) held to 0 .. 1, T_p = original_len f_p / 2 pi
+ *                    the turns that a pair makes over original_len
+ *   GQA_ROPE_RAMP    f_p (1 - w) + f_p / factor w, w = (p - i) / max(j - i, 0.001) held to 0 .. 1, where i = max(0,
+ *                    floor(P(high))) and j = min(R - 1, ceil(P(low))), P(T) = R ln(original_len / (2 pi T)) / (2 ln base) the
+ *                    index at which a pair makes T turns over original_len
+ * magnitude 0 stands for 1 (RAMP: 0.1 ln(factor) + 1).  base > 1, factor >= 1, 0 < low < high, original_len >= 1 where they
+ * are used.  Everything else as above; angles are 64-bit, in turns (of which the whole ones go before the rounding).
+ * gqa_rope_frequencies: f_p [R / 2] and the magnitude (NULL: not wanted) of a form, on the host. */
+#define GQA_ROPE_PAIRS  0
+#define GQA_ROPE_HALVES 1
+#define GQA_ROPE_PLAIN  0
+#define GQA_ROPE_LINEAR 1
+#define GQA_ROPE_BANDS  2
+#define GQA_ROPE_RAMP   3
+typedef struct gqa_rope {
+    int32_t layout;        /* GQA_ROPE_PAIRS or _HALVES */
+    int32_t rotary_dim;    /* R; 0: head_dim            */
+    int32_t scaling;       /* GQA_ROPE_PLAIN .. _RAMP   */
+    int32_t original_len;
+    double  base;
+    double  factor;
+    double  low, high;
+    double  magnitude;
+} gqa_rope;
+int gqa_rope_frequencies(const gqa_rope* rope, int32_t head_dim, double* frequencies, double* magnitude);
+int gqa_qk_norm_rotary_device(gqa_ctx* ctx, int32_t b, const void* qkv, int64_t ld, int32_t n_tokens, const void* q_weight,
+                              const void* k_weight, float eps, int32_t q_pos_base, int32_t kv_pos_base, int32_t kv_row0,
+                              const gqa_rope* rope, void* q_out, void* stream);
+int gqa_qk_norm_rotary_step_device(gqa_ctx* ctx, const void* qkv, int64_t ld, const void* q_weight, const void* k_weight,
+                                   float eps, const int32_t* positions, const int32_t* rows, const gqa_rope* rope, void* q_out,
+                                   void* stream);
+
+/* ---- decode over a shared prefix -----------------------------------------------------------
+ * No reference counterpart (the board holds one sequence).  For batches whose sequences begin alike (a system prompt, a
+ * document): the rows that they share are held once, as the first rows of a sequence of the cache, and read once a step for
+ * the whole batch.  gqa_decode_prefix_device is gqa_decode_device where sequence b attends rows 0 .. prefix_lens[b] - 1 of
+ * sequence prefix_b and then rows 0 .. ctx_lens[b] - 1 of its own, as one softmax (o and lse over both).  prefix_lens [B] is
+ * in device memory, each held to 0 .. prefix_len; NULL: prefix_len for every sequence.  Sequence prefix_b is one of the batch
+ * like the others (0 and 0 for a slot that only holds the prefix: zeros, -inf); where it goes on behind the prefix itself, 0
+ * for its prefix_lens and all of its rows for its ctx_lens.  gqa_decode_append_prefix_device appends first, as
+ * gqa_decode_append_device does, one row of each sequence's own; a row below prefix_len of sequence prefix_b is not written.
+ * bf16 and E4M3 caches, contiguous and paged (rows 0 .. prefix_len - 1 of prefix_b are mapped, else GQA_ERR_RANGE), groups of
+ * 1 .. 16.  Error as of decode; a V row that holds an infinity or NaN reaches the sequences that see it and no others.
+ * Two launches.  Their partials are the context's: the first call allocates them (GQA_ERR_UNSUPPORTED under a stream capture),
+ * and the caller orders the calls of one context, replays of captured ones among them, as for decode. */
+int gqa_decode_prefix_device(gqa_ctx* ctx, const void* q, int32_t prefix_b, int32_t prefix_len, const int32_t* prefix_lens,
+                             const int32_t* ctx_lens, void* o, float* lse, void* stream);
+int gqa_decode_append_prefix_device(gqa_ctx* ctx, const void* q, const void* k_rows, const void* v_rows,
+                                    const int32_t* positions, int32_t prefix_b, int32_t prefix_len,
+                                    const int32_t* prefix_lens, const int32_t* ctx_lens, void* o, float* lse, void* stream);
+
+/* ---- a budget of rows: accumulated attention weight, eviction ---------------------------------
+ * No reference counterpart.  mass is [B][H_kv][max_seq_len] fp32 in device memory, the caller's: the attention weight that
+ * each row of the active layer's cache has got so far.
+ * gqa_attention_mass_step_device: after a decode step, with its q [B][H_q][D], ctx_lens and lse [B][H_q] (a step over a
+ * shared prefix counts its own rows only): for the rows t < ctx_lens[b] of each kv head
+ *   mass[t] = decay * mass[t] + sum over the group's query heads of exp(scale * q . k_t - lse)
+ * gqa_attention_mass_device: the same for a block of query rows of sequence b, with the q, lse and positions of the
+ * gqa_prefill_device call behind it: each row t < kv_len gets the sum over the group's query heads and the q_len rows that
+ * see it.  lse is that of all keys that the rows saw; q may be the last rows of a prompt alone.  decay is 0 .. 1, and 0
+ * overwrites (what mass held is not read).  A query row whose lse is not finite adds nothing.  Other rows' mass stays.  fp32.
+ * gqa_evict_device: every sequence with ctx_lens[b] > keep is cut down to keep rows, for each kv head by itself: its first
+ * `sinks` rows, its last `recent` ones and the heaviest of the others by mass (equal ones: those of lower index; NaN counts as
+ * least).  They move, in their order, to rows 0 .. keep - 1, in place; rows behind them keep what they hold.  sinks + recent
+ * <= keep.  new_lens[b] is min(ctx_lens[b], keep); kept [B][H_kv][keep] the former rows (-1 past new_lens[b]); new_mass the
+ * kept rows' mass, 0 for the rows keep .. ctx_lens[b] - 1, as mass for sequences that are not cut, and otherwise as it was.
+ * new_mass may be mass and new_lens ctx_lens; no other operands overlap (GQA_ERR_RANGE).  Lengths are held to 0 ..
+ * max_seq_len.  Rows keep their rotation, so positions go on counting tokens, not rows.  Paged contexts: pages stay mapped,
+ * rows of unmapped ones are zeros and not written.
+ * None of these calls allocates or synchronises.  gqa_attention_mass_device and gqa_evict_device use workspaces of the
+ * context: the caller orders such calls of one context. */
+int gqa_attention_mass_step_device(gqa_ctx* ctx, const void* q, const int32_t* ctx_lens, const float* lse, float decay,
+                                   float* mass, void* stream);
+int gqa_attention_mass_device(gqa_ctx* ctx, int32_t b, const void* q, int32_t q_len, int32_t q_pos_base, int32_t kv_len,
+                              int32_t kv_pos_base, int32_t causal, const float* lse, float decay, float* mass, void* stream);
+int gqa_evict_device(gqa_ctx* ctx, const float* mass, const int32_t* ctx_lens, int32_t keep, int32_t sinks, int32_t recent,
+                     float* new_mass, int32_t* new_lens, int32_t* kept, void* stream);
 
 /* ---- 4-bit weights -----------------------------------------------------------------------
  * No reference counterpart.  The projection of a few tokens is the stream of its weights; 4-bit ones are a quarter of

@@ -43,7 +43,9 @@ GQA_TIMER_PREFILL = 3
 GQA_TIMER_NORM = 4
 GQA_TIMER_PROJECTION = 5
 GQA_TIMER_ROPE = 6
-GQA_TIMER_COUNT = 7
+GQA_TIMER_MASS = 7
+GQA_TIMER_EVICT = 8
+GQA_TIMER_COUNT = 9
 
 GQA_OPT_DECODE_CHUNK = 1
 GQA_OPT_PROFILE = 2
@@ -63,6 +65,12 @@ GQA_PREFILL_KERNEL_ROWS = 2
 GQA_PREFILL_KERNEL_PAIRED = 3
 GQA_NUMERICS_EXACT = 0
 GQA_NUMERICS_KV260 = 1
+GQA_ROPE_PAIRS = 0
+GQA_ROPE_HALVES = 1
+GQA_ROPE_PLAIN = 0
+GQA_ROPE_LINEAR = 1
+GQA_ROPE_BANDS = 2
+GQA_ROPE_RAMP = 3
 
 
 class GqaConfig(Structure):
@@ -75,6 +83,20 @@ class GqaConfig(Structure):
         ("max_q_len", c_int32),
         ("scale", c_float),
         ("device", c_int32),
+    ]
+
+
+class GqaRope(Structure):
+    _fields_ = [
+        ("layout", c_int32),
+        ("rotary_dim", c_int32),
+        ("scaling", c_int32),
+        ("original_len", c_int32),
+        ("base", c_double),
+        ("factor", c_double),
+        ("low", c_double),
+        ("high", c_double),
+        ("magnitude", c_double),
     ]
 
 
@@ -143,6 +165,18 @@ _SIGNATURES = {
                                 c_int32, c_double, c_void_p, c_void_p],
     "gqa_qk_norm_rope_step_device": [_CTX, c_void_p, c_int64, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_double,
                                      c_void_p, c_void_p],
+    "gqa_rope_frequencies": [POINTER(GqaRope), c_int32, POINTER(c_double), POINTER(c_double)],
+    "gqa_qk_norm_rotary_device": [_CTX, c_int32, c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_float, c_int32, c_int32,
+                                  c_int32, POINTER(GqaRope), c_void_p, c_void_p],
+    "gqa_qk_norm_rotary_step_device": [_CTX, c_void_p, c_int64, c_void_p, c_void_p, c_float, c_void_p, c_void_p,
+                                       POINTER(GqaRope), c_void_p, c_void_p],
+    "gqa_decode_prefix_device": [_CTX, c_void_p, c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
+    "gqa_decode_append_prefix_device": [_CTX, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_void_p,
+                                        c_void_p, c_void_p, c_void_p],
+    "gqa_attention_mass_step_device": [_CTX, c_void_p, c_void_p, c_void_p, c_float, c_void_p, c_void_p],
+    "gqa_attention_mass_device": [_CTX, c_int32, c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32, c_void_p, c_float,
+                                  c_void_p, c_void_p],
+    "gqa_evict_device": [_CTX, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_void_p],
     "gqa_w4_bytes": [c_int32, c_int32, c_int32, POINTER(c_int64), POINTER(c_int64)],
     "gqa_w4_pack_device": [_CTX, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p],
     "gqa_w4_unpack_device": [_CTX, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p, c_void_p],

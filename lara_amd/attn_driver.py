@@ -1022,6 +1022,67 @@ class AttentionAccelerator:
                    ctypes.c_void_p(rows_ptr) if rows_ptr else None, float(rope_base), ctypes.c_void_p(q_out_ptr),
                    ctypes.c_void_p(stream) if stream else None)
 
+    def qk_norm_rotary_device(self, qkv_ptr: int, ld: int, n_tokens: int, q_weight_ptr: int | None, k_weight_ptr: int | None,
+                              q_out_ptr: int, rope: "_lib.GqaRope", *, b: int = 0, q_pos_base: int = 0, kv_pos_base: int = 0,
+                              kv_row0: int = 0, eps: float = RMS_NORM_EPS, stream: int | None = None) -> None:
+        """``qk_norm_rope_device`` with any rotary form (``lara_amd.rope.form``; ``gqa_qk_norm_rotary_device``)."""
+        self._call("gqa_qk_norm_rotary_device", int(b), ctypes.c_void_p(qkv_ptr), int(ld), int(n_tokens),
+                   ctypes.c_void_p(q_weight_ptr) if q_weight_ptr else None,
+                   ctypes.c_void_p(k_weight_ptr) if k_weight_ptr else None, float(eps), int(q_pos_base), int(kv_pos_base),
+                   int(kv_row0), ctypes.byref(rope), ctypes.c_void_p(q_out_ptr), ctypes.c_void_p(stream) if stream else None)
+
+    def qk_norm_rotary_step_device(self, qkv_ptr: int, ld: int, q_weight_ptr: int | None, k_weight_ptr: int | None,
+                                   positions_ptr: int, q_out_ptr: int, rope: "_lib.GqaRope", *, rows_ptr: int | None = None,
+                                   eps: float = RMS_NORM_EPS, stream: int | None = None) -> None:
+        """``qk_norm_rope_step_device`` with any rotary form (``gqa_qk_norm_rotary_step_device``)."""
+        self._call("gqa_qk_norm_rotary_step_device", ctypes.c_void_p(qkv_ptr), int(ld),
+                   ctypes.c_void_p(q_weight_ptr) if q_weight_ptr else None,
+                   ctypes.c_void_p(k_weight_ptr) if k_weight_ptr else None, float(eps), ctypes.c_void_p(positions_ptr),
+                   ctypes.c_void_p(rows_ptr) if rows_ptr else None, ctypes.byref(rope), ctypes.c_void_p(q_out_ptr),
+                   ctypes.c_void_p(stream) if stream else None)
+
+    # ---- long contexts: shared prefixes, a budget of rows ------------------------------------
+    def decode_prefix_device(self, q_ptr: int, prefix_b: int, prefix_len: int, ctx_lens_ptr: int, o_ptr: int, *,
+                             prefix_lens_ptr: int | None = None, lse_ptr: int | None = None, k_rows_ptr: int | None = None,
+                             v_rows_ptr: int | None = None, positions_ptr: int | None = None, stream: int | None = None) -> None:
+        """One token of every sequence over the first rows of sequence ``prefix_b`` (``prefix_lens`` of them each, None:
+        ``prefix_len``) and its own ``ctx_lens`` rows (device pointers; ``gqa_decode_prefix_device``); with ``k_rows``,
+        ``v_rows`` and ``positions``, those rows are appended first (``gqa_decode_append_prefix_device``).  Enqueued, not
+        synchronised; the first call allocates the partials."""
+        given = [p is not None for p in (k_rows_ptr, v_rows_ptr, positions_ptr)]
+        if any(given) != all(given):
+            raise ValueError("k_rows, v_rows and positions go together")
+        rows = [ctypes.c_void_p(p) for p in (k_rows_ptr, v_rows_ptr, positions_ptr)] if all(given) else []
+        self._call("gqa_decode_append_prefix_device" if rows else "gqa_decode_prefix_device", ctypes.c_void_p(q_ptr), *rows,
+                   int(prefix_b), int(prefix_len), ctypes.c_void_p(prefix_lens_ptr) if prefix_lens_ptr else None,
+                   ctypes.c_void_p(ctx_lens_ptr), ctypes.c_void_p(o_ptr), ctypes.c_void_p(lse_ptr) if lse_ptr else None,
+                   ctypes.c_void_p(stream) if stream else None)
+
+    def attention_mass_step_device(self, q_ptr: int, ctx_lens_ptr: int, lse_ptr: int, mass_ptr: int, *, decay: float = 1.0,
+                                   stream: int | None = None) -> None:
+        """Adds a decode step's attention weight to the rows' ``mass`` [batch, H_kv, max_seq_len] fp32, times ``decay``
+        before (device pointers; ``gqa_attention_mass_step_device``); ``lse`` as the step gave it."""
+        self._call("gqa_attention_mass_step_device", ctypes.c_void_p(q_ptr), ctypes.c_void_p(ctx_lens_ptr),
+                   ctypes.c_void_p(lse_ptr), float(decay), ctypes.c_void_p(mass_ptr), ctypes.c_void_p(stream) if stream else None)
+
+    def attention_mass_device(self, q_ptr: int, q_len: int, kv_len: int, lse_ptr: int, mass_ptr: int, *, b: int = 0,
+                              q_pos_base: int = 0, kv_pos_base: int = 0, causal: bool = True, decay: float = 1.0,
+                              stream: int | None = None) -> None:
+        """The same for a block of query rows of sequence ``b`` (``gqa_attention_mass_device``): q [H_q, q_len, D] and lse
+        [H_q, q_len] of the prefill behind it."""
+        self._call("gqa_attention_mass_device", int(b), ctypes.c_void_p(q_ptr), int(q_len), int(q_pos_base), int(kv_len),
+                   int(kv_pos_base), int(bool(causal)), ctypes.c_void_p(lse_ptr), float(decay), ctypes.c_void_p(mass_ptr),
+                   ctypes.c_void_p(stream) if stream else None)
+
+    def evict_device(self, mass_ptr: int, ctx_lens_ptr: int, keep: int, kept_ptr: int, *, sinks: int = 0, recent: int = 0,
+                     new_mass_ptr: int | None = None, new_lens_ptr: int | None = None, stream: int | None = None) -> None:
+        """Cuts every sequence down to its first ``sinks`` rows, its last ``recent`` ones and the heaviest between, ``keep``
+        in all, for each kv head by itself (device pointers; ``gqa_evict_device``): ``kept`` [batch, H_kv, keep] gets their
+        former rows; mass and lengths are replaced in place unless given places of their own."""
+        self._call("gqa_evict_device", ctypes.c_void_p(mass_ptr), ctypes.c_void_p(ctx_lens_ptr), int(keep), int(sinks),
+                   int(recent), ctypes.c_void_p(new_mass_ptr or mass_ptr), ctypes.c_void_p(new_lens_ptr or ctx_lens_ptr),
+                   ctypes.c_void_p(kept_ptr), ctypes.c_void_p(stream) if stream else None)
+
     def w4_pack_device(self, codes_ptr: int, scales_ptr: int, rows: int, hidden: int, group: int, w_ptr: int,
                        w_scales_ptr: int, *, stream: int | None = None) -> None:
         """Lays a 4-bit matrix out for ``w4_project_device`` (``gqa_w4_pack_device``; ``lara_amd.w4.packed_bytes`` gives

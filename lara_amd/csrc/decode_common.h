@@ -38,6 +38,20 @@ __device__ __forceinline__ int clamp_len(int len, int l_max) {
     return len < 0 ? 0 : (len > l_max ? l_max : len);
 }
 
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int scan_dpp(int v) {
+    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
+}
+// Inclusive prefix sums over the wave's lanes (all active).
+__device__ __forceinline__ int wave_scan(int v) {
+    v = scan_dpp<0x111, 0xF>(v);  // row_shr:1, 2, 4, 8
+    v = scan_dpp<0x112, 0xF>(v);
+    v = scan_dpp<0x114, 0xF>(v);
+    v = scan_dpp<0x118, 0xF>(v);
+    v = scan_dpp<0x142, 0xA>(v);  // row_bcast:15, rows 1 and 3
+    return scan_dpp<0x143, 0xC>(v);  // row_bcast:31, rows 2 and 3
+}
+
 // The sequence of rank `rank` when the batch is ordered longest first.  Every wave computes it
 // for itself from the lengths (no LDS, no barrier); a batch of equal lengths keeps index order.
 //  * Up to 64 sequences (one per lane): exact -- by attended length, ties in index order (a wave

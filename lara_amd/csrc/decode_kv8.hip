@@ -108,20 +108,6 @@ struct Window {
     }
 };
 
-template <int CTRL, int ROWS>
-__device__ __forceinline__ int scan_dpp(int v) {
-    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
-}
-// Inclusive prefix sums over the wave's lanes (all active).
-__device__ __forceinline__ int wave_scan(int v) {
-    v = scan_dpp<0x111, 0xF>(v);  // row_shr:1, 2, 4, 8
-    v = scan_dpp<0x112, 0xF>(v);
-    v = scan_dpp<0x114, 0xF>(v);
-    v = scan_dpp<0x118, 0xF>(v);
-    v = scan_dpp<0x142, 0xA>(v);  // row_bcast:15, rows 1 and 3
-    return scan_dpp<0x143, 0xC>(v);  // row_bcast:31, rows 2 and 3
-}
-
 // Cost of a run: the batch's over `runs` work-groups.  Leaves a window of the batch's last part.
 __device__ __forceinline__ int run_cost(const DecodeArgs& a, int runs, Window& w) {
     int total = 0;

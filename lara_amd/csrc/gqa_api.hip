@@ -82,6 +82,9 @@ struct gqa_ctx {
     hipEvent_t ev_kv8_ws = nullptr;  // the last use of it has ended
     hipStream_t kv8_ws_stream = nullptr;  // where that was (only compared: it may be gone)
     bool kv8_ws_used = false;
+    float* mass_sums = nullptr;      // sums of query rows shared out over work-groups (gqa_attention_mass_device)
+    int32_t* evict_lens = nullptr;   // [B] lengths as an eviction found them
+    float* prefix_o = nullptr;       // partials of decode steps over a shared prefix, (m, l) behind O (from the first such step on)
     float* part_o = nullptr;
     float* part_ml = nullptr;
     int32_t* arrivals = nullptr;  // [B*H_kv] split arrival counters of the fused merge, then the row ticket
@@ -1386,6 +1389,8 @@ int create_ctx(const gqa_config* cfg, int32_t page_size, int32_t n_pages, int32_
     alloc((void**)&c->part_o, partials * D * sizeof(float));
     alloc((void**)&c->part_ml, partials * 2 * sizeof(float));
     alloc((void**)&c->arrivals, (units + 1) * sizeof(int32_t));
+    alloc((void**)&c->mass_sums, (size_t)kMassSums * c->n_cu * sizeof(float));
+    alloc((void**)&c->evict_lens, (size_t)k.batch * sizeof(int32_t));
     if (prefill_supported(k.head_dim, group)) {
         if (k.max_seq_len > kAutoSegmentKeys) c->auto_ws_floats = prefill_workspace_need(c, c->n_cu);
         if (c->auto_ws_floats > 0) alloc((void**)&c->auto_ws, c->auto_ws_floats * sizeof(float));
@@ -1631,6 +1636,9 @@ int gqa_destroy(gqa_ctx* c) {
     (void)hipFree(c->part_o);
     (void)hipFree(c->part_ml);
     (void)hipFree(c->arrivals);
+    (void)hipFree(c->mass_sums);
+    (void)hipFree(c->evict_lens);
+    (void)hipFree(c->prefix_o);
     (void)hipFree(c->pre_ws);
     (void)hipFree(c->auto_ws);
     (void)hipFree(c->zero_row);
@@ -2358,13 +2366,13 @@ namespace {
 
 constexpr int kHeadsMaxPosition = 1 << 30;
 
-int run_heads(gqa_ctx* c, HeadsArgs& a, const void* qkv, int64_t ld, const void* q_weight, const void* k_weight, float eps,
-              double rope_base, void* q_out, hipStream_t s) {
+// Checks a heads call's operands and fills its arguments but for the rotation.
+int check_heads(gqa_ctx* c, HeadsArgs& a, const void* qkv, int64_t ld, const void* q_weight, const void* k_weight, float eps,
+                void* q_out) {
     const int64_t width = (int64_t)(c->cfg.n_q_heads + 2 * c->cfg.n_kv_heads) * c->cfg.head_dim;
     if (ld < width || ld > INT32_MAX || ld % 8 != 0 || !aligned16(qkv) || !aligned16(q_weight) || !aligned16(k_weight) || !aligned16(q_out))
         return GQA_ERR_RANGE;
     if (!(eps >= 0.f) || !isfinite(eps)) return GQA_ERR_RANGE;
-    if (!(rope_base == 0.0 || rope_base > 1.0) || !isfinite(rope_base)) return GQA_ERR_RANGE;
     // The kernel reads the rows and the weights while it writes Q and the cache.
     const size_t weight = (size_t)c->cfg.head_dim * 2;
     const size_t in = ((size_t)(a.n_tokens - 1) * ld + width) * 2, out = (size_t)a.n_tokens * c->cfg.n_q_heads * c->cfg.head_dim * 2;
@@ -2377,12 +2385,155 @@ int run_heads(gqa_ctx* c, HeadsArgs& a, const void* qkv, int64_t ld, const void*
     a.wq = (const uint16_t*)q_weight;
     a.wk = (const uint16_t*)k_weight;
     a.eps = eps;
-    a.log2_base = rope_base > 0.0 ? log2(rope_base) : 0.0;
     a.q_out = (uint16_t*)q_out;
     a.cache = cache_view(c);
+    return GQA_OK;
+}
+
+int run_heads(gqa_ctx* c, HeadsArgs& a, const void* qkv, int64_t ld, const void* q_weight, const void* k_weight, float eps,
+              double rope_base, void* q_out, hipStream_t s) {
+    if (!(rope_base == 0.0 || rope_base > 1.0) || !isfinite(rope_base)) return GQA_ERR_RANGE;
+    const int rc = check_heads(c, a, qkv, ld, q_weight, k_weight, eps, q_out);
+    if (rc != GQA_OK) return rc;
+    a.log2_base = rope_base > 0.0 ? log2(rope_base) : 0.0;
     const DeviceScope device(c->cfg.device);
     HIP_TRY(device.status);
     HIP_TRY(launch_qk_norm_rope(c->cfg.head_dim, a, timed(c, GQA_TIMER_ROPE, s)));
+    return GQA_OK;
+}
+
+// Frequencies of a rotary form's pairs, [rotary_dim / 2], and what multiplies cosine and sine.
+int rope_frequencies(const gqa_rope& r, int head_dim, int* rotary_dim, double* f, double* magnitude) {
+    const int R = r.rotary_dim == 0 ? head_dim : r.rotary_dim;
+    if (R < 8 || R > head_dim || R % 8 != 0 || !(r.base > 1.0) || !isfinite(r.base)) return GQA_ERR_RANGE;
+    if (r.layout != GQA_ROPE_PAIRS && r.layout != GQA_ROPE_HALVES) return GQA_ERR_RANGE;
+    if (!(r.magnitude >= 0.0) || !isfinite(r.magnitude)) return GQA_ERR_RANGE;
+    const bool ends = r.scaling == GQA_ROPE_BANDS || r.scaling == GQA_ROPE_RAMP;
+    if (r.scaling != GQA_ROPE_PLAIN) {
+        if (r.scaling != GQA_ROPE_LINEAR && !ends) return GQA_ERR_RANGE;
+        if (!(r.factor >= 1.0) || !isfinite(r.factor)) return GQA_ERR_RANGE;
+        if (ends && (r.original_len < 1 || !(r.low > 0.0) || !(r.high > r.low) || !isfinite(r.high))) return GQA_ERR_RANGE;
+    }
+    const double two_pi = 2.0 * M_PI;
+    // (the index at which a pair makes so many turns over original_len)
+    auto pair_of = [&](double turns) { return R * log(r.original_len / (two_pi * turns)) / (2.0 * log(r.base)); };
+    const double first = r.scaling == GQA_ROPE_RAMP ? fmax(floor(pair_of(r.high)), 0.0) : 0.0;
+    const double last = r.scaling == GQA_ROPE_RAMP ? fmin(ceil(pair_of(r.low)), R - 1.0) : 0.0;
+    for (int p = 0; p < R / 2; ++p) {
+        const double plain = pow(r.base, -2.0 * p / R);
+        double divided = 0.0;  // share of the frequency that is divided by factor
+        if (r.scaling == GQA_ROPE_LINEAR) divided = 1.0;
+        if (r.scaling == GQA_ROPE_BANDS) divided = 1.0 - fmin(fmax((r.original_len * plain / two_pi - r.low) / (r.high - r.low), 0.0), 1.0);
+        if (r.scaling == GQA_ROPE_RAMP) divided = fmin(fmax((p - first) / fmax(last - first, 0.001), 0.0), 1.0);
+        f[p] = divided > 0.0 ? plain * (1.0 - divided) + plain / r.factor * divided : plain;
+    }
+    *rotary_dim = R;
+    *magnitude = r.magnitude > 0.0 ? r.magnitude : r.scaling == GQA_ROPE_RAMP ? 0.1 * log(r.factor) + 1.0 : 1.0;
+    return GQA_OK;
+}
+
+int run_rotary(gqa_ctx* c, RotaryArgs& a, const void* qkv, int64_t ld, const void* q_weight, const void* k_weight, float eps,
+               const gqa_rope& rope, void* q_out, hipStream_t s) {
+    double f[kMaxRopePairs], magnitude;
+    int rc = rope_frequencies(rope, c->cfg.head_dim, &a.rotary_dim, f, &magnitude);
+    if (rc == GQA_OK) rc = check_heads(c, a, qkv, ld, q_weight, k_weight, eps, q_out);
+    if (rc != GQA_OK) return rc;
+    for (int p = 0; p < a.rotary_dim / 2; ++p) a.turns[p] = f[p] / (2.0 * M_PI);
+    a.halves = rope.layout == GQA_ROPE_HALVES;
+    a.magnitude = (float)magnitude;
+    const DeviceScope device(c->cfg.device);
+    HIP_TRY(device.status);
+    HIP_TRY(launch_qk_norm_rotary(c->cfg.head_dim, a, timed(c, GQA_TIMER_ROPE, s)));
+    return GQA_OK;
+}
+
+// Checks the place of a prompt's heads: sequence b, positions and cache rows of n_tokens tokens.
+int check_heads_prompt(const gqa_ctx* c, int32_t b, int32_t n_tokens, int32_t q_pos_base, int32_t kv_pos_base, int32_t kv_row0) {
+    if (b < 0 || b >= c->cfg.batch) return GQA_ERR_STREAM_DEST;
+    if (n_tokens < 1 || kv_row0 < 0 || (int64_t)kv_row0 + n_tokens > c->cfg.max_seq_len) return GQA_ERR_RANGE;
+    if (q_pos_base < 0 || kv_pos_base < 0 || (int64_t)q_pos_base + n_tokens > kHeadsMaxPosition ||
+        (int64_t)kv_pos_base + n_tokens > kHeadsMaxPosition)
+        return GQA_ERR_RANGE;
+    return rows_backed(c, b, kv_row0, n_tokens) ? GQA_OK : GQA_ERR_RANGE;
+}
+
+inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
+
+// Bytes of a mass buffer, [B][H_kv][max_seq_len] fp32.
+size_t mass_bytes(const gqa_ctx* c) { return (size_t)c->cfg.batch * c->cfg.n_kv_heads * c->cfg.max_seq_len * sizeof(float); }
+
+// What both forms of the accumulated attention weight check, for n query rows in all.
+int check_mass(const gqa_ctx* c, const void* q, const void* lse, float decay, const void* mass, size_t n) {
+    const size_t q_bytes = n * c->cfg.head_dim * 2, bytes = mass_bytes(c);
+    if (!aligned16(q) || !aligned4(lse) || !aligned4(mass)) return GQA_ERR_RANGE;
+    if (!(decay >= 0.f && decay <= 1.f)) return GQA_ERR_RANGE;
+    if (overlaps(mass, bytes, q, q_bytes) || overlaps(mass, bytes, lse, n * sizeof(float)) || overlaps_cache(c, mass, bytes)) return GQA_ERR_RANGE;
+    return GQA_OK;
+}
+
+MassArgs mass_args(const gqa_ctx* c, const void* q, const float* lse, float decay, float* mass) {
+    MassArgs a{};
+    a.cache = cache_view(c);
+    a.q = (const uint16_t*)q;
+    a.lse = lse;
+    a.mass = mass;
+    a.mass_ld = c->cfg.max_seq_len;
+    a.decay = decay;
+    a.scale_log2 = c->scale * (float)M_LOG2E;
+    a.batch = c->cfg.batch;
+    a.group = c->group;
+    return a;
+}
+
+// The partials of decode steps over a shared prefix: allocated by the first one (not under a capture).
+int take_prefix_workspace(gqa_ctx* c, PrefixArgs& a, hipStream_t s) {
+    const int64_t rows = prefix_partial_rows_max(c->cfg.batch, c->cfg.n_kv_heads, c->group, c->n_cu);
+    if (c->prefix_o == nullptr) {
+        if (stream_capturing(s)) return GQA_ERR_UNSUPPORTED;
+        if (hipMalloc((void**)&c->prefix_o, (size_t)rows * (c->cfg.head_dim + 2) * sizeof(float)) != hipSuccess) {
+            (void)hipGetLastError();  // else the next launch reports it
+            c->prefix_o = nullptr;
+            return GQA_ERR_OOM;
+        }
+    }
+    a.part_o = c->prefix_o;
+    a.part_ml = c->prefix_o + (size_t)rows * c->cfg.head_dim;
+    return GQA_OK;
+}
+
+int run_decode_prefix(gqa_ctx* c, const void* q, const void* k_rows, const void* v_rows, const int32_t* positions, int32_t prefix_b,
+                      int32_t prefix_len, const int32_t* prefix_lens, const int32_t* ctx_lens, void* o, float* lse, hipStream_t s) {
+    if (prefix_b < 0 || prefix_b >= c->cfg.batch) return GQA_ERR_STREAM_DEST;
+    if (prefix_len < 0 || prefix_len > c->cfg.max_seq_len || !rows_backed(c, prefix_b, 0, prefix_len)) return GQA_ERR_RANGE;
+    const size_t words = (size_t)c->cfg.batch * c->cfg.n_q_heads * c->cfg.head_dim;
+    if (!aligned16(q) || !aligned16(k_rows) || !aligned16(v_rows) || (reinterpret_cast<uintptr_t>(o) & 1) || !aligned4(lse) ||
+        !aligned4(positions) || !aligned4(prefix_lens) || !aligned4(ctx_lens) || overlaps_cache(c, o, words * 2) ||
+        overlaps_cache(c, lse, lse ? words / c->cfg.head_dim * sizeof(float) : 0))
+        return GQA_ERR_RANGE;
+    if ((int64_t)c->cfg.batch * c->cfg.n_q_heads > INT32_MAX) return GQA_ERR_UNSUPPORTED;
+    const DeviceScope device(c->cfg.device);
+    HIP_TRY(device.status);
+    PrefixArgs a{};
+    a.cache = cache_view(c);
+    a.q = (const uint16_t*)q;
+    a.k_new = (const uint16_t*)k_rows;
+    a.v_new = (const uint16_t*)v_rows;
+    a.positions = positions;
+    a.lens = ctx_lens;
+    a.shared = prefix_lens;
+    a.batch = c->cfg.batch;
+    a.group = c->group;
+    a.prefix_b = prefix_b;
+    a.prefix_len = prefix_len;
+    a.scale_log2 = c->scale * (float)M_LOG2E;
+    a.out = (uint16_t*)o;
+    a.lse = lse;
+    plan_prefix(&a, c->n_cu);
+    const int rc = take_prefix_workspace(c, a, s);
+    if (rc != GQA_OK) return rc;
+    if (c->paged) c->pages.touch(prefix_b);
+    HIP_TRY(launch_decode_prefix(c->cfg.head_dim, a, timed(c, GQA_TIMER_DECODE, s)));
+    HIP_TRY(launch_decode_prefix_merge(c->cfg.head_dim, a, timed(c, GQA_TIMER_COMBINE, s)));
     return GQA_OK;
 }
 
@@ -2401,12 +2552,8 @@ int gqa_qk_norm_rope_device(gqa_ctx* c, int32_t b, const void* qkv, int64_t ld, 
                             const void* k_weight, float eps, int32_t q_pos_base, int32_t kv_pos_base, int32_t kv_row0,
                             double rope_base, void* q_out, void* stream) {
     if (!c || !qkv || !q_out) return GQA_ERR_NULL;
-    if (b < 0 || b >= c->cfg.batch) return GQA_ERR_STREAM_DEST;
-    if (n_tokens < 1 || kv_row0 < 0 || (int64_t)kv_row0 + n_tokens > c->cfg.max_seq_len) return GQA_ERR_RANGE;
-    if (q_pos_base < 0 || kv_pos_base < 0 || (int64_t)q_pos_base + n_tokens > kHeadsMaxPosition ||
-        (int64_t)kv_pos_base + n_tokens > kHeadsMaxPosition)
-        return GQA_ERR_RANGE;
-    if (!rows_backed(c, b, kv_row0, n_tokens)) return GQA_ERR_RANGE;
+    const int rc = check_heads_prompt(c, b, n_tokens, q_pos_base, kv_pos_base, kv_row0);
+    if (rc != GQA_OK) return rc;
     HeadsArgs a{};
     a.n_tokens = n_tokens;
     a.b = b;
@@ -2425,6 +2572,139 @@ int gqa_qk_norm_rope_step_device(gqa_ctx* c, const void* qkv, int64_t ld, const 
     a.positions = positions;
     a.rows = rows;
     return run_heads(c, a, qkv, ld, q_weight, k_weight, eps, rope_base, q_out, pick_stream(c, stream));
+}
+
+int gqa_rope_frequencies(const gqa_rope* rope, int32_t head_dim, double* frequencies, double* magnitude) {
+    if (!rope || !frequencies) return GQA_ERR_NULL;
+    if (head_dim != 64 && head_dim != 128) return GQA_ERR_UNSUPPORTED;
+    double f[kMaxRopePairs], m;
+    int rotary_dim;
+    const int rc = rope_frequencies(*rope, head_dim, &rotary_dim, f, &m);
+    if (rc != GQA_OK) return rc;
+    std::copy(f, f + rotary_dim / 2, frequencies);
+    if (magnitude) *magnitude = m;
+    return GQA_OK;
+}
+
+int gqa_qk_norm_rotary_device(gqa_ctx* c, int32_t b, const void* qkv, int64_t ld, int32_t n_tokens, const void* q_weight,
+                              const void* k_weight, float eps, int32_t q_pos_base, int32_t kv_pos_base, int32_t kv_row0,
+                              const gqa_rope* rope, void* q_out, void* stream) {
+    if (!c || !qkv || !rope || !q_out) return GQA_ERR_NULL;
+    const int rc = check_heads_prompt(c, b, n_tokens, q_pos_base, kv_pos_base, kv_row0);
+    if (rc != GQA_OK) return rc;
+    RotaryArgs a{};
+    a.n_tokens = n_tokens;
+    a.b = b;
+    a.pos_base = q_pos_base;
+    a.k_pos_base = kv_pos_base;
+    a.row0 = kv_row0;
+    return run_rotary(c, a, qkv, ld, q_weight, k_weight, eps, *rope, q_out, pick_stream(c, stream));
+}
+
+int gqa_qk_norm_rotary_step_device(gqa_ctx* c, const void* qkv, int64_t ld, const void* q_weight, const void* k_weight, float eps,
+                                   const int32_t* positions, const int32_t* rows, const gqa_rope* rope, void* q_out, void* stream) {
+    if (!c || !qkv || !positions || !rope || !q_out) return GQA_ERR_NULL;
+    if (!aligned4(positions) || !aligned4(rows)) return GQA_ERR_RANGE;
+    RotaryArgs a{};
+    a.n_tokens = c->cfg.batch;
+    a.positions = positions;
+    a.rows = rows;
+    return run_rotary(c, a, qkv, ld, q_weight, k_weight, eps, *rope, q_out, pick_stream(c, stream));
+}
+
+// ---- shared prefixes, accumulated attention weight, eviction ------------------------------
+
+int gqa_decode_prefix_device(gqa_ctx* c, const void* q, int32_t prefix_b, int32_t prefix_len, const int32_t* prefix_lens,
+                             const int32_t* ctx_lens, void* o, float* lse, void* stream) {
+    if (!c || !q || !ctx_lens || !o) return GQA_ERR_NULL;
+    return run_decode_prefix(c, q, nullptr, nullptr, nullptr, prefix_b, prefix_len, prefix_lens, ctx_lens, o, lse, pick_stream(c, stream));
+}
+
+int gqa_decode_append_prefix_device(gqa_ctx* c, const void* q, const void* k_rows, const void* v_rows, const int32_t* positions,
+                                    int32_t prefix_b, int32_t prefix_len, const int32_t* prefix_lens, const int32_t* ctx_lens,
+                                    void* o, float* lse, void* stream) {
+    if (!c || !q || !k_rows || !v_rows || !positions || !ctx_lens || !o) return GQA_ERR_NULL;
+    return run_decode_prefix(c, q, k_rows, v_rows, positions, prefix_b, prefix_len, prefix_lens, ctx_lens, o, lse, pick_stream(c, stream));
+}
+
+int gqa_attention_mass_step_device(gqa_ctx* c, const void* q, const int32_t* ctx_lens, const float* lse, float decay, float* mass,
+                                   void* stream) {
+    if (!c || !q || !ctx_lens || !lse || !mass) return GQA_ERR_NULL;
+    if (!aligned4(ctx_lens) || overlaps(mass, mass_bytes(c), ctx_lens, (size_t)c->cfg.batch * sizeof(int32_t))) return GQA_ERR_RANGE;
+    const int rc = check_mass(c, q, lse, decay, mass, (size_t)c->cfg.batch * c->cfg.n_q_heads);
+    if (rc != GQA_OK) return rc;
+    MassArgs a = mass_args(c, q, lse, decay, mass);
+    a.lens = ctx_lens;
+    const DeviceScope device(c->cfg.device);
+    HIP_TRY(device.status);
+    HIP_TRY(launch_mass_step(c->cfg.head_dim, a, c->n_cu, timed(c, GQA_TIMER_MASS, pick_stream(c, stream))));
+    return GQA_OK;
+}
+
+int gqa_attention_mass_device(gqa_ctx* c, int32_t b, const void* q, int32_t q_len, int32_t q_pos_base, int32_t kv_len,
+                              int32_t kv_pos_base, int32_t causal, const float* lse, float decay, float* mass, void* stream) {
+    if (!c || !q || !lse || !mass) return GQA_ERR_NULL;
+    int rc = check_prefill_args(c, b, q_len, q_pos_base, kv_len, kv_pos_base);
+    if (rc != GQA_OK) return rc;
+    if ((int64_t)q_len * c->group > kMaxRows || !rows_backed(c, b, 0, kv_len)) return GQA_ERR_RANGE;
+    rc = check_mass(c, q, lse, decay, mass, (size_t)q_len * c->cfg.n_q_heads);
+    if (rc != GQA_OK) return rc;
+    if (kv_len == 0) return GQA_OK;
+    MassArgs a = mass_args(c, q, lse, decay, mass);
+    a.b = b;
+    a.q_len = q_len;
+    a.kv_len = kv_len;
+    a.q_pos_base = q_pos_base;
+    a.kv_pos_base = kv_pos_base;
+    a.causal = causal != 0;
+    const MassPlan plan = plan_mass_block(c->group, c->cfg.n_kv_heads, q_len, kv_len, c->n_cu);
+    a.parts = plan.parts;
+    a.part_sums = c->mass_sums;
+    hipStream_t s = pick_stream(c, stream);
+    const DeviceScope device(c->cfg.device);
+    HIP_TRY(device.status);
+    HIP_TRY(launch_mass_block(c->cfg.head_dim, a, plan.key_tiles, timed(c, GQA_TIMER_MASS, s)));
+    if (a.parts > 1) HIP_TRY(launch_mass_sum(a, timed(c, GQA_TIMER_COMBINE, s)));
+    return GQA_OK;
+}
+
+int gqa_evict_device(gqa_ctx* c, const float* mass, const int32_t* ctx_lens, int32_t keep, int32_t sinks, int32_t recent,
+                     float* new_mass, int32_t* new_lens, int32_t* kept, void* stream) {
+    if (!c || !mass || !ctx_lens || !new_mass || !new_lens || !kept) return GQA_ERR_NULL;
+    if (keep < 1 || keep > c->cfg.max_seq_len || sinks < 0 || recent < 0 || (int64_t)sinks + recent > keep) return GQA_ERR_RANGE;
+    const size_t m = mass_bytes(c), n = (size_t)c->cfg.batch * sizeof(int32_t);
+    const size_t k = (size_t)c->cfg.batch * c->cfg.n_kv_heads * keep * sizeof(int32_t);
+    const struct {
+        const void* p;
+        size_t bytes;
+    } in[] = {{mass, m}, {ctx_lens, n}}, out[] = {{new_mass, m}, {new_lens, n}, {kept, k}};
+    for (int i = 0; i < 3; ++i) {
+        if (!aligned4(out[i].p) || overlaps_cache(c, out[i].p, out[i].bytes)) return GQA_ERR_RANGE;
+        for (int j = 0; j < 2; ++j)  // (a result may take its operand's place)
+            if (!aligned4(in[j].p) || ((i != j || out[i].p != in[j].p) && overlaps(out[i].p, out[i].bytes, in[j].p, in[j].bytes))) return GQA_ERR_RANGE;
+        for (int j = 0; j < i; ++j)
+            if (overlaps(out[i].p, out[i].bytes, out[j].p, out[j].bytes)) return GQA_ERR_RANGE;
+    }
+    EvictArgs a{};
+    a.cache = cache_view(c);
+    a.batch = c->cfg.batch;
+    a.row_bytes = c->cfg.head_dim * kv_value_bytes(c);
+    a.mass = mass;
+    a.new_mass = new_mass;
+    a.mass_ld = c->cfg.max_seq_len;
+    a.lens = ctx_lens;
+    a.new_lens = new_lens;
+    a.lens_copy = c->evict_lens;
+    a.keep = keep;
+    a.sinks = sinks;
+    a.recent = recent;
+    a.kept = kept;
+    hipStream_t s = pick_stream(c, stream);
+    const DeviceScope device(c->cfg.device);
+    HIP_TRY(device.status);
+    HIP_TRY(launch_evict_select(a, timed(c, GQA_TIMER_EVICT, s)));
+    HIP_TRY(launch_evict_move(a, c->n_cu, timed(c, GQA_TIMER_EVICT, s)));
+    return GQA_OK;
 }
 
 int gqa_w4_bytes(int32_t rows, int32_t hidden, int32_t group, int64_t* w_bytes, int64_t* scale_bytes) {

@@ -370,6 +370,86 @@ struct HeadsArgs {
 };
 hipError_t launch_qk_norm_rope(int head_dim, const HeadsArgs& a, const Launch& l);
 
+// The same with any rotary form (log2_base unused): the first rotary_dim dims turn, in pairs (2p, 2p + 1) or (p,
+// p + rotary_dim / 2).
+struct RotaryArgs : HeadsArgs {
+    int32_t halves, rotary_dim;    // rotary_dim: a multiple of 8
+    float magnitude;               // of cosine and sine
+    double turns[kMaxRopePairs];   // of a pair per position: frequency / (2 pi)
+};
+hipError_t launch_qk_norm_rotary(int head_dim, const RotaryArgs& a, const Launch& l);
+
+// Decode over a prefix that the batch shares and each sequence's own rows (decode_prefix.hip).
+struct PrefixArgs {
+    Kv8Cache cache;             // bf16 (k_scale == nullptr) or E4M3
+    const uint16_t* q;          // [B][H_q][D]
+    const uint16_t* k_new;      // [B][H_kv][D] rows appended by this launch, or nullptr
+    const uint16_t* v_new;
+    const int32_t* positions;   // [B]
+    const int32_t* lens;        // [B] own rows
+    const int32_t* shared;      // [B] rows of the prefix, nullptr: prefix_len
+    int32_t batch, group;
+    int32_t prefix_b, prefix_len;
+    float scale_log2;
+    int32_t row_tiles;          // of the prefix's work-groups: 32-row tiles that a tile of K and V serves (1, 2 or 4)
+    int32_t blocks;             // work-groups along the rows, per kv head
+    int32_t chunk, pieces;      // the prefix in pieces of `chunk` keys, a work-group each
+    int32_t own_wgs;            // work-groups for the sequences' own rows
+    int32_t own_slots;          // partials that own_part holds
+    float* part_o;              // prefix [pieces][H_kv][B * group][D], then own [own_slots][group][D]
+    float* part_ml;             // the same rows' (maximum in log2 units, sum)
+    uint16_t* out;              // [B][H_q][D]
+    float* lse;                 // [B][H_q] or nullptr
+};
+constexpr int kPrefixOwnSlots = 4096;  // at least; one per (sequence, kv head) where those are more
+void plan_prefix(PrefixArgs* a, int n_cu);
+// Rows of part_o (and part_ml) that plan_prefix may ask for, whatever the prefix.
+int64_t prefix_partial_rows_max(int batch, int n_kv_heads, int group, int n_cu);
+hipError_t launch_decode_prefix(int head_dim, const PrefixArgs& a, const Launch& l);
+hipError_t launch_decode_prefix_merge(int head_dim, const PrefixArgs& a, const Launch& l);
+
+// Accumulated attention weight of cache rows (mass.hip).
+struct MassArgs {
+    Kv8Cache cache;         // bf16 (k_scale == nullptr) or E4M3; V is not read
+    const uint16_t* q;      // step [B][H_q][D], block [H_q][q_len][D]
+    const float* lse;       // step [B][H_q], block [H_q][q_len]
+    const int32_t* lens;    // step: [B] keys
+    float* mass;            // [B][H_kv][mass_ld]
+    int64_t mass_ld;
+    float decay, scale_log2;
+    int32_t batch, group;
+    int32_t b, q_len, kv_len, q_pos_base, kv_pos_base, causal;  // block
+    int32_t parts, chunk;   // step: pieces of `chunk` keys a (sequence, kv head); block: work-groups that share the rows
+    float* part_sums;       // block, parts > 1: [parts][H_kv][kv_len]
+};
+struct MassPlan {
+    int32_t key_tiles;  // 32-key tiles a wave
+    int32_t parts;
+};
+constexpr int kMassMaxParts = 64;
+constexpr int kMassSums = 4 * 256;  // floats of part_sums per CU: 4 work-groups a CU of at most 256 keys
+MassPlan plan_mass_block(int group, int n_kv_heads, int q_len, int kv_len, int n_cu);
+hipError_t launch_mass_step(int head_dim, MassArgs a, int n_cu, const Launch& l);
+hipError_t launch_mass_block(int head_dim, const MassArgs& a, int key_tiles, const Launch& l);
+hipError_t launch_mass_sum(const MassArgs& a, const Launch& l);
+
+// Eviction (evict.hip): which rows of every (sequence, kv head) stay, then those moved together.
+struct EvictArgs {
+    Kv8Cache cache;
+    int32_t batch, row_bytes;  // of a K (or V) row, without its scale
+    const float* mass;         // [B][H_kv][mass_ld]
+    float* new_mass;           // the same or apart from it
+    int64_t mass_ld;
+    const int32_t* lens;       // [B]
+    int32_t* new_lens;         // the same or apart from lens
+    int32_t* lens_copy;        // [B] workspace: lens as the first launch found them
+    int32_t keep, sinks, recent;
+    int32_t* kept;             // [B][H_kv][keep]
+    int32_t slices;            // set by the launch: work-groups that share a K (or V) row
+};
+hipError_t launch_evict_select(const EvictArgs& a, const Launch& l);
+hipError_t launch_evict_move(const EvictArgs& a, int n_cu, const Launch& l);
+
 // 4-bit weights (w4.hip): hidden a multiple of `group`, group 32, 64 or 128.
 struct W4PackArgs {
     const uint8_t* codes;

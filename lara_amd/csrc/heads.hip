@@ -19,6 +19,8 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 namespace lara {
 namespace {
 
@@ -41,9 +43,14 @@ __device__ __forceinline__ float row_sum(float v) {
     return v;
 }
 
+// How a row turns: whole, pairs side by side, base^(-2p / D) (HeadsArgs); or as RotaryArgs say.
+enum Form { kPlain, kPairs, kHalves };
+template <Form FORM>
+using FormArgs = std::conditional_t<FORM == kPlain, HeadsArgs, RotaryArgs>;
+
 // TOKENS tokens a work-group (one of the step form); a thread keeps its token and its place in a row.
-template <int D, bool E4M3, int TOKENS>
-__global__ __launch_bounds__(kHeadsThreads) void qk_norm_rope_kernel(HeadsArgs a) {
+template <int D, bool E4M3, int TOKENS, Form FORM>
+__global__ __launch_bounds__(kHeadsThreads) void qk_norm_rope_kernel(FormArgs<FORM> a) {
     constexpr int LANES = D / 8, PAIRS = D / 2;
     const int token0 = wide_block() * TOKENS;
     if (token0 >= a.n_tokens) return;  // (the whole work-group)
@@ -57,23 +64,59 @@ __global__ __launch_bounds__(kHeadsThreads) void qk_norm_rope_kernel(HeadsArgs a
         if (pos0 < 0 || t0 < 0 || t0 >= a.cache.l_max) return;  // (the whole work-group) nothing of this sequence is written
     }
     const int heads = a.n_q_heads + 2 * a.cache.n_kv_heads, chunks = heads * TOKENS * LANES;
+    // A lane's 8 values are two runs of 4 dims, one behind the other; where halves turn, the lanes of the dims that turn have
+    // a run of each half, so that both values of a pair are in one lane in every form.
+    int run0 = 8 * part, run1 = 8 * part + 4;
+    bool turning = true;
+    if constexpr (FORM != kPlain) turning = 8 * part < a.rotary_dim;
+    if constexpr (FORM == kHalves)
+        if (turning) run0 = 4 * part, run1 = a.rotary_dim / 2 + 4 * part;
+    auto load_runs = [&](const uint16_t* row) __attribute__((always_inline)) {
+        const u32x2 lo = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(row + run0));
+        const u32x2 hi = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(row + run1));
+        return u32x4{lo[0], lo[1], hi[0], hi[1]};
+    };
+    auto store_runs = [&](uint16_t* row, const u32x4& w) __attribute__((always_inline)) {
+        *reinterpret_cast<u32x2*>(row + run0) = u32x2{w[0], w[1]};
+        *reinterpret_cast<u32x2*>(row + run1) = u32x2{w[2], w[3]};
+    };
     // A batch of values is loaded at once, the first ahead of the angles.
     u32x4 in[kHeadsBatch];
     auto load = [&](int from) __attribute__((always_inline)) {
 #pragma unroll
         for (int k = 0; k < kHeadsBatch; ++k) {
             const int i = from + k * kHeadsThreads, of = i / LANES % TOKENS;
-            if (i < chunks && of < tokens)
-                in[k] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(a.x + (size_t)(token0 + of) * a.ld) +
-                                                   i / (LANES * TOKENS) * LANES + part);
+            if (i >= chunks || of >= tokens) continue;
+            const uint16_t* const row = a.x + (size_t)(token0 + of) * a.ld;
+            if constexpr (FORM == kHalves)
+                in[k] = load_runs(row + i / (LANES * TOKENS) * D);
+            else
+                in[k] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(row) + i / (LANES * TOKENS) * LANES + part);
         }
     };
     load(threadIdx.x);
     u32x4 wq = {}, wk = {};
-    if (a.wq != nullptr) wq = reinterpret_cast<const u32x4*>(a.wq)[part];
-    if (a.wk != nullptr) wk = reinterpret_cast<const u32x4*>(a.wk)[part];
+    if constexpr (FORM == kHalves) {
+        if (a.wq != nullptr) wq = load_runs(a.wq);
+        if (a.wk != nullptr) wk = load_runs(a.wk);
+    } else {
+        if (a.wq != nullptr) wq = reinterpret_cast<const u32x4*>(a.wq)[part];
+        if (a.wk != nullptr) wk = reinterpret_cast<const u32x4*>(a.wk)[part];
+    }
     __shared__ float2 turn[2][TOKENS][PAIRS];
-    if (a.log2_base > 0.0) {
+    if constexpr (FORM != kPlain) {
+        const int sets = k_pos0 != pos0 ? 2 : 1;
+        for (int i = threadIdx.x; i < sets * TOKENS * PAIRS; i += kHeadsThreads) {
+            const int p = i % PAIRS, of = i / PAIRS % TOKENS, set = i / (PAIRS * TOKENS);
+            if (2 * p >= a.rotary_dim) continue;
+            // The angle in turns: its whole ones go, in 64 bits, before it is rounded (to 2^-25 of at most half a turn).
+            const double t = (double)((set ? k_pos0 : pos0) + of) * a.turns[p];
+            float s, c;
+            sincospif(2.f * (float)(t - rint(t)), &s, &c);
+            turn[set][of][p] = make_float2(c * a.magnitude, s * a.magnitude);
+        }
+        __syncthreads();
+    } else if (a.log2_base > 0.0) {
         const int sets = k_pos0 != pos0 ? 2 : 1;
         for (int i = threadIdx.x; i < sets * TOKENS * PAIRS; i += kHeadsThreads) {
             const int p = i % PAIRS, of = i / PAIRS % TOKENS, set = i / (PAIRS * TOKENS);
@@ -99,13 +142,16 @@ __global__ __launch_bounds__(kHeadsThreads) void qk_norm_rope_kernel(HeadsArgs a
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[j] = x[j] * inv * w[j];
         }
-        if (a.log2_base > 0.0 && (is_q || is_k)) {
+        bool turns = turning;
+        if constexpr (FORM == kPlain) turns = a.log2_base > 0.0;
+        if (turns && (is_q || is_k)) {
             const float2* const cs = turn[is_k && k_pos0 != pos0 ? 1 : 0][of] + 4 * part;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float c = cs[j].x, s = cs[j].y, x0 = x[2 * j], x1 = x[2 * j + 1];
-                x[2 * j] = x0 * c - x1 * s;
-                x[2 * j + 1] = x0 * s + x1 * c;
+                constexpr int STEP = FORM == kHalves ? 1 : 2, FAR = FORM == kHalves ? 4 : 1;
+                const float c = cs[j].x, s = cs[j].y, x0 = x[STEP * j], x1 = x[STEP * j + FAR];
+                x[STEP * j] = x0 * c - x1 * s;
+                x[STEP * j + FAR] = x0 * s + x1 * c;
             }
         }
         u32x4 o;
@@ -118,7 +164,10 @@ __global__ __launch_bounds__(kHeadsThreads) void qk_norm_rope_kernel(HeadsArgs a
         }
         if (is_q) {
             const size_t row = a.positions != nullptr ? (size_t)token * a.n_q_heads + head : (size_t)head * a.n_tokens + token;
-            reinterpret_cast<u32x4*>(a.q_out)[row * LANES + part] = o;
+            if constexpr (FORM == kHalves)
+                store_runs(a.q_out + row * D, o);
+            else
+                reinterpret_cast<u32x4*>(a.q_out)[row * LANES + part] = o;
             return;
         }
         const int h = head - a.n_q_heads - (is_k ? 0 : a.cache.n_kv_heads);
@@ -128,8 +177,15 @@ __global__ __launch_bounds__(kHeadsThreads) void qk_norm_rope_kernel(HeadsArgs a
         if constexpr (E4M3) {
             uint32_t byte;
             const u32x2 codes = kv8_quantise<LANES>(x, &byte);
-            reinterpret_cast<u32x2*>(to + row * D)[part] = codes;
+            if constexpr (FORM == kHalves) {
+                *reinterpret_cast<uint32_t*>(to + row * D + run0) = codes[0];
+                *reinterpret_cast<uint32_t*>(to + row * D + run1) = codes[1];
+            } else {
+                reinterpret_cast<u32x2*>(to + row * D)[part] = codes;
+            }
             if (part == 0) (is_k ? a.cache.k_scale : a.cache.v_scale)[row] = (uint8_t)byte;
+        } else if constexpr (FORM == kHalves) {
+            store_runs(reinterpret_cast<uint16_t*>(to) + row * D, o);
         } else {
             reinterpret_cast<u32x4*>(to)[row * LANES + part] = o;
         }
@@ -143,18 +199,25 @@ __global__ __launch_bounds__(kHeadsThreads) void qk_norm_rope_kernel(HeadsArgs a
 
 }  // namespace
 
-template <int D, int TOKENS>
-static hipError_t launch_tokens(const HeadsArgs& a, const Launch& l) {
+template <int D, int TOKENS, Form FORM>
+static hipError_t launch_tokens(const FormArgs<FORM>& a, const Launch& l) {
     const dim3 grid = wide_grid((a.n_tokens + TOKENS - 1) / TOKENS), block(kHeadsThreads);
-    return a.cache.k_scale != nullptr ? launch_kernel(qk_norm_rope_kernel<D, true, TOKENS>, grid, block, l, a)
-                                      : launch_kernel(qk_norm_rope_kernel<D, false, TOKENS>, grid, block, l, a);
+    return a.cache.k_scale != nullptr ? launch_kernel(qk_norm_rope_kernel<D, true, TOKENS, FORM>, grid, block, l, a)
+                                      : launch_kernel(qk_norm_rope_kernel<D, false, TOKENS, FORM>, grid, block, l, a);
 }
 
-hipError_t launch_qk_norm_rope(int head_dim, const HeadsArgs& a, const Launch& l) {
+template <Form FORM>
+static hipError_t launch_form(int head_dim, const FormArgs<FORM>& a, const Launch& l) {
     if (a.n_tokens < 1) return hipSuccess;
-    if (head_dim == 128) return launch_tokens<128, 1>(a, l);
-    if (head_dim == 64) return a.positions == nullptr ? launch_tokens<64, 2>(a, l) : launch_tokens<64, 1>(a, l);
+    if (head_dim == 128) return launch_tokens<128, 1, FORM>(a, l);
+    if (head_dim == 64) return a.positions == nullptr ? launch_tokens<64, 2, FORM>(a, l) : launch_tokens<64, 1, FORM>(a, l);
     return hipErrorInvalidValue;
+}
+
+hipError_t launch_qk_norm_rope(int head_dim, const HeadsArgs& a, const Launch& l) { return launch_form<kPlain>(head_dim, a, l); }
+
+hipError_t launch_qk_norm_rotary(int head_dim, const RotaryArgs& a, const Launch& l) {
+    return a.halves ? launch_form<kHalves>(head_dim, a, l) : launch_form<kPairs>(head_dim, a, l);
 }
 
 }  // namespace lara
