@@ -15,6 +15,8 @@
 #include "decode_common.h"
 #include "kv8_device.h"
 
+#include <type_traits>
+
 namespace lara {
 namespace {
 
@@ -23,6 +25,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kMassWaves = 4;
+constexpr int kRowTiles = 1;  // of a stage
 
 __device__ __forceinline__ f32x4 mfma16(const u32x4& a, const u32x4& b, const f32x4& c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
@@ -48,48 +51,66 @@ __device__ __forceinline__ int64_t first_row(const Kv8Cache& c, int b, int h, in
     return paged_row_uniform(c.block_table + (size_t)b * c.max_pages, c.page_shift, c.n_kv_heads, h, key0);
 }
 
+// Lanes m and m + 8 of a row of 16 add up: the lane's own value and the other's.
+__device__ __forceinline__ float add_far(float own, float far) {
+    return own + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(far), 0x128, 0xF, 0xF, true));  // row_ror:8
+}
+
 // One row of every sequence.  A work-group: `chunk` keys (a multiple of 256) of one (sequence, kv head), rounds of 64 for
 // its waves in turn.
+// Rows are loaded by whole lines: lane (m, g) has the 16-byte chunk 4 (m / 8) + g of a line of key m % 8, so an instruction
+// covers 8 lines.  A column of operand B is then half of a key's line, and is multiplied with both halves' dims of Q; of the
+// two products lanes below 8 keep the first's and add what the lanes above have of theirs.  (16 keys an instruction, half a
+// line each: 4.5 TB/s.)  Rows of 64 bytes lie as they are wanted.
 template <int D, bool E4M3>
 __global__ __launch_bounds__(kMassWaves * 64) void mass_step_kernel(MassArgs a) {
-    constexpr int CH = E4M3 ? D / 64 : D / 32;  // 16-byte chunks of a key per lane
     constexpr int BYTES = E4M3 ? D : 2 * D;
+    constexpr bool HALVES = BYTES >= 128;
+    constexpr int LOADS = BYTES / 16;           // 16-byte chunks per lane of 64 keys, and per key
+    constexpr int PARTS = E4M3 ? 2 : 1;         // steps of 32 dims in a chunk of every lane
+    constexpr int STEPS = D / 32;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int m = lane & 15, g = lane >> 4;
-    const uint32_t block = wide_block();
-    const int unit = block / a.parts, part = block - unit * a.parts;
+    const bool low = m < 8;
+    // Pieces go slowest: consecutive work-groups (XCDs in turn) take different sequences and heads, and not always the same
+    // piece, of which the later ones are few where lengths differ (64 sequences of 4000 .. 8192 keys: 156 -> 126 us).
+    const uint32_t block = wide_block(), units = (uint32_t)a.batch * a.cache.n_kv_heads;
+    const int part = block / units, unit = block - part * units;
     const int b = unit / a.cache.n_kv_heads, h = unit - b * a.cache.n_kv_heads;
-    if (b >= a.batch) return;
+    if (part >= a.parts) return;
     const int L = clamp_len(a.lens[b], a.cache.l_max);
     const int64_t begin = (int64_t)part * a.chunk;
     if (begin >= L) return;
     const int end = begin + a.chunk < L ? (int)(begin + a.chunk) : L;
     const int H_q = a.cache.n_kv_heads * a.group;
 
-    auto load = [&](int key0, u32x4 (&k)[4][CH], float (&scale)[4], bool* mapped) __attribute__((always_inline)) {
+    // Load i: rows of eight x = i / lines, line i % lines (or 16 rows i, whole).
+    constexpr int LINES = HALVES ? BYTES / 128 : 1;
+    const uint32_t lane_at = HALVES ? (m & 7) * BYTES + 16 * (4 * (m >> 3) + g) : m * BYTES + 16 * g;
+    auto load = [&](int key0, u32x4 (&k)[LOADS], float (&scale)[4], bool* mapped) __attribute__((always_inline)) {
         int64_t row = first_row(a.cache, b, h, key0);
         *mapped = row >= 0;
         if (row < 0) row = 0;
+        const uint8_t* const p = a.cache.k + row * BYTES;
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const uint8_t* const p = a.cache.k + (row + 16 * t + m) * BYTES + 16 * g;
+        for (int i = 0; i < LOADS; ++i)
+            k[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(
+                p + lane_at + (HALVES ? i / LINES * 8 * BYTES + i % LINES * 128 : i * 16 * BYTES)));
+        if constexpr (E4M3)
 #pragma unroll
-            for (int j = 0; j < CH; ++j) k[t][j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + 64 * j));
-            if constexpr (E4M3) scale[t] = kv8_scale(a.cache.k_scale[row + 16 * t + m]);
-        }
+            for (int t = 0; t < 4; ++t) scale[t] = kv8_scale(a.cache.k_scale[row + 16 * t + m]);
     };
-    u32x4 k[4][CH];
+    u32x4 k[LOADS];
     float scale[4];
     bool mapped = false;
     int key0 = (int)begin + 64 * wave;
     if (key0 < end) load(key0, k, scale, &mapped);
 
-    // Operand A: lane (m, g) holds, for chunk j, the dims that the lanes of the keys hold there.
-    constexpr int STEPS = D / 32;
+    // Operand A for step s: the dims that lane (m, g) of the keys holds there, head m.  Chunk c of a row is 16 bytes.
     u32x4 q[STEPS];
     const u32x4* const qp = reinterpret_cast<const u32x4*>(a.q + ((size_t)b * H_q + h * a.group + (m < a.group ? m : 0)) * D);
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) q[s] = m < a.group ? qp[E4M3 ? 2 * (g + 4 * (s >> 1)) + (s & 1) : g + 4 * s] : u32x4{0u, 0u, 0u, 0u};
+    for (int s = 0; s < STEPS; ++s) q[s] = m < a.group ? qp[PARTS * (g + 4 * (s / PARTS)) + s % PARTS] : u32x4{0u, 0u, 0u, 0u};
     float shift[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -97,27 +118,43 @@ __global__ __launch_bounds__(kMassWaves * 64) void mass_step_kernel(MassArgs a) 
         shift[i] = r < a.group ? row_shift(a.lse[(size_t)b * H_q + h * a.group + r]) : INFINITY;
     }
     float* const mass = a.mass + ((size_t)b * a.cache.n_kv_heads + h) * a.mass_ld;
+    // A chunk's part as operand B.
+    auto operand = [&](const u32x4& w, int part_of) __attribute__((always_inline)) {
+        if constexpr (E4M3) return codes_to_bf16x8(w[2 * part_of], w[2 * part_of + 1]);
+        else return w;
+    };
     for (; key0 < end; key0 += 64 * kMassWaves) {
         float sum = 0.f;
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < 4; ++t) {  // 16 keys
+            f32x4 s;
+            if constexpr (HALVES) {
+                f32x4 acc[2][2];  // [eight keys][half of a line]
 #pragma unroll
-            for (int s = 0; s < STEPS; ++s) {
-                u32x4 kb;
-                if constexpr (E4M3) {
-                    const u32x4& w = k[t][s >> 1];
-                    kb = codes_to_bf16x8(w[2 * (s & 1)], w[2 * (s & 1) + 1]);
-                } else {
-                    kb = k[t][s];
+                for (int x = 0; x < 2; ++x) {
+                    acc[x][0] = acc[x][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int y = 0; y < LINES; ++y)
+#pragma unroll
+                        for (int u = 0; u < PARTS; ++u) {
+                            const u32x4 kb = operand(k[(2 * t + x) * LINES + y], u);
+#pragma unroll
+                            for (int half = 0; half < 2; ++half)
+                                acc[x][half] = mfma16(q[(2 * y + half) * PARTS + u], kb, acc[x][half]);
+                        }
                 }
-                acc = mfma16(q[s], kb, acc);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[i] = add_far(low ? acc[0][0][i] : acc[1][1][i], low ? acc[1][0][i] : acc[0][1][i]);
+            } else {
+                s = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int u = 0; u < PARTS; ++u) s = mfma16(q[u], operand(k[t], u), s);
             }
             float c = a.scale_log2;
             if constexpr (E4M3) c *= scale[t];
             float p = 0.f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) p += fast_exp2(fmaf(mapped ? acc[i] : 0.f, c, -shift[i]));
+            for (int i = 0; i < 4; ++i) p += fast_exp2(fmaf(mapped ? s[i] : 0.f, c, -shift[i]));
             p = pair_sum32(pair_sum16(p));
             sum = g == t ? p : sum;
         }
@@ -128,11 +165,12 @@ __global__ __launch_bounds__(kMassWaves * 64) void mass_step_kernel(MassArgs a) 
     }
 }
 
-// A block of query rows of sequence b: the rows of a kv head's group, [group][q_len] in order, in tiles of 32; a work-group
-// takes the tiles part, part + parts, ... and KT * 32 keys a wave.
-template <int D, bool E4M3, int KT>
+// A block of query rows of sequence b: the rows of a kv head's group, [group][q_len] in order, in stages of RT tiles of 32;
+// a work-group takes the stages part, part + parts, ... and KT * 32 keys a wave.  The stage is as long as it is because one
+// tile's products take a quarter of the time that the next rows are on their way from the L2.
+template <int D, bool E4M3, int KT, int RT>
 __global__ __launch_bounds__(kMassWaves * 64, 2) void mass_block_kernel(MassArgs a) {
-    constexpr int NCH = D / 8, STEPS = D / 16, KEYS = 32 * KT;
+    constexpr int NCH = D / 8, STEPS = D / 16, KEYS = 32 * KT, ROWS = 32 * RT;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, half = lane >> 5;
     // kv heads in turn over the work-groups (XCDs), so that one's query rows stay in few L2s.
@@ -143,8 +181,8 @@ __global__ __launch_bounds__(kMassWaves * 64, 2) void mass_block_kernel(MassArgs
     if (wg_key >= a.kv_len) return;
     const int key0 = wg_key + KEYS * wave;
 
-    __shared__ __attribute__((aligned(16))) u32x4 tile[2][32 * NCH];
-    __shared__ __attribute__((aligned(16))) float shifts[2][32];
+    __shared__ __attribute__((aligned(16))) u32x4 rows_in[2][ROWS * NCH];
+    __shared__ __attribute__((aligned(16))) float shifts[2][ROWS];
 
     // Operand B: lane l keeps dims 16 s + 8 (l / 32) .. of key l % 32 of each tile.
     u32x4 k[KT][STEPS];
@@ -170,85 +208,90 @@ __global__ __launch_bounds__(kMassWaves * 64, 2) void mass_block_kernel(MassArgs
         }
     }
 
-    const int rows = a.group * a.q_len, tiles = (rows + 31) / 32;
+    const int rows = a.group * a.q_len, stages = (rows + ROWS - 1) / ROWS;
     const uint16_t* const q = a.q + (size_t)h * rows * D;
     const float* const lse = a.lse + (size_t)h * rows;
-    // The last row position that sees the work-group's first key decides whether a tile is worked on at all: of one head,
-    // its last row; of two, both ends.
+    // The last row that sees the work-group's first key decides whether a stage is worked on at all: of one head's rows
+    // their last, of several heads' any.
     const int64_t first_seen = (int64_t)a.kv_pos_base + wg_key - a.q_pos_base;  // the least query row that sees wg_key
-    auto seen = [&](int t) __attribute__((always_inline)) {
-        if (!a.causal) return true;
-        const int r0 = 32 * t, r1 = min(r0 + 31, rows - 1);
-        const int i0 = r0 % a.q_len, i1 = r1 % a.q_len;
-        return (r1 - r0 != i1 - i0 ? (int64_t)a.q_len - 1 : (int64_t)i1) >= first_seen;
+    auto next_seen = [&](int st) __attribute__((always_inline)) {
+        if (a.causal)
+            for (; st < stages; st += a.parts) {
+                const int i0 = ROWS * st % a.q_len, n = min(ROWS, rows - ROWS * st);
+                if ((int64_t)min(i0 + n, a.q_len) > first_seen) break;
+            }
+        return st;
     };
-    constexpr int PER = 32 * NCH / (kMassWaves * 64);  // 16-byte chunks of a tile per thread
-    static_assert(PER >= 1, "a tile is a load a thread at least");
+    constexpr int THREADS = kMassWaves * 64, PER = ROWS * NCH / THREADS;  // 16-byte chunks of a stage per thread
+    static_assert(PER >= 1 && ROWS <= THREADS, "a stage is a load a thread at least");
     u32x4 in[PER];
-    float in_shift = INFINITY;
-    auto load = [&](int t) __attribute__((always_inline)) {
+    float in_lse = 0.f;
+    auto load = [&](int st) __attribute__((always_inline)) {
+        const u32x4* const from = reinterpret_cast<const u32x4*>(q) + (size_t)ROWS * st * NCH;
+        const int n = rows - ROWS * st;  // rows left
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int slot = i * kMassWaves * 64 + threadIdx.x, r = 32 * t + slot / NCH;
-            in[i] = r < rows ? reinterpret_cast<const u32x4*>(q)[(size_t)r * NCH + slot % NCH] : u32x4{0u, 0u, 0u, 0u};
+            const int slot = i * THREADS + threadIdx.x;
+            in[i] = slot / NCH < n ? from[slot] : u32x4{0u, 0u, 0u, 0u};
         }
-        if (threadIdx.x < 32) {
-            const int r = 32 * t + threadIdx.x;
-            in_shift = r < rows ? row_shift(lse[r]) : INFINITY;
-        }
-    };
-    auto next_seen = [&](int t) __attribute__((always_inline)) {
-        while (t < tiles && !seen(t)) t += a.parts;
-        return t;
+        if (threadIdx.x < ROWS) in_lse = (int)threadIdx.x < n ? lse[ROWS * st + threadIdx.x] : INFINITY;  // (worked on as it is stored)
     };
     float sum[KT];
 #pragma unroll
     for (int t = 0; t < KT; ++t) sum[t] = 0.f;
-    int t = next_seen(part), at = 0;
-    if (t < tiles) load(t);
-    for (; t < tiles; at ^= 1) {
+    const int64_t sees = (int64_t)a.kv_pos_base + key0 - a.q_pos_base;  // the least query row that sees the wave's first key
+    const int first_row = (int)(sees < -(1 << 30) ? -(1 << 30) : sees) + col;
+    int st = next_seen(part), at = 0;
+    if (st < stages) load(st);
+    for (; st < stages; at ^= 1) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int slot = i * kMassWaves * 64 + threadIdx.x, r = slot / NCH, c = slot % NCH;
-            tile[at][r * NCH + (c ^ (NCH == 16 ? r & 15 : (r >> 1) & 7))] = in[i];
+            const int slot = i * THREADS + threadIdx.x, r = slot / NCH, c = slot % NCH;
+            rows_in[at][r * NCH + (c ^ (NCH == 16 ? r & 15 : (r >> 1) & 7))] = in[i];
         }
-        if (threadIdx.x < 32) shifts[at][threadIdx.x] = in_shift;
-        const int next = next_seen(t + a.parts);
-        if (next < tiles) load(next);
-        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the tile is written; the loads stay in flight
-        __builtin_amdgcn_s_barrier();  // (two tiles: the one before is read by now, or will not be written before the next barrier)
+        if (threadIdx.x < ROWS) shifts[at][threadIdx.x] = row_shift(in_lse);
+        const int next = next_seen(st + a.parts);
+        if (next < stages) load(next);
+        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the stage is written; the loads stay in flight
+        __builtin_amdgcn_s_barrier();  // (two stages: the one before is read by now, or will not be written before the next barrier)
         asm volatile("" ::: "memory");
-        const int i0 = 32 * t % a.q_len;
-        f32x16 acc[KT];
+        // Whether some row of the stage does not see some key of the wave.
+        const int i0 = ROWS * st % a.q_len;
+        const bool several = i0 + ROWS > a.q_len;
+        const bool mask = a.causal && (several || i0 < sees + KEYS - 1);
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
+        for (int rt = 0; rt < RT; ++rt) {
+            f32x16 acc[KT];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[kt][i] = 0.f;
+            for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s) {
-            const u32x4 qa = tile[at][col * NCH + ((2 * s + half) ^ (NCH == 16 ? col & 15 : (col >> 1) & 7))];
+                for (int i = 0; i < 16; ++i) acc[kt][i] = 0.f;
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt) acc[kt] = mfma32(qa, k[kt][s], acc[kt]);
-        }
-        // Whether some row of the tile does not see some key of the wave.
-        const bool mask = a.causal && (i0 + 31 >= a.q_len || (int64_t)i0 + a.q_pos_base < (int64_t)a.kv_pos_base + key0 + KEYS - 1);
+            for (int s = 0; s < STEPS; ++s) {
+                const u32x4 qa = rows_in[at][(32 * rt + col) * NCH + ((2 * s + half) ^ (NCH == 16 ? col & 15 : (col >> 1) & 7))];
 #pragma unroll
-        for (int i4 = 0; i4 < 4; ++i4) {
-            const f32x4 shift = *reinterpret_cast<const f32x4*>(&shifts[at][8 * i4 + 4 * half]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-#pragma unroll
-                for (int kt = 0; kt < KT; ++kt) {
-                    float p = fast_exp2(fmaf(acc[kt][4 * i4 + i], scale[kt], -shift[i]));
-                    if (mask) {
-                        const int r = (32 * t + 8 * i4 + 4 * half + i) % a.q_len;
-                        if ((int64_t)r + a.q_pos_base < (int64_t)a.kv_pos_base + key0 + 32 * kt + col) p = 0.f;
-                    }
-                    sum[kt] += p;
-                }
+                for (int kt = 0; kt < KT; ++kt) acc[kt] = mfma32(qa, k[kt][s], acc[kt]);
             }
+            auto add = [&](auto masked) __attribute__((always_inline)) {
+#pragma unroll
+                for (int i4 = 0; i4 < 4; ++i4) {
+                    const f32x4 shift = *reinterpret_cast<const f32x4*>(&shifts[at][32 * rt + 8 * i4 + 4 * half]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        int row = i0 + 32 * rt + 8 * i4 + 4 * half + i;
+                        if (masked && several) row %= a.q_len;
+#pragma unroll
+                        for (int kt = 0; kt < KT; ++kt) {
+                            const float p = fast_exp2(fmaf(acc[kt][4 * i4 + i], scale[kt], -shift[i]));
+                            sum[kt] += masked && row < first_row + 32 * kt ? 0.f : p;
+                        }
+                    }
+                }
+            };
+            if (mask) add(std::true_type{});
+            else add(std::false_type{});
         }
-        t = next;
+        st = next;
     }
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
@@ -277,10 +320,10 @@ __global__ __launch_bounds__(256) void mass_sum_kernel(MassArgs a) {
 
 }  // namespace
 
-// Work-groups of a step: pieces of 1024 keys, or fewer down to 256 while those do not make four work-groups a CU.
+// Work-groups of a step: pieces of 512 keys, or 256 while those do not make four work-groups a CU.
 hipError_t launch_mass_step(int head_dim, MassArgs a, int n_cu, const Launch& l) {
     const int64_t units = (int64_t)a.batch * a.cache.n_kv_heads;
-    a.chunk = 1024;
+    a.chunk = 512;
     while (a.chunk > 256 && units * ((a.cache.l_max + a.chunk - 1) / a.chunk) < 4 * n_cu) a.chunk /= 2;
     a.parts = (a.cache.l_max + a.chunk - 1) / a.chunk;
     const int64_t wgs = units * a.parts;
@@ -297,10 +340,8 @@ hipError_t launch_mass_step(int head_dim, MassArgs a, int n_cu, const Launch& l)
 MassPlan plan_mass_block(int group, int n_kv_heads, int q_len, int kv_len, int n_cu) {
     const int tiles = (int)(((int64_t)group * q_len + 31) / 32);
     MassPlan p;
-    p.key_tiles = 2;
-    auto wgs = [&](int kt) { return (int64_t)n_kv_heads * ((kv_len + 128 * kt - 1) / (128 * kt)); };
-    if (wgs(2) < 2 * n_cu) p.key_tiles = 1;
-    const int64_t of_keys = wgs(p.key_tiles);
+    p.key_tiles = kv_len > 128 ? 2 : 1;
+    const int64_t keys = 32 * p.key_tiles * kMassWaves, of_keys = n_kv_heads * ((kv_len + keys - 1) / keys);
     p.parts = (int)std::max<int64_t>(1, std::min<int64_t>({4 * n_cu / of_keys, (int64_t)tiles / 4, kMassMaxParts}));
     return p;
 }
@@ -311,7 +352,7 @@ static hipError_t launch_mass_block_t(const MassArgs& a, int key_tiles, const La
     const int64_t wgs = (int64_t)a.cache.n_kv_heads * a.parts * ((a.kv_len + keys - 1) / keys);
     if (wgs > INT32_MAX) return hipErrorInvalidValue;
     const dim3 grid = wide_grid(wgs), block(kMassWaves * 64);
-    return key_tiles == 2 ? launch_kernel(mass_block_kernel<D, E4M3, 2>, grid, block, l, a) : launch_kernel(mass_block_kernel<D, E4M3, 1>, grid, block, l, a);
+    return key_tiles == 2 ? launch_kernel(mass_block_kernel<D, E4M3, 2, kRowTiles>, grid, block, l, a) : launch_kernel(mass_block_kernel<D, E4M3, 1, kRowTiles>, grid, block, l, a);
 }
 
 hipError_t launch_mass_block(int head_dim, const MassArgs& a, int key_tiles, const Launch& l) {
