@@ -489,9 +489,9 @@ int gqa_qk_norm_rotary_step_device(gqa_ctx* ctx, const void* qkv, int64_t ld, co
  * document): the rows that they share are held once, as the first rows of a sequence of the cache, and read once a step for
  * the whole batch.  gqa_decode_prefix_device is gqa_decode_device where sequence b attends rows 0 .. prefix_lens[b] - 1 of
  * sequence prefix_b and then rows 0 .. ctx_lens[b] - 1 of its own, as one softmax (o and lse over both).  prefix_lens [B] is
- * in device memory, each held to 0 .. prefix_len; NULL: prefix_len for every sequence.  Sequence prefix_b is one of the batch
- * like the others (0 and 0 for a slot that only holds the prefix: zeros, -inf); where it goes on behind the prefix itself, 0
- * for its prefix_lens and all of its rows for its ctx_lens.  gqa_decode_append_prefix_device appends first, as
+ * in device memory, each held to 0 .. prefix_len; NULL: prefix_len for every sequence.  Sequence prefix_b, whose rows the
+ * prefix is, attends rows 0 .. ctx_lens - 1 and no other (ctx_lens 0 for a slot that only holds the prefix: zeros, -inf; the
+ * prefix's rows and those behind for one that goes on itself).  gqa_decode_append_prefix_device appends first, as
  * gqa_decode_append_device does, one row of each sequence's own; a row below prefix_len of sequence prefix_b is not written.
  * bf16 and E4M3 caches, contiguous and paged (rows 0 .. prefix_len - 1 of prefix_b are mapped, else GQA_ERR_RANGE), groups of
  * 1 .. 16.  Error as of decode; a V row that holds an infinity or NaN reaches the sequences that see it and no others.

@@ -387,7 +387,7 @@ struct PrefixArgs {
     const uint16_t* v_new;
     const int32_t* positions;   // [B]
     const int32_t* lens;        // [B] own rows
-    const int32_t* shared;      // [B] rows of the prefix, nullptr: prefix_len
+    const int32_t* shared;      // [B] rows of the prefix, nullptr: prefix_len (prefix_b's is not read: it has its own rows alone)
     int32_t batch, group;
     int32_t prefix_b, prefix_len;
     float scale_log2;
@@ -396,12 +396,12 @@ struct PrefixArgs {
     int32_t chunk, pieces;      // the prefix in pieces of `chunk` keys, a work-group each
     int32_t own_wgs;            // work-groups for the sequences' own rows
     int32_t own_slots;          // partials that own_part holds
-    float* part_o;              // prefix [pieces][H_kv][B * group][D], then own [own_slots][group][D]
+    float* part_o;              // prefix [pieces][H_kv][(B - 1) * group][D], then own [own_slots][group][D]
     float* part_ml;             // the same rows' (maximum in log2 units, sum)
     uint16_t* out;              // [B][H_q][D]
     float* lse;                 // [B][H_q] or nullptr
 };
-constexpr int kPrefixOwnSlots = 4096;  // at least; one per (sequence, kv head) where those are more
+constexpr int kPrefixOwnSlots = 16384;  // at least; one per (sequence, kv head) where those are more
 void plan_prefix(PrefixArgs* a, int n_cu);
 // Rows of part_o (and part_ml) that plan_prefix may ask for, whatever the prefix.
 int64_t prefix_partial_rows_max(int batch, int n_kv_heads, int group, int n_cu);

@@ -81,6 +81,7 @@ class Batch:
         kp, vp = (stored(t, self.kv_format) for t in (self.k[-1], self.v[-1]))
         for b in range(self.B):
             p = self.prefix if shared is None else min(max(int(shared[b]), 0), self.prefix)
+            p = 0 if b == self.B - 1 else p  # (the prefix's own sequence has its rows alone)
             n = int(lens[b])
             k, v = self.k[b][:, :n].copy(), self.v[b][:, :n].copy()
             if append and 0 <= positions[b] < n:
@@ -209,7 +210,7 @@ def test_a_prefix_that_goes_on_and_rows_not_appended_to_it():
         batch.acc.load_kv(hold, hold, b=3, start_pos=130)
         batch.k[3], batch.v[3] = np.concatenate((batch.k[3], hold), 1), np.concatenate((batch.v[3], hold), 1)
         lens = np.array([20, 9, 64, 150], np.int32)
-        shared = np.array([130, 130, 50, 0])
+        shared = np.array([130, 130, 50, 130])
         pos = np.array([4, 200, 64, 149], np.int32)  # inside; out of range; written but not attended
         batch.check(*batch.run(shared, lens=lens, positions=pos), shared, lens=lens, positions=pos)
         assert np.array_equal(batch.acc.read_kv(2, 64, 1)[0][:, 0], batch.k_new[2])
