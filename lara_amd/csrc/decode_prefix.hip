@@ -32,8 +32,11 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kWaves = 8;
-constexpr int kOwnKeys = 32;  // keys of a step of own rows
+constexpr int kOwnKeys = kPrefixOwnKeys;
 
+__device__ __forceinline__ f32x4 mfma16(const u32x4& a, const u32x4& b, const f32x4& c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
 __device__ __forceinline__ f32x16 mfma32(const u32x4& a, const u32x4& b, const f32x16& c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
 }
@@ -61,6 +64,12 @@ __device__ __forceinline__ u32x4 codes_to_bf16x8(uint32_t lo, uint32_t hi, float
                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true))};
 }
 
+// The same for transposing reads of eight (own rows).
+template <int D>
+__device__ __forceinline__ int v_chunk_own(int row, int c) {
+    return c ^ 2 * (D == 128 ? row & 7 : (row >> 1) & 3);
+}
+
 // LDS traffic of the wave is complete; its global loads stay in flight.
 __device__ __forceinline__ void lds_done() {
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
@@ -79,25 +88,34 @@ constexpr int kRoundKeys = 32 * kWaves;  // keys that a work-group has in LDS
 template <int D>
 constexpr int tile_bytes() { return kWaves * 2 * kOwnKeys * D * 2; }
 
-// ---- own rows' pieces ------------------------------------------------------------------------------------
+// ---- runs of own rows ------------------------------------------------------------------------------------
 
-// Lengths of own rows, 64 sequences at a time, one per lane.
 __device__ __forceinline__ int own_len(const PrefixArgs& a, int s) { return s < a.batch ? clamp_len(a.lens[s], a.cache.l_max) : 0; }
+__device__ __forceinline__ int own_steps(int len) { return (len + kOwnKeys - 1) / kOwnKeys; }
 
-// Pieces have 2^log2 keys, the least of 64 and more with which they fit the partials and there are at most `most` of
-// them -- or one each, which always fits.  (The same for every wave and both launches: it follows from the lengths.)
-constexpr int kOwnLog2 = 6;
-__device__ __forceinline__ int own_pieces(int len, int log2) { return (len + (1 << log2) - 1) >> log2; }
-__device__ __forceinline__ int own_log2(const PrefixArgs& a) {
-    const int lane = threadIdx.x & 63;
-    const int64_t most = a.own_slots;
-    for (int log2 = kOwnLog2; log2 < 30; ++log2) {
-        int64_t n = 0;
-        for (int c0 = 0; c0 < a.batch; c0 += 64) n += __builtin_amdgcn_readlane(wave_scan(own_pieces(own_len(a, c0 + lane), log2)), 63);
-        if (n * a.cache.n_kv_heads <= most) return log2;
+// The steps (32 keys) of all (sequence, kv head)s in order are cut into one run for every wave of the launch: `first` steps
+// for the first `others` waves and `rest` for the others, those of work-groups that had a part of the prefix and come late by
+// about as many steps as the difference.  It follows from the lengths, so that both launches know it (all steps
+// are at most 2^30: the caller sees to it).  A part of a (sequence,
+// kv head) u in the run of wave w leaves its partial in slot u + w (one of the two rises from part to part).
+struct Runs {
+    int others, first, rest;
+    __device__ __forceinline__ Runs(const PrefixArgs& a, int prefix_wgs, int wgs) {
+        const int lane = threadIdx.x & 63;
+        int steps = 0;
+        for (int c0 = 0; c0 < a.batch; c0 += 64) steps += __builtin_amdgcn_readlane(wave_scan(own_steps(own_len(a, c0 + lane))), 63);
+        steps *= a.cache.n_kv_heads;
+        others = (wgs - prefix_wgs) * kWaves;
+        const int waves = wgs * kWaves;
+        const int late = others > 0 && prefix_wgs > 0 ? kLateSteps + a.chunk / kRoundKeys : 0;
+        rest = steps > others * late ? (steps - others * late + waves - 1) / waves : 0;
+        first = rest > 0 ? rest + late : others > 0 ? (steps + others - 1) / others : 0;
     }
-    return 30;
-}
+    // Where wave w's run begins, and the wave in whose run step `at` lies.
+    __device__ __forceinline__ int begin(int w) const { return w < others ? w * first : others * first + (w - others) * rest; }
+    __device__ __forceinline__ int wave_of(int at) const { return at < others * first ? at / first : others + (at - others * first) / rest; }
+    static constexpr int kLateSteps = 2;  // a part of the prefix costs about this and a step for each of its rounds
+};
 
 // ---- one task: 32 query rows over a run of tiles -----------------------------------------------------------
 
@@ -119,23 +137,30 @@ __device__ __forceinline__ void rows_clear(Rows<D>& r) {
     r.l = 0.f;
 }
 
-// A tile of NT * 32 keys on its way into LDS through the registers of TEAM waves; `t` is the thread's place among them.  ONCE:
-// nothing else reads the rows (loads that pass the L2 stream faster).  FINITE: zeros take the place of infinities and NaN in V,
-// and store() says whether there were any.
-template <int D, bool E4M3, int NT, int TEAM, bool ONCE, bool FINITE>
+// A wave's share of a tile on its way into LDS: 32 keys for each wave that the tile serves.
+template <int D, bool E4M3>
+struct Loaded {
+    static constexpr int PIECES = E4M3 ? D / 16 : D / 8;  // 16-byte loads of a row
+    static constexpr int N = 32 * PIECES / 64;
+    u32x4 k[N], v[N];
+    uint8_t ks[N], vs[N];  // E4M3: scale bytes
+    int live[2];           // rows that hold keys, of the first 64 and the others
+};
+
+// A tile of 32 * TEAM keys, loaded by TEAM waves; `t` is the thread's place among them.  OWN: nothing else reads the rows
+// (loads that pass the L2 stream faster); the others' V has zeros for infinities and NaN, and store() says whether there were
+// any.
+template <int D, bool E4M3, int TEAM, bool OWN>
 struct Staged {
-    static constexpr int NCH = D / 8, KEYS = 32 * NT, THREADS = 64 * TEAM;
-    static constexpr int PIECES = E4M3 ? D / 16 : NCH;  // 16-byte loads of a row
-    static constexpr int N = KEYS * PIECES / THREADS;
-    static_assert(N >= 1 && N * THREADS == KEYS * PIECES, "whole loads");
+    using Share = Loaded<D, E4M3>;
+    static constexpr int NCH = D / 8, KEYS = 32 * TEAM, THREADS = 64 * TEAM;
+    static constexpr int PIECES = Loaded<D, E4M3>::PIECES, N = Loaded<D, E4M3>::N;
     // Rows of up to 64 keys lie together (a page's, at least); a tile of more has two such parts.
     static constexpr int PARTS = KEYS > 64 ? KEYS / 64 : 1, PER = N / PARTS;
     static_assert(PARTS * PER == N, "loads of one part each");
-    u32x4 k[N], v[N];
-    uint8_t ks[N], vs[N];  // E4M3: scale bytes
-    int live[PARTS];       // rows of a part that hold keys
+    static_assert(PARTS <= 2, "live");
 
-    __device__ __forceinline__ void load(const PrefixArgs& a, int b, int h, int key0, int end, int t) {
+    __device__ static __forceinline__ void load(Share& x, const PrefixArgs& a, int b, int h, int key0, int end, int t) {
         const uint32_t at = 16 * t, row_at = (uint32_t)t / PIECES;
 #pragma unroll
         for (int g = 0; g < PARTS; ++g) {
@@ -145,7 +170,7 @@ struct Staged {
                 row = ((int64_t)b * a.cache.n_kv_heads + h) * a.cache.l_cap + key;
             else
                 row = paged_row_uniform(a.cache.block_table + (size_t)b * a.cache.max_pages, a.cache.page_shift, a.cache.n_kv_heads, h, key);
-            live[g] = row < 0 ? 0 : end - key0 - 64 * g;  // (an unmapped page: rows of zeros, from any that is there)
+            x.live[g] = row < 0 ? 0 : end - key0 - 64 * g;  // (an unmapped page: rows of zeros, from any that is there)
             if (row < 0) row = 0;
             // (a uniform base and a 32-bit offset a lane)
             const uint8_t* const kp = a.cache.k + row * (PIECES * 16);
@@ -154,36 +179,36 @@ struct Staged {
             for (int i = 0; i < PER; ++i) {
                 const u32x4* const kfrom = reinterpret_cast<const u32x4*>(kp + i * (THREADS * 16) + at);
                 const u32x4* const vfrom = reinterpret_cast<const u32x4*>(vp + i * (THREADS * 16) + at);
-                k[g * PER + i] = ONCE ? __builtin_nontemporal_load(kfrom) : *kfrom;
-                v[g * PER + i] = ONCE ? __builtin_nontemporal_load(vfrom) : *vfrom;
+                x.k[g * PER + i] = OWN ? __builtin_nontemporal_load(kfrom) : *kfrom;
+                x.v[g * PER + i] = OWN ? __builtin_nontemporal_load(vfrom) : *vfrom;
             }
             if constexpr (E4M3)
 #pragma unroll
                 for (int i = 0; i < PER; ++i) {
-                    ks[g * PER + i] = (a.cache.k_scale + row + i * (THREADS / PIECES))[row_at];
-                    vs[g * PER + i] = (a.cache.v_scale + row + i * (THREADS / PIECES))[row_at];
+                    x.ks[g * PER + i] = (a.cache.k_scale + row + i * (THREADS / PIECES))[row_at];
+                    x.vs[g * PER + i] = (a.cache.v_scale + row + i * (THREADS / PIECES))[row_at];
                 }
         }
     }
-    __device__ __forceinline__ bool store(u32x4* lk, u32x4* lv, int t) {
+    __device__ static __forceinline__ bool store(Share& x, u32x4* lk, u32x4* lv, int t) {
         bool odd = false;
-        if constexpr (FINITE) odd = clear_odd();
+        if constexpr (!OWN) odd = clear_odd(x);
         auto put = [&](int part, int key, int c, u32x4 kw, u32x4 vw) __attribute__((always_inline)) {
-            if (live[part] < (KEYS < 64 ? KEYS : 64) && key - 64 * part >= live[part]) kw = vw = u32x4{0u, 0u, 0u, 0u};
+            if (x.live[part] < (KEYS < 64 ? KEYS : 64) && key - 64 * part >= x.live[part]) kw = vw = u32x4{0u, 0u, 0u, 0u};
             lk[key * NCH + k_chunk<D>(key, c)] = kw;
-            lv[key * NCH + v_chunk<D>(key, c)] = vw;
+            lv[key * NCH + (OWN ? v_chunk_own<D>(key, c) : v_chunk<D>(key, c))] = vw;
         };
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int slot = i * THREADS + t, key = slot / PIECES, c = slot % PIECES;
             if constexpr (E4M3) {
-                const float kscale = kv8_scale(ks[i]), vscale = kv8_scale(vs[i]);
+                const float kscale = kv8_scale(x.ks[i]), vscale = kv8_scale(x.vs[i]);
 #pragma unroll
                 for (int half = 0; half < 2; ++half)
-                    put(i / PER, key, 2 * c + half, codes_to_bf16x8(k[i][2 * half], k[i][2 * half + 1], kscale),
-                        codes_to_bf16x8(v[i][2 * half], v[i][2 * half + 1], vscale));
+                    put(i / PER, key, 2 * c + half, codes_to_bf16x8(x.k[i][2 * half], x.k[i][2 * half + 1], kscale),
+                        codes_to_bf16x8(x.v[i][2 * half], x.v[i][2 * half + 1], vscale));
             } else {
-                put(i / PER, key, c, k[i], v[i]);
+                put(i / PER, key, c, x.k[i], x.v[i]);
             }
         }
         return odd;
@@ -192,21 +217,21 @@ struct Staged {
   private:
     // Zeros for infinities and NaN among the V values in the registers; whether there were any (in rows behind the end, too:
     // add_odd() looks closer).  A value's exponent of ones (a code's seven ones) carries into the bit above it.
-    __device__ __forceinline__ bool clear_odd() {
+    __device__ static __forceinline__ bool clear_odd(Share& x) {
         constexpr uint32_t FIELD = E4M3 ? 0x7F7F7F7Fu : 0x7F807F80u, ONE = E4M3 ? 0x01010101u : 0x00800080u, TOP = E4M3 ? 0x80808080u : 0x80008000u;
         uint32_t any = 0;
 #pragma unroll
         for (int i = 0; i < N; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) any |= (v[i][j] & FIELD) + ONE;
+            for (int j = 0; j < 4; ++j) any |= (x.v[i][j] & FIELD) + ONE;
         if (__ballot((any & TOP) != 0) == 0) return false;
         constexpr int BITS = E4M3 ? 8 : 16;
 #pragma unroll
         for (int i = 0; i < N; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const uint32_t at = (((v[i][j] & FIELD) + ONE) & TOP) >> (BITS - 1);  // a one for each
-                v[i][j] &= ~(at * ((1u << BITS) - 1u));
+                const uint32_t at = (((x.v[i][j] & FIELD) + ONE) & TOP) >> (BITS - 1);  // a one for each
+                x.v[i][j] &= ~(at * ((1u << BITS) - 1u));
             }
         return (any & TOP) != 0;
     }
@@ -292,19 +317,6 @@ __device__ __forceinline__ void attend(Rows<D>& r, const u32x4* lk, const u32x4*
     }
 }
 
-// The lane's row of a partial: 4 dims a store, in the order of the registers.
-template <int D>
-__device__ __forceinline__ void store_partial(const PrefixArgs& a, const Rows<D>& r, float l, size_t row) {
-    const int half = (threadIdx.x & 63) >> 5;
-#pragma unroll
-    for (int t = 0; t < D / 32; ++t)
-#pragma unroll
-        for (int i4 = 0; i4 < 4; ++i4)
-            *reinterpret_cast<f32x4*>(a.part_o + row * D + 32 * t + 8 * i4 + 4 * half) =
-                f32x4{r.o[t][4 * i4], r.o[t][4 * i4 + 1], r.o[t][4 * i4 + 2], r.o[t][4 * i4 + 3]};
-    if (half == 0) reinterpret_cast<float2*>(a.part_ml)[row] = make_float2(r.m, l);
-}
-
 // ---- the prefix ---------------------------------------------------------------------------------------------
 
 // Query rows that attend it, per kv head: every sequence's but its own.
@@ -339,9 +351,10 @@ __device__ __forceinline__ void add_odd(Rows<D>& r, const PrefixArgs& a, int h, 
                 }
 }
 
+// last() is called when the last rows are in LDS: what it loads into `first` comes while they are worked on.
 // TEAM waves share 32 * TEAM keys in LDS at a time, for 32 rows each; the work-group's TEAMS teams take the others of a round.
-template <int D, bool E4M3, int TEAM>
-__device__ __forceinline__ void prefix_task(const PrefixArgs& a, int index, uint8_t* lds, float2* lds_ml, int* lds_odd) {
+template <int D, bool E4M3, int TEAM, typename Last>
+__device__ __forceinline__ void prefix_task(const PrefixArgs& a, int index, uint8_t* lds, float2* lds_ml, int* lds_odd, Loaded<D, E4M3>& first, Last&& last) {
     constexpr int NT = 1, KEYS = 32 * TEAM, TEAMS = kWaves / TEAM, NCH = D / 8;
     const int lane = threadIdx.x & 63, col = lane & 31, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int tile_of = wave % TEAM, team = wave / TEAM, t = threadIdx.x % (64 * TEAM);
@@ -353,8 +366,8 @@ __device__ __forceinline__ void prefix_task(const PrefixArgs& a, int index, uint
 
     u32x4* const lk = reinterpret_cast<u32x4*>(lds) + (size_t)team * 2 * KEYS * NCH;
     u32x4* const lv = lk + KEYS * NCH;
-    Staged<D, E4M3, TEAM, TEAM, false, true> staged;
-    if (begin + team * KEYS < end) staged.load(a, a.prefix_b, h, begin + team * KEYS, end, t);
+    using Tile = Staged<D, E4M3, TEAM, false>;
+    if (begin + team * KEYS < end) Tile::load(first, a, a.prefix_b, h, begin + team * KEYS, end, t);
 
     const int row = (block * TEAM + tile_of) * 32 + col;
     int b = row / a.group;
@@ -379,8 +392,9 @@ __device__ __forceinline__ void prefix_task(const PrefixArgs& a, int index, uint
     for (int round = begin; round < end; round += kRoundKeys) {
         const int key0 = round + team * KEYS;
         if (TEAM > 1 && round > begin) lds_barrier();  // the round before is read
-        if (key0 < end) odd |= staged.store(lk, lv, t);
-        if (key0 + kRoundKeys < end) staged.load(a, a.prefix_b, h, key0 + kRoundKeys, end, t);
+        if (key0 < end) odd |= Tile::store(first, lk, lv, t);
+        if (key0 + kRoundKeys < end) Tile::load(first, a, a.prefix_b, h, key0 + kRoundKeys, end, t);
+        if (round + kRoundKeys >= end) last();
         if constexpr (TEAM > 1) lds_barrier();
         else lds_done();
         for (int k = 0; k < KEYS; k += 32 * NT)
@@ -409,27 +423,35 @@ __device__ __forceinline__ void prefix_task(const PrefixArgs& a, int index, uint
     lds_barrier();
     const int row0 = block * TEAM * 32;
     const size_t to = ((size_t)piece * a.cache.n_kv_heads + h) * rows + row0;
-    for (int i = threadIdx.x; i < TEAM * 32 * WORDS; i += kWaves * 64) {
-        const int at = i / WORDS, word = i % WORDS;  // row of the block
-        if (row0 + at >= rows) break;
-        float M = lds_ml[at].x;
+    constexpr int THREADS = kWaves * 64, EACH = TEAM * 32 * WORDS / THREADS;
+    const int word = threadIdx.x % WORDS;
 #pragma unroll
-        for (int k = 1; k < TEAMS; ++k) M = fmaxf(M, lds_ml[k * TEAM * 32 + at].x);
+    for (int i = 0; i < EACH; ++i) {
+        const int at = (i * THREADS + threadIdx.x) / WORDS;  // row of the block
+        float2 ml[TEAMS];
+        f32x4 v[TEAMS];
+#pragma unroll
+        for (int k = 0; k < TEAMS; ++k) {
+            ml[k] = lds_ml[k * TEAM * 32 + at];
+            v[k] = lo[(k * TEAM * 32 + at) * WORDS + (word ^ (at & 31 & (WORDS - 1)))];
+        }
+        float M = ml[0].x;
+#pragma unroll
+        for (int k = 1; k < TEAMS; ++k) M = fmaxf(M, ml[k].x);
         const float base = softmax_base(M);
         f32x4 O = {0.f, 0.f, 0.f, 0.f};
         float L = 0.f;
 #pragma unroll
         for (int k = 0; k < TEAMS; ++k) {
-            const int from = k * TEAM * 32 + at;
-            const float2 ml = lds_ml[from];
-            const float f = fast_exp2(ml.x - base);
-            const f32x4 v = lo[from * WORDS + (word ^ (at & 31 & (WORDS - 1)))];
-            L = fmaf(f, ml.y, L);
+            const float f = fast_exp2(ml[k].x - base);
+            L = fmaf(f, ml[k].y, L);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) O[j] = fmaf(f, v[j], O[j]);
+            for (int j = 0; j < 4; ++j) O[j] = fmaf(f, v[k][j], O[j]);
         }
-        reinterpret_cast<f32x4*>(a.part_o)[(to + at) * WORDS + word] = O;
-        if (word == 0) reinterpret_cast<float2*>(a.part_ml)[to + at] = make_float2(M, L);
+        if (row0 + at < rows) {
+            reinterpret_cast<f32x4*>(a.part_o)[(to + at) * WORDS + word] = O;
+            if (word == 0) reinterpret_cast<float2*>(a.part_ml)[to + at] = make_float2(M, L);
+        }
     }
     lds_barrier();  // (own rows follow in the same LDS)
 }
@@ -474,111 +496,208 @@ __device__ __forceinline__ void put_row(const PrefixArgs& a, int b, int h, int k
         const u32x2 c = kv8_quantise<LANES>(x, &byte);
         w = codes_to_bf16x8(c[0], c[1], kv8_scale(byte));
     }
-    if (side) lv[key * LANES + v_chunk<D>(key, at)] = w;
+    if (side) lv[key * LANES + v_chunk_own<D>(key, at)] = w;
     else lk[key * LANES + k_chunk<D>(key, at)] = w;
 }
 
+// A wave's run of own rows as one stream of steps of 32 keys.  Two steps' loads are under way while one is worked on:
+// of the group's up to 16 heads as columns,
+//   S^T [16 keys x 16] = K . Q^T, O^T [D x 16] += V^T [D x 32 keys] . P^T by v_mfma_f32_16x16x32_bf16,
+// which needs half the registers of 32 rows.
 template <int D, bool E4M3>
-__device__ __forceinline__ void own_tasks(const PrefixArgs& a, int index, int prefix_wgs, int wgs, uint8_t* lds, size_t part0) {
-    constexpr int NCH = D / 8;
-    const int lane = threadIdx.x & 63, col = lane & 31, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int H_q = a.cache.n_kv_heads * a.group;
-    const int n_waves = wgs * kWaves, me = wave * wgs + index;
-    u32x4* const lk = reinterpret_cast<u32x4*>(lds) + (size_t)wave * 2 * kOwnKeys * NCH;
-    u32x4* const lv = lk + kOwnKeys * NCH;
+struct OwnRows {
+    static constexpr int NCH = D / 8;
+    struct Step {
+        int b, h, L, key, pos;
+        bool opens, closes, there;  // the first and last of a part; whether there is such a step
+    };
+    const PrefixArgs& a;
+    u32x4 *lk, *lv;
+    size_t part0;
+    int lane, m, g, n_waves, me;
+    int wave, left;  // the wave's place among the runs; steps left behind the last one issued
+    // A window of 64 sequences, one a lane: own rows and the appended row.
+    int c0 = -64, len = 0, pos_of = -1;
+    Step at[2], ahead;  // what the two loads under way are for; the last one issued
+    Loaded<D, E4M3> staged[2];
+    // The part's rows: lane (m, g) has head m.
+    u32x4 q[D / 32];
+    f32x4 o[D / 16];
+    float top, sum;
 
+    __device__ __forceinline__ OwnRows(const PrefixArgs& args, int index, int prefix_wgs, int wgs, uint8_t* lds) : a(args) {
+        lane = threadIdx.x & 63;
+        m = lane & 15;
+        g = lane >> 4;
+        const int in_wg = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        lk = reinterpret_cast<u32x4*>(lds) + (size_t)in_wg * 2 * kOwnKeys * NCH;
+        lv = lk + kOwnKeys * NCH;
+        part0 = (size_t)a.pieces * a.cache.n_kv_heads * prefix_rows(a);
+        n_waves = wgs * kWaves;
+        me = in_wg * wgs + index;
+        const Runs runs(a, prefix_wgs, wgs);
+        wave = index >= prefix_wgs ? in_wg * (wgs - prefix_wgs) + index - prefix_wgs : runs.others + in_wg * prefix_wgs + index;
+        const int begin = runs.begin(wave);
+        left = wave < runs.others ? runs.first : runs.rest;
+        ahead.there = left > 0 && find(begin);
+        finish();
+        at[0] = ahead;
+        forward();
+        at[1] = ahead;
+    }
     // The appended row of sequence b: inside the cache, and not among the prefix's rows, which others are reading.
-    auto row_of = [&](int b) __attribute__((always_inline)) {
-        if (a.k_new == nullptr) return -1;
+    __device__ __forceinline__ int row_of(int b) const {
+        if (a.k_new == nullptr || b >= a.batch) return -1;
         const int pos = a.positions[b];
         return pos < 0 || pos >= a.cache.l_max || (b == a.prefix_b && pos < a.prefix_len) ? -1 : pos;
-    };
-    if (a.k_new != nullptr)
+    }
+    __device__ __forceinline__ void window(int from) {
+        c0 = from;
+        len = own_len(a, c0 + lane);
+        pos_of = row_of(c0 + lane);
+    }
+    __device__ __forceinline__ void take(int i) {  // the window's i-th sequence
+        ahead.b = c0 + i;
+        ahead.L = __builtin_amdgcn_readlane(len, i);
+        ahead.pos = __builtin_amdgcn_readlane(pos_of, i);
+    }
+    // Sets `ahead` to the step that lies `to` steps behind the first of all; false: there are not so many.
+    __device__ __forceinline__ bool find(int to) {
+        int before = 0;
+        for (int from = 0; from < a.batch; from += 64) {
+            window(from);
+            const int upto = before + wave_scan(own_steps(len)) * a.cache.n_kv_heads;
+            const unsigned long long past = __ballot(upto > to);
+            if (past != 0) {
+                const int i = (int)__builtin_ctzll(past);
+                take(i);
+                const int each = own_steps(ahead.L);
+                const int in = to - (__builtin_amdgcn_readlane(upto, i) - each * a.cache.n_kv_heads);
+                ahead.h = in / each;
+                ahead.key = (in - ahead.h * each) * kOwnKeys;
+                ahead.opens = true;
+                return true;
+            }
+            before = __builtin_amdgcn_readlane(upto, 63);
+        }
+        return false;
+    }
+    __device__ __forceinline__ void finish() {
+        left -= 1;
+        ahead.closes = left == 0 || ahead.key + kOwnKeys >= ahead.L;
+    }
+    __device__ __forceinline__ void forward() {
+        if (!ahead.there) return;
+        ahead.there = left > 0;
+        if (!ahead.there) return;
+        ahead.key += kOwnKeys;
+        ahead.opens = ahead.key >= ahead.L;
+        if (ahead.opens) {
+            ahead.key = 0;
+            if (++ahead.h == a.cache.n_kv_heads) {
+                ahead.h = 0;
+                unsigned long long next = __ballot(len > 0 && lane > ahead.b - c0);
+                while (next == 0) {
+                    if (c0 + 64 >= a.batch) {
+                        ahead.there = false;
+                        return;
+                    }
+                    window(c0 + 64);
+                    next = __ballot(len > 0);
+                }
+                take((int)__builtin_ctzll(next));
+            }
+        }
+        finish();
+    }
+    __device__ __forceinline__ void append() const {
+        if (a.k_new == nullptr) return;
         for (int u = me; u < a.batch * a.cache.n_kv_heads; u += n_waves) {
             const int b = u / a.cache.n_kv_heads, pos = row_of(b);
             if (pos >= 0) append_row<D, E4M3>(a, b, u - b * a.cache.n_kv_heads, pos);
         }
-
-    const int log2 = own_log2(a);
-    // Tasks are dealt to the waves in turn.  Those of work-groups that had a part of the prefix come late: the others get the
-    // first `ahead` rounds alone (a round of the prefix, 256 keys, takes about as long as 32 own keys on every wave, and its
-    // beginning and end as two more).
-    const int others = (wgs - prefix_wgs) * kWaves, late = 2 + a.chunk / kRoundKeys;
-    const int ahead = others > 0 && prefix_wgs > 0 ? max(1, late * kOwnKeys >> log2) : 0;
-    const bool is_late = index < prefix_wgs;
-    const int me_first = is_late ? 0 : wave * (wgs - prefix_wgs) + index - prefix_wgs;
-    auto task_at = [&](int n) __attribute__((always_inline)) {  // the wave's n-th
-        if (is_late || n >= ahead) return ahead * others + (n - (is_late ? 0 : ahead)) * n_waves + me;
-        return n * others + me_first;
-    };
-    // Task i: kv head i % H_kv of piece i / H_kv, pieces of the sequences in order; a step is 32 keys of one.  What is loaded
-    // is a step ahead of what is computed, across tasks.
-    struct Step {
-        int task, b, h, L, key, end;
-    };
-    int c0 = -64, before = 0, len = 0, upto = 0;  // a window of 64 sequences: pieces before it, a lane's own rows, its pieces' running sum
-    int total = 0;
-    auto open = [&](Step& s) __attribute__((always_inline)) -> bool {
-        const int piece = s.task / a.cache.n_kv_heads;
-        while (piece >= total) {  // (tasks come in order: the window only moves on)
-            c0 += 64;
-            if (c0 >= a.batch) return false;
-            before = total;
-            len = own_len(a, c0 + lane);
-            upto = wave_scan(own_pieces(len, log2));
-            total = before + __builtin_amdgcn_readlane(upto, 63);
-        }
-        const int at = (int)__builtin_ctzll(__ballot(before + upto > piece));
-        s.L = __builtin_amdgcn_readlane(len, at);
-        s.b = c0 + at;
-        s.h = s.task - piece * a.cache.n_kv_heads;
-        const int k = piece - before - (__builtin_amdgcn_readlane(upto, at) - own_pieces(s.L, log2));
-        s.key = k << log2;
-        s.end = (int)min((int64_t)s.L, ((int64_t)k + 1) << log2);
-        return true;
-    };
-    Step now, next;
-    int n = 0;
-    now.task = task_at(0);
-    if (!open(now)) return;
-    next = now;
-    Staged<D, E4M3, 1, 1, true, false> staged;
-    staged.load(a, now.b, now.h, now.key, now.end, lane);
-    Rows<D> r;
-    int pos = -1;
-    bool opening = true, more = true;
-    do {
-        if (opening) {
-            rows_clear(r);
-            r.limit = now.L;
-            const u32x4* const q = reinterpret_cast<const u32x4*>(a.q + ((size_t)now.b * H_q + now.h * a.group + (col < a.group ? col : 0)) * D);
+    }
+    template <int I>
+    __device__ __forceinline__ void load() {
+        if (at[I].there) Staged<D, E4M3, 1, true>::load(staged[I], a, at[I].b, at[I].h, at[I].key, at[I].L, lane);
+    }
+    template <int I>
+    __device__ __forceinline__ void step() {
+        const Step now = at[I];
+        const int H_q = a.cache.n_kv_heads * a.group;
+        if (now.opens) {
+            const u32x4* const from = reinterpret_cast<const u32x4*>(a.q + ((size_t)now.b * H_q + now.h * a.group + (m < a.group ? m : 0)) * D);
 #pragma unroll
-            for (int s = 0; s < D / 16; ++s) r.q[s] = q[2 * s + (lane >> 5)];
-            pos = row_of(now.b);
-        }
-        next.key += kOwnKeys;
-        const bool closing = next.key >= next.end;
-        if (closing) {
-            next.task = task_at(++n);
-            more = open(next);
+            for (int s = 0; s < D / 32; ++s) q[s] = from[4 * s + g];
+#pragma unroll
+            for (int t = 0; t < D / 16; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+            top = -INFINITY;
+            sum = 0.f;
         }
         asm volatile("" ::: "memory");  // (the tile before is read)
-        staged.store(lk, lv, lane);
-        if (more) staged.load(a, next.b, next.h, next.key, next.end, lane);
-        if (pos >= now.key && pos < now.key + kOwnKeys && pos < now.end) {
+        Staged<D, E4M3, 1, true>::store(staged[I], lk, lv, lane);
+        forward();
+        at[I] = ahead;
+        load<I>();
+        if (now.pos >= now.key && now.pos < now.key + kOwnKeys && now.pos < now.L) {
             lds_done();
-            put_row<D, E4M3>(a, now.b, now.h, pos - now.key, lk, lv);
+            put_row<D, E4M3>(a, now.b, now.h, now.pos - now.key, lk, lv);
         }
         lds_done();
-        attend<D, 1>(r, lk, lv, now.key, a.scale_log2);
-        if (closing) {
-            const float l = pair_sum32(r.l);
-            if (col < a.group) store_partial<D>(a, r, l, part0 + (size_t)now.task * a.group + col);
+        float s[8];
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int st = 0; st < D / 32; ++st) acc = mfma16(lk[(16 * kt + m) * NCH + k_chunk<D>(m, 4 * st + g)], q[st], acc);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[4 * kt + i] = 16 * kt + i < now.L - now.key - 4 * g ? acc[i] : -INFINITY;
         }
-        now = next;
-        opening = closing;
-    } while (more);
-}
+        float mx = s[0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) mx = fmaxf(mx, s[i]);
+        const float cand = fmaxf(top, pair_max32(pair_max16(mx)) * a.scale_log2);
+        if (__ballot(cand > top + kRescaleSlack) != 0) {
+            const float corr = cand == -INFINITY ? 1.f : fast_exp2(top - cand);
+            top = cand;
+            sum *= corr;
+#pragma unroll
+            for (int t = 0; t < D / 16; ++t) o[t] *= corr;
+        }
+        const float shift = softmax_base(top);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            s[i] = fast_exp2(fmaf(s[i], a.scale_log2, -shift));
+            sum += s[i];
+        }
+        // The lane's keys of both products: 4 g .. 4 g + 3 of either half.
+        const u32x4 p = {pack_bf16x2(s[0], s[1]), pack_bf16x2(s[2], s[3]), pack_bf16x2(s[4], s[5]), pack_bf16x2(s[6], s[7])};
+        const int key = 4 * g + (m >> 2);
+        const uint8_t* const base = reinterpret_cast<const uint8_t*>(lv) + key * (2 * D) + 8 * (m & 1);
+#pragma unroll
+        for (int t = 0; t < D / 16; ++t) {
+            const uint8_t* const v = base + 16 * v_chunk_own<D>(key, 2 * t + ((m >> 1) & 1));
+            const u32x2 v0 = lds_read_tr16(v), v1 = lds_read_tr16(v + 16 * (2 * D));
+            o[t] = mfma16(u32x4{v0[0], v0[1], v1[0], v1[1]}, p, o[t]);
+        }
+        if (now.closes) {
+            const float l = pair_sum32(pair_sum16(sum));
+            const size_t row = part0 + ((size_t)now.b * a.cache.n_kv_heads + now.h + wave) * a.group + m;
+            if (m < a.group) {
+#pragma unroll
+                for (int t = 0; t < D / 16; ++t) reinterpret_cast<f32x4*>(a.part_o + row * D)[4 * t + g] = o[t];
+                if (g == 0) reinterpret_cast<float2*>(a.part_ml)[row] = make_float2(top, l);
+            }
+        }
+    }
+    __device__ __forceinline__ void run() {
+        while (at[0].there) {
+            step<0>();
+            if (!at[1].there) break;
+            step<1>();
+        }
+    }
+};
 
 // ---- the launches --------------------------------------------------------------------------------------------
 
@@ -590,8 +709,15 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_prefix_kernel(PrefixArg
     // A work-group has a part of the prefix, if there are so many, and then some of the own rows.
     const int prefix_wgs = a.pieces * a.blocks * a.cache.n_kv_heads, wgs = max(prefix_wgs, a.own_wgs), index = wide_block();
     if (index >= wgs) return;
-    if (index < prefix_wgs) prefix_task<D, E4M3, TEAM>(a, index, lds, lds_ml, lds_odd);
-    own_tasks<D, E4M3>(a, index, prefix_wgs, wgs, lds, (size_t)a.pieces * a.cache.n_kv_heads * prefix_rows(a));
+    OwnRows<D, E4M3> own(a, index, prefix_wgs, wgs, lds);
+    if (index < prefix_wgs) {
+        prefix_task<D, E4M3, TEAM>(a, index, lds, lds_ml, lds_odd, own.staged[0], [&]() __attribute__((always_inline)) { own.template load<0>(); });
+    } else {
+        own.template load<0>();
+    }
+    own.template load<1>();
+    own.append();
+    own.run();
 }
 
 // Joins a query row's partials: a work-group per row, D / 4 threads for every (256 / (D / 4))-th of them.
@@ -605,15 +731,19 @@ __global__ __launch_bounds__(kMergeThreads) void decode_prefix_merge_kernel(Pref
     const int part = threadIdx.x / E, e = threadIdx.x % E;
     const int limit = b == a.prefix_b ? 0 : a.shared != nullptr ? min(a.shared[b], a.prefix_len) : a.prefix_len;
     const int n_prefix = limit > 0 ? (limit + a.chunk - 1) / a.chunk : 0;
-    const int log2 = own_log2(a);
-    int before = 0;  // pieces of the sequences before this one
+    const int prefix_wgs = a.pieces * a.blocks * a.cache.n_kv_heads;
+    const Runs runs(a, prefix_wgs, max(prefix_wgs, a.own_wgs));
+    int before = 0;  // steps of the sequences before this one
     for (int c0 = 0; c0 < b; c0 += 64)
-        before += __builtin_amdgcn_readlane(wave_scan(c0 + lane < b ? own_pieces(own_len(a, c0 + lane), log2) : 0), 63);
-    const int n_own = own_pieces(own_len(a, b), log2), n = n_prefix + n_own;
+        before += __builtin_amdgcn_readlane(wave_scan(c0 + lane < b ? own_steps(own_len(a, c0 + lane)) : 0), 63);
+    const int steps = own_steps(own_len(a, b));
+    const int first = before * a.cache.n_kv_heads + h * steps;
+    const int first_wave = steps > 0 ? runs.wave_of(first) : 0;
+    const int n_own = steps > 0 ? runs.wave_of(first + steps - 1) - first_wave + 1 : 0, n = n_prefix + n_own;
     const size_t rows = prefix_rows(a);
     const size_t prefix_row = h * rows + (size_t)(b - (b > a.prefix_b ? 1 : 0)) * a.group + g, prefix_step = a.cache.n_kv_heads * rows;
-    const size_t own_row = (size_t)a.pieces * prefix_step + ((size_t)before * a.cache.n_kv_heads + h) * a.group + g;
-    const size_t own_step = (size_t)a.cache.n_kv_heads * a.group;
+    const size_t own_row = (size_t)a.pieces * prefix_step + ((size_t)b * a.cache.n_kv_heads + h + first_wave) * a.group + g;
+    const size_t own_step = a.group;
     float M = -INFINITY, L = 0.f;
     f32x4 O = {0.f, 0.f, 0.f, 0.f};
     for (int s = part; s < n; s += PARTS) {
@@ -674,7 +804,6 @@ void plan_prefix(PrefixArgs* a, int n_cu) {
     a->chunk = (int)std::max<int64_t>(least, (keys + least - 1) / least * least);
     a->pieces = a->prefix_len > 0 && rows > 0 ? (int)(((int64_t)a->prefix_len + a->chunk - 1) / a->chunk) : 0;
     a->own_wgs = n_cu;
-    a->own_slots = (int)std::max<int64_t>(kPrefixOwnSlots, (int64_t)a->batch * a->cache.n_kv_heads);
 }
 
 int64_t prefix_partial_rows_max(int batch, int n_kv_heads, int group, int n_cu) {
@@ -683,7 +812,8 @@ int64_t prefix_partial_rows_max(int batch, int n_kv_heads, int group, int n_cu) 
     a.group = group;
     a.cache.n_kv_heads = n_kv_heads;
     plan_prefix(&a, n_cu);
-    return most_pieces(a, n_cu) * n_kv_heads * batch * group + (int64_t)a.own_slots * group;
+    const int64_t pieces = most_pieces(a, n_cu), wgs = std::max<int64_t>(pieces * a.blocks * n_kv_heads, a.own_wgs);
+    return pieces * n_kv_heads * batch * group + ((int64_t)batch * n_kv_heads + wgs * kWaves) * group;
 }
 
 hipError_t launch_decode_prefix(int head_dim, const PrefixArgs& a, const Launch& l) {

@@ -394,14 +394,13 @@ struct PrefixArgs {
     int32_t row_tiles;          // of the prefix's work-groups: 32-row tiles that a tile of K and V serves (1, 2 or 4)
     int32_t blocks;             // work-groups along the rows, per kv head
     int32_t chunk, pieces;      // the prefix in pieces of `chunk` keys, a work-group each
-    int32_t own_wgs;            // work-groups for the sequences' own rows
-    int32_t own_slots;          // partials that own_part holds
-    float* part_o;              // prefix [pieces][H_kv][(B - 1) * group][D], then own [own_slots][group][D]
+    int32_t own_wgs;            // work-groups at least: all of them share the sequences' own rows
+    float* part_o;              // prefix [pieces][H_kv][(B - 1) * group][D], then own [B * H_kv + waves][group][D]
     float* part_ml;             // the same rows' (maximum in log2 units, sum)
     uint16_t* out;              // [B][H_q][D]
     float* lse;                 // [B][H_q] or nullptr
 };
-constexpr int kPrefixOwnSlots = 16384;  // at least; one per (sequence, kv head) where those are more
+constexpr int kPrefixOwnKeys = 32;  // of a step of own rows
 void plan_prefix(PrefixArgs* a, int n_cu);
 // Rows of part_o (and part_ml) that plan_prefix may ask for, whatever the prefix.
 int64_t prefix_partial_rows_max(int batch, int n_kv_heads, int group, int n_cu);
