@@ -31,7 +31,7 @@ typedef short i16x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-constexpr int kWaves = 8;
+constexpr int kWaves = 4;
 constexpr int kOwnKeys = kPrefixOwnKeys;
 
 __device__ __forceinline__ f32x4 mfma16(const u32x4& a, const u32x4& b, const f32x4& c) {
@@ -114,7 +114,7 @@ struct Runs {
     // Where wave w's run begins, and the wave in whose run step `at` lies.
     __device__ __forceinline__ int begin(int w) const { return w < others ? w * first : others * first + (w - others) * rest; }
     __device__ __forceinline__ int wave_of(int at) const { return at < others * first ? at / first : others + (at - others * first) / rest; }
-    static constexpr int kLateSteps = 2;  // a part of the prefix costs about this and a step for each of its rounds
+    static constexpr int kLateSteps = 6;  // a part of the prefix costs about this and a step for each of its rounds
 };
 
 // ---- one task: 32 query rows over a run of tiles -----------------------------------------------------------
@@ -237,41 +237,23 @@ struct Staged {
     }
 };
 
-// The tile of keys key0 .. in LDS, for 32 rows.
-template <int D, int NT>
+// 32 keys from key0 on, in LDS, for 32 rows.
+template <int D>
 __device__ __forceinline__ void attend(Rows<D>& r, const u32x4* lk, const u32x4* lv, int key0, float scale_log2) {
     constexpr int NCH = D / 8, STEPS = D / 16, MT = D / 32;
     const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
-    f32x16 s[NT];
+    f32x16 s;
 #pragma unroll
-    for (int kt = 0; kt < NT; ++kt)
+    for (int i = 0; i < 16; ++i) s[i] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[kt][i] = 0.f;
-    // Fragments are read a few steps before their products, and no further (sched_barrier): registers would not hold them.
-    constexpr int kAhead = 2;
-    u32x4 kf[STEPS][NT];
-    auto read_k = [&](int st) __attribute__((always_inline)) {
-#pragma unroll
-        for (int kt = 0; kt < NT; ++kt) kf[st][kt] = lk[(32 * kt + col) * NCH + k_chunk<D>(col, 2 * st + half)];
-    };
-#pragma unroll
-    for (int st = 0; st < kAhead; ++st) read_k(st);
-#pragma unroll
-    for (int st = 0; st < STEPS; ++st) {
-        if (st + kAhead < STEPS) read_k(st + kAhead);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int kt = 0; kt < NT; ++kt) s[kt] = mfma32(kf[st][kt], r.q[st], s[kt]);
-    }
-    // Keys that a row does not see (every tile: a branch around it costs more, in copies of O that registers do not hold).
+    for (int st = 0; st < STEPS; ++st) s = mfma32(lk[col * NCH + k_chunk<D>(col, 2 * st + half)], r.q[st], s);
+    // Keys that a row does not see (in every tile: a branch around it costs more, in copies of O that registers do not hold).
     float mx = -INFINITY;
 #pragma unroll
-    for (int kt = 0; kt < NT; ++kt)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            s[kt][i] = 32 * kt + 8 * (i >> 2) + (i & 3) < r.limit - key0 - 4 * half ? s[kt][i] : -INFINITY;
-            mx = fmaxf(mx, s[kt][i]);
-        }
+    for (int i = 0; i < 16; ++i) {
+        s[i] = 8 * (i >> 2) + (i & 3) < r.limit - key0 - 4 * half ? s[i] : -INFINITY;
+        mx = fmaxf(mx, s[i]);
+    }
     const float cand = fmaxf(r.m, pair_max32(mx) * scale_log2);
     if (__ballot(cand > r.m + kRescaleSlack) != 0) {
         const float corr = cand == -INFINITY ? 1.f : fast_exp2(r.m - cand);
@@ -283,38 +265,28 @@ __device__ __forceinline__ void attend(Rows<D>& r, const u32x4* lk, const u32x4*
             for (int i = 0; i < 16; ++i) r.o[t][i] *= corr;
     }
     const float shift = softmax_base(r.m);  // (no key yet: every score is -inf, and 2^-inf is 0)
-    u32x4 p[2 * NT];
+    u32x4 p[2];
 #pragma unroll
-    for (int kt = 0; kt < NT; ++kt)
+    for (int u = 0; u < 2; ++u) {
+        float e[8];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            float e[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                e[i] = fast_exp2(fmaf(s[kt][8 * u + i], scale_log2, -shift));
-                r.l += e[i];
-            }
-            p[2 * kt + u] = u32x4{pack_bf16x2(e[0], e[1]), pack_bf16x2(e[2], e[3]), pack_bf16x2(e[4], e[5]), pack_bf16x2(e[6], e[7])};
+        for (int i = 0; i < 8; ++i) {
+            e[i] = fast_exp2(fmaf(s[8 * u + i], scale_log2, -shift));
+            r.l += e[i];
         }
+        p[u] = u32x4{pack_bf16x2(e[0], e[1]), pack_bf16x2(e[2], e[3]), pack_bf16x2(e[4], e[5]), pack_bf16x2(e[6], e[7])};
+    }
     // A lane's keys of step `st`: 16 st + 4 half + 0..3 and 8 further, in the order that S^T leaves them.
     const int from = (lane & 15) >> 2;  // key of the four that the lane addresses
     const uint8_t* const base = reinterpret_cast<const uint8_t*>(lv);
-    auto value = [&](int t, int st) __attribute__((always_inline)) {
-        const int dim = 32 * t + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-        const uint8_t* const at = base + (from + 4 * half + 16 * st) * (2 * D) + 16 * v_chunk<D>(from, dim >> 3) + 8 * ((dim >> 2) & 1);
+    auto value = [&](int i) __attribute__((always_inline)) {  // tile i / 2, step i % 2
+        const int dim = 32 * (i / 2) + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+        const uint8_t* const at = base + (from + 4 * half + 16 * (i % 2)) * (2 * D) + 16 * v_chunk<D>(from, dim >> 3) + 8 * ((dim >> 2) & 1);
         const u32x2 v0 = lds_read_tr16(at), v1 = lds_read_tr16(at + 8 * (2 * D));
         return u32x4{v0[0], v0[1], v1[0], v1[1]};
     };
-    constexpr int PV = MT * 2 * NT, kAheadV = 3;
-    u32x4 vf[PV];
 #pragma unroll
-    for (int i = 0; i < kAheadV; ++i) vf[i] = value(i / (2 * NT), i % (2 * NT));
-#pragma unroll
-    for (int i = 0; i < PV; ++i) {
-        if (i + kAheadV < PV) vf[i + kAheadV] = value((i + kAheadV) / (2 * NT), (i + kAheadV) % (2 * NT));
-        __builtin_amdgcn_sched_barrier(0);
-        r.o[i / (2 * NT)] = mfma32(vf[i], p[i % (2 * NT)], r.o[i / (2 * NT)]);
-    }
+    for (int i = 0; i < 2 * MT; ++i) r.o[i / 2] = mfma32(value(i), p[i % 2], r.o[i / 2]);
 }
 
 // ---- the prefix ---------------------------------------------------------------------------------------------
@@ -355,7 +327,7 @@ __device__ __forceinline__ void add_odd(Rows<D>& r, const PrefixArgs& a, int h, 
 // TEAM waves share 32 * TEAM keys in LDS at a time, for 32 rows each; the work-group's TEAMS teams take the others of a round.
 template <int D, bool E4M3, int TEAM, typename Last>
 __device__ __forceinline__ void prefix_task(const PrefixArgs& a, int index, uint8_t* lds, float2* lds_ml, int* lds_odd, Loaded<D, E4M3>& first, Last&& last) {
-    constexpr int NT = 1, KEYS = 32 * TEAM, TEAMS = kWaves / TEAM, NCH = D / 8;
+    constexpr int KEYS = 32 * TEAM, TEAMS = kWaves / TEAM, NCH = D / 8;
     const int lane = threadIdx.x & 63, col = lane & 31, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int tile_of = wave % TEAM, team = wave / TEAM, t = threadIdx.x % (64 * TEAM);
     // kv heads in turn, so that consecutive work-groups (XCDs in turn) take one each and an L2 holds few heads' rows.
@@ -397,8 +369,7 @@ __device__ __forceinline__ void prefix_task(const PrefixArgs& a, int index, uint
         if (round + kRoundKeys >= end) last();
         if constexpr (TEAM > 1) lds_barrier();
         else lds_done();
-        for (int k = 0; k < KEYS; k += 32 * NT)
-            if (key0 + k < hi) attend<D, NT>(r, lk + k * NCH, lv + k * NCH, key0 + k, a.scale_log2);
+        for (int k = 0; k < KEYS && key0 + k < hi; k += 32) attend<D>(r, lk + k * NCH, lv + k * NCH, key0 + k, a.scale_log2);
     }
     // What is not finite reaches the rows that see it, and no others: 0 times it would be NaN in the products.
     odd = __ballot(odd) != 0;
@@ -410,14 +381,14 @@ __device__ __forceinline__ void prefix_task(const PrefixArgs& a, int index, uint
     // The teams meet in LDS, every wave's O row by row (16-byte words permuted by the row: no bank is met twice), and leave it
     // as whole rows.
     constexpr int WORDS = D / 4;
-    f32x4* const lo = reinterpret_cast<f32x4*>(lds);
+    f32x4* const lds_o = reinterpret_cast<f32x4*>(lds);
     const float l = pair_sum32(r.l);
     lds_barrier();  // (the tiles are read)
 #pragma unroll
     for (int m = 0; m < D / 32; ++m)
 #pragma unroll
         for (int i4 = 0; i4 < 4; ++i4)
-            lo[(wave * 32 + col) * WORDS + ((8 * m + 2 * i4 + (lane >> 5)) ^ (col & (WORDS - 1)))] =
+            lds_o[(wave * 32 + col) * WORDS + ((8 * m + 2 * i4 + (lane >> 5)) ^ (col & (WORDS - 1)))] =
                 f32x4{r.o[m][4 * i4], r.o[m][4 * i4 + 1], r.o[m][4 * i4 + 2], r.o[m][4 * i4 + 3]};
     if (lane < 32) lds_ml[wave * 32 + lane] = make_float2(r.m, l);
     lds_barrier();
@@ -433,16 +404,20 @@ __device__ __forceinline__ void prefix_task(const PrefixArgs& a, int index, uint
 #pragma unroll
         for (int k = 0; k < TEAMS; ++k) {
             ml[k] = lds_ml[k * TEAM * 32 + at];
-            v[k] = lo[(k * TEAM * 32 + at) * WORDS + (word ^ (at & 31 & (WORDS - 1)))];
+            v[k] = lds_o[(k * TEAM * 32 + at) * WORDS + (word ^ (at & 31 & (WORDS - 1)))];
         }
         float M = ml[0].x;
 #pragma unroll
         for (int k = 1; k < TEAMS; ++k) M = fmaxf(M, ml[k].x);
         const float base = softmax_base(M);
-        f32x4 O = {0.f, 0.f, 0.f, 0.f};
-        float L = 0.f;
+        f32x4 O = v[0];
+        float L = ml[0].y;
+        if constexpr (TEAMS > 1) {
+            O = f32x4{0.f, 0.f, 0.f, 0.f};
+            L = 0.f;
+        }
 #pragma unroll
-        for (int k = 0; k < TEAMS; ++k) {
+        for (int k = 0; k < (TEAMS > 1 ? TEAMS : 0); ++k) {
             const float f = fast_exp2(ml[k].x - base);
             L = fmaf(f, ml[k].y, L);
 #pragma unroll
@@ -803,7 +778,7 @@ void plan_prefix(PrefixArgs* a, int n_cu) {
     const int64_t most = most_pieces(*a, n_cu), keys = (a->prefix_len + most - 1) / most;
     a->chunk = (int)std::max<int64_t>(least, (keys + least - 1) / least * least);
     a->pieces = a->prefix_len > 0 && rows > 0 ? (int)(((int64_t)a->prefix_len + a->chunk - 1) / a->chunk) : 0;
-    a->own_wgs = n_cu;
+    a->own_wgs = 2 * n_cu;
 }
 
 int64_t prefix_partial_rows_max(int batch, int n_kv_heads, int group, int n_cu) {
