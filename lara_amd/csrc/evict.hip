@@ -2,14 +2,17 @@
 // the heaviest between stay, by the mass that they have; equal ones go by their index, NaN counts as less than anything.
 // The rows that stay move together, in their order, to the first `keep`.
 //
-// Selection, a work-group per (sequence, kv head): the least mass that stays is found by its bits, 11, 11 and 10 at a time
-// (masses as unsigned numbers of the same order; a histogram of the masses that share the bits found so far).  Then the rows
-// are counted by 64, which gives every row that stays its place.
+// Selection, a work-group per (sequence, kv head): masses are taken as unsigned numbers of the same order, and rows that stay
+// in any case have the greatest; the least that stays is found by its bits, 11, 11 and 10 at a time, from a histogram of those
+// that share the bits found so far.  A thread has a run of rows, so that the rows that stay in the runs before give its own
+// their places.  It is latency: 8 us for eight sequences of 8 kv heads and 8192 rows, 15 us for 64 of them.  (Rows in turn over
+// the lanes with ballots for places take 13 and 21 us: the code of a ballot per 64 rows is long, and runs once.)
 //
 // Moving, in place: row j comes from row kept[j] >= j, and kept rises, so a work-group that takes the rows in order, a batch
 // at a time, has read all that a batch's stores may overwrite once the batch itself is read; the next batch's loads may even
 // pass them.  Rows do not mix along their bytes, so a (sequence, kv head) is shared out by K and V and by columns, which
-// need nothing of each other: no work-group waits for another.  Scales and masses are one more work-group's.
+// need nothing of each other: no work-group waits for another.  Scales and masses are one more work-group's.  The memory
+// bounds it: 64 sequences of 8 kv heads, 2048 rows of 256 bytes kept of 8192, 222 us (read and written at 4.9 TB/s).
 #include "decode_common.h"
 #include "kv8_device.h"
 
@@ -17,20 +20,28 @@ namespace lara {
 namespace {
 
 constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64;
-constexpr int kSelectHeld = 16;  // masses a thread keeps in registers; those past them are read again
+constexpr int kSelectHeld = 2;  // steps of four masses that a thread keeps in registers; those past them are read again
 constexpr int kBins = 2048;
-constexpr int kMoveThreads = 256, kMoveBatch = 8;  // 16-byte words of a batch per thread
+constexpr int kMoveThreads = 512, kMoveBatch = 8;  // 16-byte words of a batch per thread
 
-// The order of masses as that of unsigned numbers: NaN below all, -0 as 0.
+// The order of masses as that of unsigned numbers from 2 to 2^32 - 2: NaN has 1, -0 is 0.
 __device__ __forceinline__ uint32_t mass_key(float x) {
     const uint32_t u = __float_as_uint(x + 0.f);
-    return x != x ? 0u : u >> 31 ? ~u : u | 0x80000000u;
+    return x != x ? 1u : u >> 31 ? ~u : u | 0x80000000u;
+}
+constexpr uint32_t kSure = 0xFFFFFFFFu;  // a row that stays whatever its mass
+
+// The sums of the waves' numbers before wave `wave`'s, lane by lane; `of` holds one per wave.
+__device__ __forceinline__ int waves_before(const int* of, int wave, int lane) {
+    const int n = lane < kSelectWaves ? of[lane] : 0;
+    return __builtin_amdgcn_readlane(wave_scan(n) - n, wave);
 }
 
-__global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictArgs a) {
+__global__ __launch_bounds__(kSelectThreads, 8) void evict_select_kernel(EvictArgs a) {
     const int unit = wide_block(), b = unit / a.cache.n_kv_heads;
     if (b >= a.batch) return;
-    const int L = clamp_len(a.lens[b], a.cache.l_max), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int L = clamp_len(a.lens[b], a.cache.l_max);
     if (unit == b * a.cache.n_kv_heads && tid == 0) a.lens_copy[b] = L;
     int32_t* const kept = a.kept + (size_t)unit * a.keep;
     if (L <= a.keep) {
@@ -38,115 +49,102 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictArgs 
         return;
     }
     const float* const mass = a.mass + (size_t)unit * a.mass_ld;
-    const int lo = a.sinks, hi = L - a.recent, need = a.keep - a.sinks - a.recent;
-    uint32_t held[kSelectHeld];
+    // A thread has one run of rows, four a step.
+    const int lo = a.sinks, hi = L - a.recent, per = 4 * ((L + 4 * kSelectThreads - 1) / (4 * kSelectThreads)), first = tid * per;
+    struct Step {
+        uint32_t k[4];
+    };
+    auto step = [&](int t) __attribute__((always_inline)) {
+        float m[4] = {0.f, 0.f, 0.f, 0.f};
+        if (t + 4 <= L) {
+            __builtin_memcpy(m, mass + t, 16);
+        } else {
 #pragma unroll
-    for (int c = 0; c < kSelectHeld; ++c) {
-        const int t = c * kSelectThreads + tid;
-        held[c] = t >= lo && t < hi ? mass_key(mass[t]) : 0u;
-    }
-    // Calls f(row, key) for the thread's rows of the middle.
+            for (int i = 0; i < 4; ++i)
+                if (t + i < L) m[i] = mass[t + i];
+        }
+        Step s;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s.k[i] = t + i >= L ? 0u : t + i < lo || t + i >= hi ? kSure : mass_key(m[i]);
+        return s;
+    };
+    Step held[kSelectHeld];
+#pragma unroll
+    for (int c = 0; c < kSelectHeld; ++c)
+        if (4 * c < per) held[c] = step(first + 4 * c);
+    // Calls f(row, key) for the thread's rows in their order; rows past L have the key 0, which nothing else has.
     auto each = [&](auto&& f) __attribute__((always_inline)) {
 #pragma unroll
-        for (int c = 0; c < kSelectHeld; ++c) {
-            const int t = c * kSelectThreads + tid;
-            if (t >= lo && t < hi) f(held[c]);
+        for (int c = 0; c < kSelectHeld; ++c)
+            if (4 * c < per)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) f(first + 4 * c + i, held[c].k[i]);
+#pragma unroll 1
+        for (int c = kSelectHeld; 4 * c < per; ++c) {
+            const Step s = step(first + 4 * c);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f(first + 4 * c + i, s.k[i]);
         }
-        for (int t = kSelectHeld * kSelectThreads + tid; t < hi; t += kSelectThreads)
-            if (t >= lo) f(mass_key(mass[t]));
     };
-    __shared__ int hist[kBins];
-    __shared__ int wave_total[kSelectWaves];
-    __shared__ int found[2];
-    uint32_t least = 0xFFFFFFFFu, mask = 0;  // (no mass has that key: nothing of the middle stays where need is 0)
-    int quota = 0;                           // rows that stay of those with the least key
-    if (need > 0) {
-        least = 0;
-        quota = need;
+    __shared__ int hist[3][kBins];
+    __shared__ int total[2][kSelectWaves];
+    __shared__ int found[3][2];
+    for (int i = tid; i < 3 * kBins; i += kSelectThreads) hist[0][i] = 0;
+    __syncthreads();
+    uint32_t least = 0, mask = 0;
+    int quota = a.keep;  // rows that stay of those whose key begins with the bits of `least`: in the end, is it
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
+        each([&](int, uint32_t k) __attribute__((always_inline)) {
+            if (k != 0 && (k & mask) == least) atomicAdd(&hist[pass][(k >> shift) & (bins - 1)], 1);
+        });
+        __syncthreads();
+        // Bins from the top, kPer a thread; the one in which the count reaches the quota is it.
+        constexpr int kPer = kBins / kSelectThreads;
+        const int top = bins - 1 - kPer * tid;
+        int n[kPer], sum = 0;
 #pragma unroll
-        for (int pass = 0; pass < 3; ++pass) {
-            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
-            for (int i = tid; i < kBins; i += kSelectThreads) hist[i] = 0;
-            __syncthreads();
-            each([&](uint32_t k) {
-                if ((k & mask) == least) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1);
-            });
-            __syncthreads();
-            // Bins from the top: thread t has two of them; the one in which the count reaches the quota is it.
-            const int top = bins - 1 - 2 * tid;
-            const int n0 = top >= 0 ? hist[top] : 0, n1 = top >= 1 ? hist[top - 1] : 0;
-            const int upto = wave_scan(n0 + n1);
-            if (lane == 63) wave_total[wave] = upto;
-            __syncthreads();
-            int before = upto - n0 - n1;
-            for (int w = 0; w < wave; ++w) before += wave_total[w];
-            if (before < quota && quota <= before + n0 + n1) {
-                const bool second = quota > before + n0;
-                found[0] = top - (second ? 1 : 0);
-                found[1] = quota - before - (second ? n0 : 0);
+        for (int i = 0; i < kPer; ++i) sum += n[i] = top >= i ? hist[pass][top - i] : 0;
+        const int upto = wave_scan(sum);
+        if (lane == 63) total[pass & 1][wave] = upto;
+        __syncthreads();
+        int before = waves_before(total[pass & 1], wave, lane) + upto - sum;
+        if (before < quota && quota <= before + sum) {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                if (before < quota && quota <= before + n[i]) {
+                    found[pass][0] = top - i;
+                    found[pass][1] = quota - before;
+                }
+                before += n[i];
             }
-            __syncthreads();
-            least |= (uint32_t)found[0] << shift;
-            mask |= (uint32_t)(bins - 1) << shift;
-            quota = found[1];
         }
+        __syncthreads();
+        least |= (uint32_t)found[pass][0] << shift;
+        mask |= (uint32_t)(bins - 1) << shift;
+        quota = found[pass][1];
     }
-    // Places, 256 runs of 64 rows at a time: run 16 c + w is wave w's.
-    __shared__ int sure_of[16 * kSelectWaves], even_of[16 * kSelectWaves];
-    __shared__ int scan_total[4][2];
-    int sure_before = 0, even_before = 0;
-    for (int t0 = 0; t0 < L; t0 += 16 * kSelectThreads) {
-        unsigned long long sure[16], even[16];
-#pragma unroll
-        for (int c = 0; c < 16; ++c) {
-            const int t = t0 + c * kSelectThreads + tid;
-            const bool middle = t >= lo && t < hi;
-            const uint32_t k = t0 == 0 ? held[c] : middle ? mass_key(mass[t]) : 0u;
-            sure[c] = __ballot(t < L && (!middle || k > least));
-            even[c] = __ballot(middle && k == least);
-            if (lane == 0) {
-                sure_of[c * kSelectWaves + wave] = __popcll(sure[c]);
-                even_of[c * kSelectWaves + wave] = __popcll(even[c]);
-            }
-        }
-        __syncthreads();
-        int s = 0, e = 0, s_upto = 0, e_upto = 0;
-        if (wave < 4) {
-            s = sure_of[tid];
-            e = even_of[tid];
-            s_upto = wave_scan(s);
-            e_upto = wave_scan(e);
-            if (lane == 63) {
-                scan_total[wave][0] = s_upto;
-                scan_total[wave][1] = e_upto;
-            }
-        }
-        __syncthreads();
-        if (wave < 4) {
-            int sb = sure_before, eb = even_before;
-            for (int w = 0; w < wave; ++w) {
-                sb += scan_total[w][0];
-                eb += scan_total[w][1];
-            }
-            sure_of[tid] = sb + s_upto - s;
-            even_of[tid] = eb + e_upto - e;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int c = 0; c < 16; ++c) {
-            const int t = t0 + c * kSelectThreads + tid;
-            const unsigned long long below = (1ull << lane) - 1;
-            const int e_rank = even_of[c * kSelectWaves + wave] + __popcll(even[c] & below);
-            const int place = sure_of[c * kSelectWaves + wave] + __popcll(sure[c] & below) + min(e_rank, quota);
-            const bool stays = (sure[c] >> lane & 1) != 0 || ((even[c] >> lane & 1) != 0 && e_rank < quota);
-            if (stays) kept[place] = t;
-        }
-        for (int w = 0; w < 4; ++w) {
-            sure_before += scan_total[w][0];
-            even_before += scan_total[w][1];
-        }
-        __syncthreads();  // the counts are read
+    // Places: what stays of the waves, lanes and rows before.
+    int more = 0, even = 0;
+    each([&](int, uint32_t k) __attribute__((always_inline)) {
+        more += k > least ? 1 : 0;
+        even += k == least ? 1 : 0;
+    });
+    const int more_upto = wave_scan(more), even_upto = wave_scan(even);
+    __shared__ int more_of[kSelectWaves], even_of[kSelectWaves];
+    if (lane == 63) {
+        more_of[wave] = more_upto;
+        even_of[wave] = even_upto;
     }
+    __syncthreads();
+    more = waves_before(more_of, wave, lane) + more_upto - more;
+    even = waves_before(even_of, wave, lane) + even_upto - even;
+    each([&](int t, uint32_t k) __attribute__((always_inline)) {
+        if (k > least || (k == least && even < quota)) kept[more + min(even, quota)] = t;
+        more += k > least ? 1 : 0;
+        even += k == least ? 1 : 0;
+    });
 }
 
 // What a value held in registers needs before a barrier that stands for "read by all".
@@ -268,12 +266,14 @@ hipError_t launch_evict_select(const EvictArgs& a, const Launch& l) {
     return launch_kernel(evict_select_kernel, wide_grid((int64_t)a.batch * a.cache.n_kv_heads), dim3(kSelectThreads), l, a);
 }
 
-// Rows go in slices of a whole line (128 bytes), or finer ones down to 32 bytes while those do not make two work-groups a CU.
+// Rows go in slices of a whole line (128 bytes), or in halves of one while those do not make a work-group for every second
+// CU.  With 8 kv heads of 8192 rows of 256 bytes, 2048 kept: whole lines against halves 29 -> 38 us for eight sequences,
+// 14.8 -> 20.3 for four, but 12.7 -> 10.8 for two.
 hipError_t launch_evict_move(const EvictArgs& from, int n_cu, const Launch& l) {
     EvictArgs a = from;
     const int64_t units = (int64_t)a.batch * a.cache.n_kv_heads;
     a.slices = a.row_bytes > 128 ? a.row_bytes / 128 : 1;
-    while (a.row_bytes / a.slices > 32 && units * 2 * a.slices < 2 * n_cu) a.slices *= 2;
+    while (a.row_bytes / a.slices > 64 && units * 2 * a.slices < n_cu / 2) a.slices *= 2;
     const int64_t wgs = units * (2 * a.slices + 1);
     if (wgs > INT32_MAX) return hipErrorInvalidValue;
     return launch_kernel(evict_move_kernel, wide_grid(wgs), dim3(kMoveThreads), l, a);
