@@ -100,10 +100,16 @@ __device__ __forceinline__ int own_steps(int len) { return (len + kOwnKeys - 1) 
 // kv head) u in the run of wave w leaves its partial in slot u + w (one of the two rises from part to part).
 struct Runs {
     int others, first, rest;
-    __device__ __forceinline__ Runs(const PrefixArgs& a, int prefix_wgs, int wgs) {
+    int before;  // steps of a kv head's sequences before `b`
+    __device__ __forceinline__ Runs(const PrefixArgs& a, int prefix_wgs, int wgs, int b) {
         const int lane = threadIdx.x & 63;
         int steps = 0;
-        for (int c0 = 0; c0 < a.batch; c0 += 64) steps += __builtin_amdgcn_readlane(wave_scan(own_steps(own_len(a, c0 + lane))), 63);
+        before = 0;
+        for (int c0 = 0; c0 < a.batch; c0 += 64) {
+            const int of = own_steps(own_len(a, c0 + lane)), upto = wave_scan(of);
+            if (b >= c0 && b < c0 + 64) before = steps + __builtin_amdgcn_readlane(upto - of, b - c0);
+            steps += __builtin_amdgcn_readlane(upto, 63);
+        }
         steps *= a.cache.n_kv_heads;
         others = (wgs - prefix_wgs) * kWaves;
         const int waves = wgs * kWaves;
@@ -510,7 +516,7 @@ struct OwnRows {
         part0 = (size_t)a.pieces * a.cache.n_kv_heads * prefix_rows(a);
         n_waves = wgs * kWaves;
         me = in_wg * wgs + index;
-        const Runs runs(a, prefix_wgs, wgs);
+        const Runs runs(a, prefix_wgs, wgs, 0);
         wave = index >= prefix_wgs ? in_wg * (wgs - prefix_wgs) + index - prefix_wgs : runs.others + in_wg * prefix_wgs + index;
         const int begin = runs.begin(wave);
         left = wave < runs.others ? runs.first : runs.rest;
@@ -695,64 +701,98 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_prefix_kernel(PrefixArg
     own.run();
 }
 
-// Joins a query row's partials: a work-group per row, D / 4 threads for every (256 / (D / 4))-th of them.
-constexpr int kMergeThreads = 256;
-template <int D>
-__global__ __launch_bounds__(kMergeThreads) void decode_prefix_merge_kernel(PrefixArgs a) {
-    constexpr int E = D / 4, PARTS = kMergeThreads / E;
-    const int block = wide_block(), H_q = a.cache.n_kv_heads * a.group, b = block / H_q, head = block - b * H_q;
-    if (b >= a.batch) return;
-    const int h = head / a.group, g = head - h * a.group, lane = threadIdx.x & 63;
-    const int part = threadIdx.x / E, e = threadIdx.x % E;
+// Joins a query row's partials with log-sum-exp weights: WAVES waves per row, which take them in turn.  A wave has the weights
+// of 64 partials in its lanes, and D / 4 lanes for each of the partials that it adds at a time.
+constexpr int kMergeWaves = 4;
+template <int D, int WAVES>
+__global__ __launch_bounds__(kMergeWaves * 64) void decode_prefix_merge_kernel(PrefixArgs a) {
+    constexpr int E = D / 4, AT_ONCE = 64 / E, DEEP = 4;
+    const int in_wg = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, e = lane % E, of = lane / E;
+    const int H_q = a.cache.n_kv_heads * a.group, out_row = wide_block() * (kMergeWaves / WAVES) + in_wg / WAVES, b = out_row / H_q;
+    if (b >= a.batch) return;  // (with WAVES > 1 for the whole work-group)
+    const int head = out_row - b * H_q, h = head / a.group, g = head - h * a.group;
     const int limit = b == a.prefix_b ? 0 : a.shared != nullptr ? min(a.shared[b], a.prefix_len) : a.prefix_len;
     const int n_prefix = limit > 0 ? (limit + a.chunk - 1) / a.chunk : 0;
     const int prefix_wgs = a.pieces * a.blocks * a.cache.n_kv_heads;
-    const Runs runs(a, prefix_wgs, max(prefix_wgs, a.own_wgs));
-    int before = 0;  // steps of the sequences before this one
-    for (int c0 = 0; c0 < b; c0 += 64)
-        before += __builtin_amdgcn_readlane(wave_scan(c0 + lane < b ? own_steps(own_len(a, c0 + lane)) : 0), 63);
+    const Runs runs(a, prefix_wgs, max(prefix_wgs, a.own_wgs), b);
     const int steps = own_steps(own_len(a, b));
-    const int first = before * a.cache.n_kv_heads + h * steps;
+    const int first = runs.before * a.cache.n_kv_heads + h * steps;
     const int first_wave = steps > 0 ? runs.wave_of(first) : 0;
     const int n_own = steps > 0 ? runs.wave_of(first + steps - 1) - first_wave + 1 : 0, n = n_prefix + n_own;
     const size_t rows = prefix_rows(a);
     const size_t prefix_row = h * rows + (size_t)(b - (b > a.prefix_b ? 1 : 0)) * a.group + g, prefix_step = a.cache.n_kv_heads * rows;
     const size_t own_row = (size_t)a.pieces * prefix_step + ((size_t)b * a.cache.n_kv_heads + h + first_wave) * a.group + g;
     const size_t own_step = a.group;
+    auto row_of = [&](int s) __attribute__((always_inline)) {
+        return s < n_prefix ? prefix_row + s * prefix_step : own_row + (s - n_prefix) * own_step;
+    };
     float M = -INFINITY, L = 0.f;
     f32x4 O = {0.f, 0.f, 0.f, 0.f};
-    for (int s = part; s < n; s += PARTS) {
-        const size_t row = s < n_prefix ? prefix_row + s * prefix_step : own_row + (s - n_prefix) * own_step;
-        const float2 ml = reinterpret_cast<const float2*>(a.part_ml)[row];
-        const f32x4 o = reinterpret_cast<const f32x4*>(a.part_o + row * D)[e];
-        const float m = fmaxf(M, ml.x), base = softmax_base(m);
-        const float keep = fast_exp2(M - base), f = fast_exp2(ml.x - base);
-        L = fmaf(f, ml.y, L * keep);
+    const int mine = n > in_wg % WAVES ? (n - in_wg % WAVES + WAVES - 1) / WAVES : 0;  // partials of this wave
+    for (int c0 = 0; c0 < mine; c0 += 64) {
+        const int here = min(mine - c0, 64);
+        float2 ml = make_float2(-INFINITY, 0.f);
+        if (lane < here) ml = reinterpret_cast<const float2*>(a.part_ml)[row_of((c0 + lane) * WAVES + in_wg % WAVES)];
+        float top = ml.x;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) O[i] = fmaf(f, o[i], O[i] * keep);
-        M = m;
+        for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
+        top = fmaxf(M, top);
+        const float base = softmax_base(top), keep = fast_exp2(M - base), f = fast_exp2(ml.x - base);
+        float l = f * ml.y;
+#pragma unroll
+        for (int x = 1; x < 64; x *= 2) l += __shfl_xor(l, x);
+        L = fmaf(L, keep, l);
+        O *= keep;
+        M = top;
+        for (int i0 = 0; i0 < here; i0 += AT_ONCE * DEEP) {
+            f32x4 o[DEEP];
+#pragma unroll
+            for (int d = 0; d < DEEP; ++d) {
+                const int i = i0 + d * AT_ONCE + of;
+                o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (i < here) o[d] = reinterpret_cast<const f32x4*>(a.part_o + row_of((c0 + i) * WAVES + in_wg % WAVES) * D)[e];
+            }
+#pragma unroll
+            for (int d = 0; d < DEEP; ++d) {
+                const float weight = __shfl(f, (i0 + d * AT_ONCE + of) & 63);
+#pragma unroll
+                for (int x = 0; x < 4; ++x) O[x] = fmaf(weight, o[d][x], O[x]);
+            }
+        }
     }
-    __shared__ __attribute__((aligned(16))) float lds_o[PARTS * D];
-    __shared__ float2 lds_ml[PARTS];
-    reinterpret_cast<f32x4*>(lds_o)[part * E + e] = O;
-    if (e == 0) lds_ml[part] = make_float2(M, L);
-    __syncthreads();
-    for (int d = threadIdx.x; d < D; d += kMergeThreads) {
+#pragma unroll
+    for (int x = E; x < 64; x *= 2)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) O[k] += __shfl_xor(O[k], x);
+    if constexpr (WAVES > 1) {
+        __shared__ __attribute__((aligned(16))) f32x4 lds_o[WAVES][E];
+        __shared__ float2 lds_ml[WAVES];
+        if (of == 0) lds_o[in_wg][e] = O;
+        if (lane == 0) lds_ml[in_wg] = make_float2(M, L);
+        __syncthreads();
+        if (in_wg != 0) return;
         float top = -INFINITY;
 #pragma unroll
-        for (int p = 0; p < PARTS; ++p) top = fmaxf(top, lds_ml[p].x);
+        for (int w = 0; w < WAVES; ++w) top = fmaxf(top, lds_ml[w].x);
         const float base = softmax_base(top);
-        float o = 0.f, l = 0.f;
+        O = f32x4{0.f, 0.f, 0.f, 0.f};
+        L = 0.f;
+        M = top;
 #pragma unroll
-        for (int p = 0; p < PARTS; ++p) {
-            const float f = fast_exp2(lds_ml[p].x - base);
-            o = fmaf(f, lds_o[p * D + d], o);
-            l = fmaf(f, lds_ml[p].y, l);
+        for (int w = 0; w < WAVES; ++w) {
+            const float f = fast_exp2(lds_ml[w].x - base);
+            L = fmaf(f, lds_ml[w].y, L);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) O[k] = fmaf(f, lds_o[w][e][k], O[k]);
         }
-        const size_t row = (size_t)b * H_q + head;
-        a.out[row * D + d] = f32_to_bf16_rne(softmax_out(o, l));
-        if (d == 0 && a.lse != nullptr) a.lse[row] = softmax_lse(top, l);
     }
+    if (of == 0) {
+        u32x2 w;
+        w[0] = pack_bf16x2(softmax_out(O[0], L), softmax_out(O[1], L));
+        w[1] = pack_bf16x2(softmax_out(O[2], L), softmax_out(O[3], L));
+        reinterpret_cast<u32x2*>(a.out + (size_t)out_row * D)[e] = w;
+    }
+    if (lane == 0 && a.lse != nullptr) a.lse[out_row] = softmax_lse(M, L);
 }
 
 template <int D, bool E4M3>
@@ -799,11 +839,19 @@ hipError_t launch_decode_prefix(int head_dim, const PrefixArgs& a, const Launch&
     return hipErrorInvalidValue;
 }
 
-hipError_t launch_decode_prefix_merge(int head_dim, const PrefixArgs& a, const Launch& l) {
-    const int64_t wgs = (int64_t)a.batch * a.cache.n_kv_heads * a.group;
-    if (wgs > INT32_MAX) return hipErrorInvalidValue;
-    if (head_dim == 128) return launch_kernel(decode_prefix_merge_kernel<128>, wide_grid(wgs), dim3(kMergeThreads), l, a);
-    if (head_dim == 64) return launch_kernel(decode_prefix_merge_kernel<64>, wide_grid(wgs), dim3(kMergeThreads), l, a);
+hipError_t launch_decode_prefix_merge(int head_dim, const PrefixArgs& a, int n_cu, const Launch& l) {
+    const int64_t rows = (int64_t)a.batch * a.cache.n_kv_heads * a.group;
+    if (rows > INT32_MAX - kMergeWaves) return hipErrorInvalidValue;
+    const bool many = rows >= (int64_t)kMergeWaves * n_cu;
+    const dim3 grid = wide_grid(many ? (rows + kMergeWaves - 1) / kMergeWaves : rows), block(kMergeWaves * 64);
+    if (head_dim == 128) {
+        if (many) return launch_kernel(decode_prefix_merge_kernel<128, 1>, grid, block, l, a);
+        return launch_kernel(decode_prefix_merge_kernel<128, kMergeWaves>, grid, block, l, a);
+    }
+    if (head_dim == 64) {
+        if (many) return launch_kernel(decode_prefix_merge_kernel<64, 1>, grid, block, l, a);
+        return launch_kernel(decode_prefix_merge_kernel<64, kMergeWaves>, grid, block, l, a);
+    }
     return hipErrorInvalidValue;
 }
 

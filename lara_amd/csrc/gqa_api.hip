@@ -2536,7 +2536,7 @@ int run_decode_prefix(gqa_ctx* c, const void* q, const void* k_rows, const void*
     if (rc != GQA_OK) return rc;
     if (c->paged) c->pages.touch(prefix_b);
     HIP_TRY(launch_decode_prefix(c->cfg.head_dim, a, timed(c, GQA_TIMER_DECODE, s)));
-    HIP_TRY(launch_decode_prefix_merge(c->cfg.head_dim, a, timed(c, GQA_TIMER_COMBINE, s)));
+    HIP_TRY(launch_decode_prefix_merge(c->cfg.head_dim, a, c->n_cu, timed(c, GQA_TIMER_COMBINE, s)));
     return GQA_OK;
 }
 

@@ -405,7 +405,7 @@ void plan_prefix(PrefixArgs* a, int n_cu);
 // Rows of part_o (and part_ml) that plan_prefix may ask for, whatever the prefix.
 int64_t prefix_partial_rows_max(int batch, int n_kv_heads, int group, int n_cu);
 hipError_t launch_decode_prefix(int head_dim, const PrefixArgs& a, const Launch& l);
-hipError_t launch_decode_prefix_merge(int head_dim, const PrefixArgs& a, const Launch& l);
+hipError_t launch_decode_prefix_merge(int head_dim, const PrefixArgs& a, int n_cu, const Launch& l);
 
 // Accumulated attention weight of cache rows (mass.hip).
 struct MassArgs {
