@@ -8,10 +8,12 @@
 // p, the sums and the mass are fp32.  A row whose lse is not finite (it has no keys, or a NaN among its scores) adds nothing.
 //
 // One row of every sequence: a wave loads 64 keys, whose 16-byte chunks are operand B as they lie (the order of the dims in
-// the sum is free), and the group's query heads are the 16 rows of operand A, so nothing passes through LDS.
+// the sum is free), and the group's query heads are the 16 rows of operand A, so nothing passes through LDS.  K bounds it: 137
+// us for 64 sequences of 4000 .. 8192 keys of 8 kv heads of 128 (6.0 TB/s).
 // A block of query rows: a wave keeps 32 or 64 keys as operand B and the rows stream through LDS for the work-group's four
 // waves, 32 at a time; rows are shared out over several work-groups where the keys alone do not fill the GPU, and their
-// sums meet in a second launch, in a fixed order.
+// sums meet in a second launch, in a fixed order.  Exponentials beside the products bound it: 23 us for 2048 causal rows of 32
+// heads of 128 over 8 kv heads (740 TFLOP/s), 5.7 for the last 64 rows behind 8192 keys.
 #include "decode_common.h"
 #include "kv8_device.h"
 
@@ -26,6 +28,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kMassWaves = 4;
 constexpr int kRowTiles = 1;  // of a stage
+constexpr int kMassWgs = 32;  // work-groups a CU, of a step
 
 __device__ __forceinline__ f32x4 mfma16(const u32x4& a, const u32x4& b, const f32x4& c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
@@ -56,8 +59,8 @@ __device__ __forceinline__ float add_far(float own, float far) {
     return own + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(far), 0x128, 0xF, 0xF, true));  // row_ror:8
 }
 
-// One row of every sequence.  A work-group: `chunk` keys (a multiple of 256) of one (sequence, kv head), rounds of 64 for
-// its waves in turn.
+// One row of every sequence.  A work-group: pieces part, part + parts .. of `chunk` keys (a multiple of 256) of one (sequence,
+// kv head), rounds of 64 for its waves in turn.
 // Rows are loaded by whole lines: lane (m, g) has the 16-byte chunk 4 (m / 8) + g of a line of key m % 8, so an instruction
 // covers 8 lines.  A column of operand B is then half of a key's line, and is multiplied with both halves' dims of Q; of the
 // two products lanes below 8 keep the first's and add what the lanes above have of theirs.  (16 keys an instruction, half a
@@ -73,15 +76,13 @@ __global__ __launch_bounds__(kMassWaves * 64) void mass_step_kernel(MassArgs a) 
     const int m = lane & 15, g = lane >> 4;
     const bool low = m < 8;
     // Pieces go slowest: consecutive work-groups (XCDs in turn) take different sequences and heads, and not always the same
-    // piece, of which the later ones are few where lengths differ (64 sequences of 4000 .. 8192 keys: 156 -> 126 us).
+    // piece, of which the later ones are few where lengths differ (64 sequences of 4000 .. 8192 keys: 156 -> 137 us).
     const uint32_t block = wide_block(), units = (uint32_t)a.batch * a.cache.n_kv_heads;
     const int part = block / units, unit = block - part * units;
     const int b = unit / a.cache.n_kv_heads, h = unit - b * a.cache.n_kv_heads;
     if (part >= a.parts) return;
     const int L = clamp_len(a.lens[b], a.cache.l_max);
-    const int64_t begin = (int64_t)part * a.chunk;
-    if (begin >= L) return;
-    const int end = begin + a.chunk < L ? (int)(begin + a.chunk) : L;
+    if ((int64_t)part * a.chunk >= L) return;
     const int H_q = a.cache.n_kv_heads * a.group;
 
     // Load i: rows of eight x = i / lines, line i % lines (or 16 rows i, whole).
@@ -103,8 +104,13 @@ __global__ __launch_bounds__(kMassWaves * 64) void mass_step_kernel(MassArgs a) 
     u32x4 k[LOADS];
     float scale[4];
     bool mapped = false;
-    int key0 = (int)begin + 64 * wave;
-    if (key0 < end) load(key0, k, scale, &mapped);
+    int64_t at = (int64_t)part * a.chunk + 64 * wave;
+    // The wave's next 64 keys: of the piece, or of the next one.
+    auto behind = [&](int64_t key) __attribute__((always_inline)) {
+        key += 64 * kMassWaves;
+        return ((key - 64 * wave) & (a.chunk - 1)) != 0 ? key : key + (int64_t)(a.parts - 1) * a.chunk;
+    };
+    if (at < L) load((int)at, k, scale, &mapped);
 
     // Operand A for step s: the dims that lane (m, g) of the keys holds there, head m.  Chunk c of a row is 16 bytes.
     u32x4 q[STEPS];
@@ -123,7 +129,7 @@ __global__ __launch_bounds__(kMassWaves * 64) void mass_step_kernel(MassArgs a) 
         if constexpr (E4M3) return codes_to_bf16x8(w[2 * part_of], w[2 * part_of + 1]);
         else return w;
     };
-    for (; key0 < end; key0 += 64 * kMassWaves) {
+    for (int64_t next; at < L; at = next) {
         float sum = 0.f;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {  // 16 keys
@@ -154,14 +160,17 @@ __global__ __launch_bounds__(kMassWaves * 64) void mass_step_kernel(MassArgs a) 
             if constexpr (E4M3) c *= scale[t];
             float p = 0.f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) p += fast_exp2(fmaf(mapped ? s[i] : 0.f, c, -shift[i]));
+            for (int i = 0; i < 4; ++i) {  // (a row that adds nothing may have scores of NaN)
+                const float e = fast_exp2(fmaf(mapped ? s[i] : 0.f, c, -shift[i]));
+                p += shift[i] < INFINITY ? e : 0.f;
+            }
             p = pair_sum32(pair_sum16(p));
             sum = g == t ? p : sum;
         }
-        const int key = key0 + lane;
-        const int next = key0 + 64 * kMassWaves;
-        if (next < end) load(next, k, scale, &mapped);
-        if (key < end) mass[key] = a.decay == 0.f ? sum : fmaf(a.decay, mass[key], sum);
+        const int key = (int)at + lane;
+        next = behind(at);
+        if (next < L) load((int)next, k, scale, &mapped);
+        if (key < L) mass[key] = a.decay == 0.f ? sum : fmaf(a.decay, mass[key], sum);
     }
 }
 
@@ -183,6 +192,8 @@ __global__ __launch_bounds__(kMassWaves * 64, 2) void mass_block_kernel(MassArgs
 
     __shared__ __attribute__((aligned(16))) u32x4 rows_in[2][ROWS * NCH];
     __shared__ __attribute__((aligned(16))) float shifts[2][ROWS];
+    __shared__ int silent[2];  // whether some row of the stage adds nothing
+    static_assert(ROWS <= 64, "silent is wave 0's");
 
     // Operand B: lane l keeps dims 16 s + 8 (l / 32) .. of key l % 32 of each tile.
     u32x4 k[KT][STEPS];
@@ -240,7 +251,7 @@ __global__ __launch_bounds__(kMassWaves * 64, 2) void mass_block_kernel(MassArgs
 #pragma unroll
     for (int t = 0; t < KT; ++t) sum[t] = 0.f;
     const int64_t sees = (int64_t)a.kv_pos_base + key0 - a.q_pos_base;  // the least query row that sees the wave's first key
-    const int first_row = (int)(sees < -(1 << 30) ? -(1 << 30) : sees) + col;
+    const int first_row = !a.causal ? -(1 << 30) : (int)(sees < -(1 << 30) ? -(1 << 30) : sees) + col;
     int st = next_seen(part), at = 0;
     if (st < stages) load(st);
     for (; st < stages; at ^= 1) {
@@ -249,7 +260,11 @@ __global__ __launch_bounds__(kMassWaves * 64, 2) void mass_block_kernel(MassArgs
             const int slot = i * THREADS + threadIdx.x, r = slot / NCH, c = slot % NCH;
             rows_in[at][r * NCH + (c ^ (NCH == 16 ? r & 15 : (r >> 1) & 7))] = in[i];
         }
-        if (threadIdx.x < ROWS) shifts[at][threadIdx.x] = row_shift(in_lse);
+        if (threadIdx.x < ROWS) {
+            const float shift = row_shift(in_lse);
+            shifts[at][threadIdx.x] = shift;
+            silent[at] = __ballot(shift == INFINITY) != 0;
+        }
         const int next = next_seen(st + a.parts);
         if (next < stages) load(next);
         __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the stage is written; the loads stay in flight
@@ -259,6 +274,7 @@ __global__ __launch_bounds__(kMassWaves * 64, 2) void mass_block_kernel(MassArgs
         const int i0 = ROWS * st % a.q_len;
         const bool several = i0 + ROWS > a.q_len;
         const bool mask = a.causal && (several || i0 < sees + KEYS - 1);
+        const int silence = silent[at];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             f32x16 acc[KT];
@@ -280,6 +296,7 @@ __global__ __launch_bounds__(kMassWaves * 64, 2) void mass_block_kernel(MassArgs
                     for (int i = 0; i < 4; ++i) {
                         int row = i0 + 32 * rt + 8 * i4 + 4 * half + i;
                         if (masked && several) row %= a.q_len;
+                        if (masked) row = shift[i] == INFINITY ? INT_MIN : row;  // (it adds nothing, whatever its scores)
 #pragma unroll
                         for (int kt = 0; kt < KT; ++kt) {
                             const float p = fast_exp2(fmaf(acc[kt][4 * i4 + i], scale[kt], -shift[i]));
@@ -288,7 +305,7 @@ __global__ __launch_bounds__(kMassWaves * 64, 2) void mass_block_kernel(MassArgs
                     }
                 }
             };
-            if (mask) add(std::true_type{});
+            if (((mask ? 1 : 0) | __builtin_amdgcn_readfirstlane(silence)) != 0) add(std::true_type{});
             else add(std::false_type{});
         }
         st = next;
@@ -320,12 +337,14 @@ __global__ __launch_bounds__(256) void mass_sum_kernel(MassArgs a) {
 
 }  // namespace
 
-// Work-groups of a step: pieces of 512 keys, or 256 while those do not make four work-groups a CU.
+// Work-groups of a step: pieces of 512 keys, or 256 while those do not make four work-groups a CU; 32 work-groups a CU at most,
+// which take the pieces in turn, so that a context's capacity does not cost what it does not hold (64 sequences of
+// 1000 keys in contexts of 131072, 8 kv heads: 78 -> 24.5 us).
 hipError_t launch_mass_step(int head_dim, MassArgs a, int n_cu, const Launch& l) {
     const int64_t units = (int64_t)a.batch * a.cache.n_kv_heads;
     a.chunk = 512;
     while (a.chunk > 256 && units * ((a.cache.l_max + a.chunk - 1) / a.chunk) < 4 * n_cu) a.chunk /= 2;
-    a.parts = (a.cache.l_max + a.chunk - 1) / a.chunk;
+    a.parts = (int)std::min<int64_t>(((int64_t)a.cache.l_max + a.chunk - 1) / a.chunk, std::max<int64_t>(1, kMassWgs * n_cu / units));
     const int64_t wgs = units * a.parts;
     if (wgs > INT32_MAX) return hipErrorInvalidValue;
     const dim3 grid = wide_grid(wgs), block(kMassWaves * 64);

@@ -270,3 +270,49 @@ def test_evict_rows_of_unmapped_pages():
                 assert np.array_equal(t[h, :n], rows[at[:n]])
                 assert np.array_equal(t[h, n:], k[b, h, n:t.shape[1]])
     assert np.array_equal(new_lens, [100, 100])
+
+
+@pytest.mark.parametrize("kv_format", ["bf16", "e4m3"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_rows_whose_scores_are_nan_add_nothing(kv_format, d):
+    """A key of NaN makes the lse of the rows that see it NaN: they add nothing, to any key; the others add what they do."""
+    rng = np.random.default_rng(31)
+    hq, hkv, L, n = 8, 2, 300, 40
+    k, v = bf16_normal(rng, (2, hkv, L, d)), bf16_normal(rng, (2, hkv, L, d))
+    k[1, 0, 280] = 0x7FC0
+    q, qs = bf16_normal(rng, (hq, n, d)), bf16_normal(rng, (2, hq, d))
+    qs[0, 3] = 0x7FC0  # a query head of NaN
+    with AttentionAccelerator(batch=2, n_q_heads=hq, n_kv_heads=hkv, head_dim=d, max_seq_len=L, max_q_len=n, kv_format=kv_format) as acc:
+        for b in range(2):
+            acc.load_kv(k[b], v[b], b=b)
+        mass = torch.zeros((2, hkv, L), device="cuda")
+        lens = dev(np.array([L, L], np.int32))
+        lse = np.full((2, hq), 3.0, np.float32)
+        lse[0, 3] = lse[1, :4] = np.nan
+        qd, ld = dev(qs), dev(lse)
+        torch.cuda.synchronize()
+        acc.attention_mass_step_device(qd.data_ptr(), lens.data_ptr(), ld.data_ptr(), mass.data_ptr())
+        torch.cuda.synchronize()
+        got = mass.cpu().numpy()
+        for b in range(2):
+            kk, l64 = stored(k[b], kv_format), lse[b].astype(np.float64)[:, None]
+            kk[np.isnan(kk)] = 0.0
+            qq = f64(qs[b])[:, None]
+            qq[np.isnan(qq)] = 0.0
+            new = lo.mass(qq, kk, l64, acc.scale)
+            assert np.all(np.abs(got[b] - new) <= bound(new, qq, kk, l64, acc.scale, 0.0, 1.0))
+            assert b == 0 or not got[1, 0].any()
+        # a block: the last 40 rows; the 20 from key 280 on see it
+        for causal in (True, False):
+            lse = np.full((hq, n), 2.0, np.float32)
+            lse[:4, 20 if causal else 0:] = np.nan
+            m, qd, ld = torch.zeros_like(mass), dev(q), dev(lse)
+            torch.cuda.synchronize()
+            acc.attention_mass_device(qd.data_ptr(), n, L, ld.data_ptr(), m.data_ptr(), b=1, q_pos_base=L - n, causal=causal)
+            torch.cuda.synchronize()
+            got = m[1].cpu().numpy()
+            seen = np.arange(L) <= L - n + np.arange(n)[:, None] if causal else None
+            kk, l64 = stored(k[1], kv_format), lse.astype(np.float64)
+            kk[np.isnan(kk)] = 0.0
+            new = lo.mass(f64(q), kk, l64, acc.scale, seen)
+            assert np.all(np.abs(got - new) <= bound(new, f64(q), kk, l64, acc.scale, 0.0, 1.0))
