@@ -278,3 +278,26 @@ def test_refusals():
             batch.acc.decode_prefix_device(batch.dev[0].data_ptr(), 2, 64, i32.data_ptr(), o.data_ptr(), k_rows_ptr=batch.dev[1].data_ptr())
         assert rc(shared=None, lse=None) == 0
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("B,prefix_b", [(1, 0), (6, 0), (6, 2), (70, 33)])
+def test_any_sequence_can_hold_the_prefix(B, prefix_b):
+    """The first, one in the middle, one behind a window of 32 rows; the only one, which has its own rows alone."""
+    rng = np.random.default_rng(B + prefix_b)
+    hq, hkv, d, n = 8, 2, 64, 150
+    lens = rng.integers(0, 40, B).astype(np.int32)
+    lens[prefix_b] = 170
+    with AttentionAccelerator(batch=B, n_q_heads=hq, n_kv_heads=hkv, head_dim=d, max_seq_len=200, max_q_len=1) as acc:
+        k, v = (bf16_normal(rng, (B, hkv, 200, d)) for _ in range(2))
+        for b in range(B):
+            acc.load_kv(k[b], v[b], b=b)
+        q = bf16_normal(rng, (B, hq, d))
+        qd, ln = dev(q), dev(lens)
+        o, lse = torch.zeros((B, hq, d), dtype=torch.int16, device="cuda"), torch.zeros((B, hq), device="cuda")
+        torch.cuda.synchronize()
+        acc.decode_prefix_device(qd.data_ptr(), prefix_b, n, ln.data_ptr(), o.data_ptr(), lse_ptr=lse.data_ptr())
+        torch.cuda.synchronize()
+        for b in range(B):
+            p = 0 if b == prefix_b else n
+            kk, vv = (np.concatenate((f64(t[prefix_b][:, :p]), f64(t[b][:, :lens[b]])), 1) for t in (k, v))
+            near(words(o)[b], lse.cpu().numpy()[b], f64(q[b]), kk, vv, acc.scale)
