@@ -426,7 +426,8 @@ struct MassPlan {
     int32_t parts;
 };
 constexpr int kMassMaxParts = 64;
-constexpr int kMassSums = 4 * 256;  // floats of part_sums per CU: 4 work-groups a CU of at most 256 keys
+constexpr int kMassBlockWgs = 3;               // work-groups a CU that share out the rows of a block
+constexpr int kMassSums = kMassBlockWgs * 256;  // floats of part_sums per CU: so many work-groups, of at most 256 keys
 MassPlan plan_mass_block(int group, int n_kv_heads, int q_len, int kv_len, int n_cu);
 hipError_t launch_mass_step(int head_dim, MassArgs a, int n_cu, const Launch& l);
 hipError_t launch_mass_block(int head_dim, const MassArgs& a, int key_tiles, const Launch& l);

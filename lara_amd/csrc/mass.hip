@@ -12,8 +12,8 @@
 // us for 64 sequences of 4000 .. 8192 keys of 8 kv heads of 128 (6.0 TB/s).
 // A block of query rows: a wave keeps 32 or 64 keys as operand B and the rows stream through LDS for the work-group's four
 // waves, 32 at a time; rows are shared out over several work-groups where the keys alone do not fill the GPU, and their
-// sums meet in a second launch, in a fixed order.  Exponentials beside the products bound it: 23 us for 2048 causal rows of 32
-// heads of 128 over 8 kv heads (740 TFLOP/s), 5.7 for the last 64 rows behind 8192 keys.
+// sums meet in a second launch, in a fixed order.  Exponentials beside the products bound it: 22 us for 2048 causal rows of 32
+// heads of 128 over 8 kv heads (785 TFLOP/s), 5.7 for the last 64 rows behind 8192 keys.
 #include "decode_common.h"
 #include "kv8_device.h"
 
@@ -365,8 +365,8 @@ MassPlan plan_mass_block(int group, int n_kv_heads, int q_len, int kv_len, int n
     // keys, 8 stages, 5.5 us against 7.1)
     if (of_keys >= n_cu && tiles <= 16)
         p.parts = 1;
-    else
-        p.parts = (int)std::max<int64_t>(1, std::min<int64_t>({4 * n_cu / of_keys, (int64_t)tiles / 4, kMassMaxParts}));
+    else  // (a prompt of 2048 rows and 32 heads: 3 work-groups a CU, which all are on it at once, 21.9 us; 4 of them 22.9)
+        p.parts = (int)std::max<int64_t>(1, std::min<int64_t>({kMassBlockWgs * n_cu / of_keys, (int64_t)tiles / 4, kMassMaxParts}));
     return p;
 }
 
