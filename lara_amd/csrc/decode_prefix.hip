@@ -88,6 +88,7 @@ __device__ __forceinline__ void lds_barrier() {
 }
 
 constexpr int kRoundKeys = 32 * kWaves;  // keys that a work-group has in LDS
+constexpr int kWholeWaves = 8, kWholeValues = 1024 * 128;  // the most K values of a (sequence, kv head) for one work-group
 
 // LDS of a work-group: K and V of 32 keys for each wave.
 template <int D>
@@ -486,10 +487,76 @@ __device__ __forceinline__ void put_row(const PrefixArgs& a, int b, int h, int k
     else lk[key * LANES + k_chunk<D>(key, at)] = w;
 }
 
-// A wave's run of own rows as one stream of steps of 32 keys.  Two steps' loads are under way while one is worked on:
-// of the group's up to 16 heads as columns,
+// Up to 16 heads of a group over some keys, 32 at a time, as columns:
 //   S^T [16 keys x 16] = K . Q^T, O^T [D x 16] += V^T [D x 32 keys] . P^T by v_mfma_f32_16x16x32_bf16,
-// which needs half the registers of 32 rows.
+// which needs half the registers of 32 rows.  Lane (m, g) has head m.
+template <int D>
+struct Heads {
+    static constexpr int NCH = D / 8;
+    u32x4 q[D / 32];
+    f32x4 o[D / 16];
+    float top, sum;
+
+    __device__ __forceinline__ void open(const PrefixArgs& a, int b, int h, int m, int g) {
+        const u32x4* const from =
+            reinterpret_cast<const u32x4*>(a.q + ((size_t)b * a.cache.n_kv_heads * a.group + h * a.group + (m < a.group ? m : 0)) * D);
+#pragma unroll
+        for (int s = 0; s < D / 32; ++s) q[s] = from[4 * s + g];
+#pragma unroll
+        for (int t = 0; t < D / 16; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        top = -INFINITY;
+        sum = 0.f;
+    }
+    // The first `left` of the 32 keys in LDS.
+    __device__ __forceinline__ void step(const u32x4* lk, const u32x4* lv, int left, float scale_log2, int m, int g) {
+        float s[8];
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int st = 0; st < D / 32; ++st) acc = mfma16(lk[(16 * kt + m) * NCH + k_chunk<D>(m, 4 * st + g)], q[st], acc);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[4 * kt + i] = 16 * kt + i < left - 4 * g ? acc[i] : -INFINITY;
+        }
+        float mx = s[0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) mx = fmaxf(mx, s[i]);
+        const float cand = fmaxf(top, pair_max32(pair_max16(mx)) * scale_log2);
+        if (__ballot(cand > top + kRescaleSlack) != 0) {
+            const float corr = cand == -INFINITY ? 1.f : fast_exp2(top - cand);
+            top = cand;
+            sum *= corr;
+#pragma unroll
+            for (int t = 0; t < D / 16; ++t) o[t] *= corr;
+        }
+        const float shift = softmax_base(top);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            s[i] = fast_exp2(fmaf(s[i], scale_log2, -shift));
+            sum += s[i];
+        }
+        // The lane's keys of both products: 4 g .. 4 g + 3 of either half.
+        const u32x4 p = {pack_bf16x2(s[0], s[1]), pack_bf16x2(s[2], s[3]), pack_bf16x2(s[4], s[5]), pack_bf16x2(s[6], s[7])};
+        const int key = 4 * g + (m >> 2);
+        const uint8_t* const base = reinterpret_cast<const uint8_t*>(lv) + key * (2 * D) + 8 * (m & 1);
+#pragma unroll
+        for (int t = 0; t < D / 16; ++t) {
+            const uint8_t* const v = base + 16 * v_chunk_own<D>(key, 2 * t + ((m >> 1) & 1));
+            const u32x2 v0 = lds_read_tr16(v), v1 = lds_read_tr16(v + 16 * (2 * D));
+            o[t] = mfma16(u32x4{v0[0], v0[1], v1[0], v1[1]}, p, o[t]);
+        }
+    }
+    __device__ __forceinline__ float l() const { return pair_sum32(pair_sum16(sum)); }
+};
+
+// The appended row of sequence b: inside the cache, and not among the prefix's rows, which others are reading; or -1.
+__device__ __forceinline__ int appended_row(const PrefixArgs& a, int b) {
+    if (a.k_new == nullptr || b >= a.batch) return -1;
+    const int pos = a.positions[b];
+    return pos < 0 || pos >= a.cache.l_max || (b == a.prefix_b && pos < a.prefix_len) ? -1 : pos;
+}
+
+// A wave's run of own rows as one stream of steps of 32 keys.  Two steps' loads are under way while one is worked on.
 template <int D, bool E4M3>
 struct OwnRows {
     static constexpr int NCH = D / 8;
@@ -506,10 +573,7 @@ struct OwnRows {
     int c0 = -64, len = 0, pos_of = -1;
     Step at[2], ahead;  // what the two loads under way are for; the last one issued
     Loaded<D, E4M3> staged[2];
-    // The part's rows: lane (m, g) has head m.
-    u32x4 q[D / 32];
-    f32x4 o[D / 16];
-    float top, sum;
+    Heads<D> rows;  // the part's
 
     __device__ __forceinline__ OwnRows(const PrefixArgs& args, int index, int prefix_wgs, int wgs, uint8_t* lds) : a(args) {
         lane = threadIdx.x & 63;
@@ -531,16 +595,10 @@ struct OwnRows {
         forward();
         at[1] = ahead;
     }
-    // The appended row of sequence b: inside the cache, and not among the prefix's rows, which others are reading.
-    __device__ __forceinline__ int row_of(int b) const {
-        if (a.k_new == nullptr || b >= a.batch) return -1;
-        const int pos = a.positions[b];
-        return pos < 0 || pos >= a.cache.l_max || (b == a.prefix_b && pos < a.prefix_len) ? -1 : pos;
-    }
     __device__ __forceinline__ void window(int from) {
         c0 = from;
         len = own_len(a, c0 + lane);
-        pos_of = row_of(c0 + lane);
+        pos_of = appended_row(a, c0 + lane);
     }
     __device__ __forceinline__ void take(int i) {  // the window's i-th sequence
         ahead.b = c0 + i;
@@ -599,7 +657,7 @@ struct OwnRows {
     __device__ __forceinline__ void append() const {
         if (a.k_new == nullptr) return;
         for (int u = me; u < a.batch * a.cache.n_kv_heads; u += n_waves) {
-            const int b = u / a.cache.n_kv_heads, pos = row_of(b);
+            const int b = u / a.cache.n_kv_heads, pos = appended_row(a, b);
             if (pos >= 0) append_row<D, E4M3>(a, b, u - b * a.cache.n_kv_heads, pos);
         }
     }
@@ -610,16 +668,7 @@ struct OwnRows {
     template <int I>
     __device__ __forceinline__ void step() {
         const Step now = at[I];
-        const int H_q = a.cache.n_kv_heads * a.group;
-        if (now.opens) {
-            const u32x4* const from = reinterpret_cast<const u32x4*>(a.q + ((size_t)now.b * H_q + now.h * a.group + (m < a.group ? m : 0)) * D);
-#pragma unroll
-            for (int s = 0; s < D / 32; ++s) q[s] = from[4 * s + g];
-#pragma unroll
-            for (int t = 0; t < D / 16; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-            top = -INFINITY;
-            sum = 0.f;
-        }
+        if (now.opens) rows.open(a, now.b, now.h, m, g);
         asm volatile("" ::: "memory");  // (the tile before is read)
         Staged<D, E4M3, 1, true>::store(staged[I], lk, lv, lane);
         forward();
@@ -630,49 +679,14 @@ struct OwnRows {
             put_row<D, E4M3>(a, now.b, now.h, now.pos - now.key, lk, lv);
         }
         lds_done();
-        float s[8];
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
-            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int st = 0; st < D / 32; ++st) acc = mfma16(lk[(16 * kt + m) * NCH + k_chunk<D>(m, 4 * st + g)], q[st], acc);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[4 * kt + i] = 16 * kt + i < now.L - now.key - 4 * g ? acc[i] : -INFINITY;
-        }
-        float mx = s[0];
-#pragma unroll
-        for (int i = 1; i < 8; ++i) mx = fmaxf(mx, s[i]);
-        const float cand = fmaxf(top, pair_max32(pair_max16(mx)) * a.scale_log2);
-        if (__ballot(cand > top + kRescaleSlack) != 0) {
-            const float corr = cand == -INFINITY ? 1.f : fast_exp2(top - cand);
-            top = cand;
-            sum *= corr;
-#pragma unroll
-            for (int t = 0; t < D / 16; ++t) o[t] *= corr;
-        }
-        const float shift = softmax_base(top);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            s[i] = fast_exp2(fmaf(s[i], a.scale_log2, -shift));
-            sum += s[i];
-        }
-        // The lane's keys of both products: 4 g .. 4 g + 3 of either half.
-        const u32x4 p = {pack_bf16x2(s[0], s[1]), pack_bf16x2(s[2], s[3]), pack_bf16x2(s[4], s[5]), pack_bf16x2(s[6], s[7])};
-        const int key = 4 * g + (m >> 2);
-        const uint8_t* const base = reinterpret_cast<const uint8_t*>(lv) + key * (2 * D) + 8 * (m & 1);
-#pragma unroll
-        for (int t = 0; t < D / 16; ++t) {
-            const uint8_t* const v = base + 16 * v_chunk_own<D>(key, 2 * t + ((m >> 1) & 1));
-            const u32x2 v0 = lds_read_tr16(v), v1 = lds_read_tr16(v + 16 * (2 * D));
-            o[t] = mfma16(u32x4{v0[0], v0[1], v1[0], v1[1]}, p, o[t]);
-        }
+        rows.step(lk, lv, now.L - now.key, a.scale_log2, m, g);
         if (now.closes) {
-            const float l = pair_sum32(pair_sum16(sum));
+            const float l = rows.l();
             const size_t row = part0 + ((size_t)now.b * a.cache.n_kv_heads + now.h + wave) * a.group + m;
             if (m < a.group) {
 #pragma unroll
-                for (int t = 0; t < D / 16; ++t) reinterpret_cast<f32x4*>(a.part_o + row * D)[4 * t + g] = o[t];
-                if (g == 0) reinterpret_cast<float2*>(a.part_ml)[row] = make_float2(top, l);
+                for (int t = 0; t < D / 16; ++t) reinterpret_cast<f32x4*>(a.part_o + row * D)[4 * t + g] = rows.o[t];
+                if (g == 0) reinterpret_cast<float2*>(a.part_ml)[row] = make_float2(rows.top, l);
             }
         }
     }
@@ -704,6 +718,86 @@ __global__ __launch_bounds__(kWaves * 64, 2) void decode_prefix_kernel(PrefixArg
     own.template load<1>();
     own.append();
     own.run();
+}
+
+// Short prefixes and contexts, few sequences: a work-group per (sequence, kv head) takes all of its keys, the prefix's first,
+// wave by wave in steps of 32, and its waves meet in LDS.  No partials and one launch; the prefix is read once a sequence.
+template <int D, bool E4M3>
+__global__ __launch_bounds__(kWholeWaves * 64, 2) void decode_prefix_whole_kernel(PrefixArgs a) {
+    constexpr int NCH = D / 8, WORDS = D / 4;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kWholeWaves * 2 * kOwnKeys * D * 2];
+    __shared__ float2 lds_ml[kWholeWaves * 16];
+    const int unit = wide_block(), b = unit / a.cache.n_kv_heads, h = unit - b * a.cache.n_kv_heads;
+    if (b >= a.batch) return;
+    const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int L = own_len(a, b), pos = appended_row(a, b);
+    const int shared = b == a.prefix_b ? 0 : a.shared != nullptr ? max(min(a.shared[b], a.prefix_len), 0) : a.prefix_len;
+    const int n_prefix = own_steps(shared), n = n_prefix + own_steps(L);
+    u32x4* const lk = reinterpret_cast<u32x4*>(lds) + (size_t)wave * 2 * kOwnKeys * NCH;
+    u32x4* const lv = lk + kOwnKeys * NCH;
+    using Tile = Staged<D, E4M3, 1, true>;
+    Loaded<D, E4M3> staged[2];
+    auto load = [&](Loaded<D, E4M3>& x, int s) __attribute__((always_inline)) {
+        if (s >= n) return;
+        const bool own = s >= n_prefix;
+        Tile::load(x, a, own ? b : a.prefix_b, h, kOwnKeys * (own ? s - n_prefix : s), own ? L : shared, lane);
+    };
+    load(staged[0], wave);
+    load(staged[1], wave + kWholeWaves);
+    Heads<D> rows;
+    rows.open(a, b, h, m, g);
+    auto step = [&](Loaded<D, E4M3>& x, int s) __attribute__((always_inline)) {
+        const int key = kOwnKeys * (s >= n_prefix ? s - n_prefix : s), left = (s >= n_prefix ? L : shared) - key;
+        asm volatile("" ::: "memory");  // (the tile before is read)
+        Tile::store(x, lk, lv, lane);
+        load(x, s + 2 * kWholeWaves);
+        if (s >= n_prefix && pos >= key && pos < key + kOwnKeys && pos < L) {
+            lds_done();
+            put_row<D, E4M3>(a, b, h, pos - key, lk, lv);
+        }
+        lds_done();
+        rows.step(lk, lv, left, a.scale_log2, m, g);
+    };
+    for (int s = wave; s < n; s += 2 * kWholeWaves) {
+        step(staged[0], s);
+        if (s + kWholeWaves >= n) break;
+        step(staged[1], s + kWholeWaves);
+    }
+    if (wave == 0 && pos >= 0) append_row<D, E4M3>(a, b, h, pos);
+    // The waves meet: [wave][head] rows of O.
+    const float l = rows.l();
+    lds_barrier();  // (the tiles are read)
+    f32x4* const lds_o = reinterpret_cast<f32x4*>(lds);
+    if (m < a.group) {
+#pragma unroll
+        for (int t = 0; t < D / 16; ++t) lds_o[(wave * 16 + m) * WORDS + ((4 * t + g) ^ m)] = rows.o[t];
+        if (g == 0) lds_ml[wave * 16 + m] = make_float2(rows.top, l);
+    }
+    lds_barrier();
+    for (int i = threadIdx.x; i < a.group * WORDS; i += kWholeWaves * 64) {
+        const int head = i / WORDS, word = i % WORDS;
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWholeWaves; ++w) top = fmaxf(top, lds_ml[w * 16 + head].x);
+        const float base = softmax_base(top);
+        f32x4 O = {0.f, 0.f, 0.f, 0.f};
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWholeWaves; ++w) {
+            const float2 ml = lds_ml[w * 16 + head];
+            const f32x4 o = lds_o[(w * 16 + head) * WORDS + (word ^ head)];
+            const float f = fast_exp2(ml.x - base);
+            sum = fmaf(f, ml.y, sum);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) O[k] = fmaf(f, o[k], O[k]);
+        }
+        const size_t row = ((size_t)b * a.cache.n_kv_heads + h) * a.group + head;
+        u32x2 w;
+        w[0] = pack_bf16x2(softmax_out(O[0], sum), softmax_out(O[1], sum));
+        w[1] = pack_bf16x2(softmax_out(O[2], sum), softmax_out(O[3], sum));
+        __builtin_memcpy(a.out + row * D + 4 * word, &w, 8);  // (2-byte aligned)
+        if (word == 0 && a.lse != nullptr) a.lse[row] = softmax_lse(top, sum);
+    }
 }
 
 // Joins a query row's partials with log-sum-exp weights: WAVES waves per row, which take them in turn.  A wave has the weights
@@ -795,7 +889,7 @@ __global__ __launch_bounds__(kMergeWaves * 64) void decode_prefix_merge_kernel(P
         u32x2 w;
         w[0] = pack_bf16x2(softmax_out(O[0], L), softmax_out(O[1], L));
         w[1] = pack_bf16x2(softmax_out(O[2], L), softmax_out(O[3], L));
-        reinterpret_cast<u32x2*>(a.out + (size_t)out_row * D)[e] = w;
+        __builtin_memcpy(a.out + (size_t)out_row * D + 4 * e, &w, 8);  // (2-byte aligned)
     }
     if (lane == 0 && a.lse != nullptr) a.lse[out_row] = softmax_lse(M, L);
 }
@@ -808,7 +902,28 @@ hipError_t launch_prefix_t(const PrefixArgs& a, const Launch& l) {
     return launch_kernel(decode_prefix_kernel<D, E4M3, 1>, grid, block, l, a);
 }
 
+template <int D, bool E4M3>
+hipError_t launch_whole_t(const PrefixArgs& a, const Launch& l) {
+    return launch_kernel(decode_prefix_whole_kernel<D, E4M3>, wide_grid((int64_t)a.batch * a.cache.n_kv_heads), dim3(kWholeWaves * 64), l, a);
+}
+
 }  // namespace
+
+// Whether a work-group per (sequence, kv head) takes all of its keys, which the context's capacity bounds (the lengths are on
+// the device): where they are few and every work-group has a CU.  us beside other launches, against pieces and a join, 32
+// query heads over 8 of 128: a sequence of 100 rows behind 100 3.5 against 6.2, eight of 300 behind 300 4.1 / 6.4, eight of 500 behind
+// 500 5.8 / 6.9 (alone 25.5 / 24.7 with the host's share), but four of 1000 behind 1000 9.4 / 7.2; 8 over 2 heads of 64,
+// 1000 behind 1000 5.0 / 6.4.
+bool prefix_whole(int head_dim, const PrefixArgs& a, int n_cu) {
+    return (int64_t)a.batch * a.cache.n_kv_heads <= n_cu && ((int64_t)a.prefix_len + a.cache.l_max) * head_dim <= kWholeValues;
+}
+
+hipError_t launch_decode_prefix_whole(int head_dim, const PrefixArgs& a, const Launch& l) {
+    const bool e4m3 = a.cache.k_scale != nullptr;
+    if (head_dim == 128) return e4m3 ? launch_whole_t<128, true>(a, l) : launch_whole_t<128, false>(a, l);
+    if (head_dim == 64) return e4m3 ? launch_whole_t<64, true>(a, l) : launch_whole_t<64, false>(a, l);
+    return hipErrorInvalidValue;
+}
 
 // Pieces of a prefix, whatever its length: with them the prefix's work-groups are about as many as CUs.
 static int64_t most_pieces(const PrefixArgs& a, int n_cu) {

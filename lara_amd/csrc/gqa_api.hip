@@ -2531,10 +2531,17 @@ int run_decode_prefix(gqa_ctx* c, const void* q, const void* k_rows, const void*
     a.scale_log2 = c->scale * (float)M_LOG2E;
     a.out = (uint16_t*)o;
     a.lse = lse;
-    plan_prefix(&a, c->n_cu);
-    const int rc = take_prefix_workspace(c, a, s);
-    if (rc != GQA_OK) return rc;
+    const bool whole = prefix_whole(c->cfg.head_dim, a, c->n_cu);
+    if (!whole) {
+        plan_prefix(&a, c->n_cu);
+        const int rc = take_prefix_workspace(c, a, s);
+        if (rc != GQA_OK) return rc;
+    }
     if (c->paged) c->pages.touch(prefix_b);
+    if (whole) {
+        HIP_TRY(launch_decode_prefix_whole(c->cfg.head_dim, a, timed(c, GQA_TIMER_DECODE, s)));
+        return GQA_OK;
+    }
     HIP_TRY(launch_decode_prefix(c->cfg.head_dim, a, timed(c, GQA_TIMER_DECODE, s)));
     HIP_TRY(launch_decode_prefix_merge(c->cfg.head_dim, a, c->n_cu, timed(c, GQA_TIMER_COMBINE, s)));
     return GQA_OK;

@@ -401,6 +401,9 @@ struct PrefixArgs {
     float* lse;                 // [B][H_q] or nullptr
 };
 constexpr int kPrefixOwnKeys = 32;  // of a step of own rows
+// One launch without partials (and without a plan), where that is sooner done.
+bool prefix_whole(int head_dim, const PrefixArgs& a, int n_cu);
+hipError_t launch_decode_prefix_whole(int head_dim, const PrefixArgs& a, const Launch& l);
 void plan_prefix(PrefixArgs* a, int n_cu);
 // Rows of part_o (and part_ml) that plan_prefix may ask for, whatever the prefix.
 int64_t prefix_partial_rows_max(int batch, int n_kv_heads, int group, int n_cu);

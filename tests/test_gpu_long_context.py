@@ -42,13 +42,14 @@ def f64(w):
 class Serving:
     """Sequences behind one system prompt, each with a budget of rows; every call on torch's current stream."""
 
-    HQ, HKV, D, L, KEEP, SINKS, RECENT = 16, 4, 128, 256, 40, 2, 8
+    HQ, HKV, D, KEEP, SINKS, RECENT = 16, 4, 128, 40, 2, 8
 
-    def __init__(self, seed, kv_format="bf16", page=None, prefix=150, prompts=(0, 1, 33, 100)):
+    def __init__(self, seed, kv_format="bf16", page=None, prefix=150, prompts=(0, 1, 33, 100), L=256):
         rng = np.random.default_rng(seed)
+        self.L = L
         self.rng, self.prefix, self.B = rng, prefix, len(prompts) + 1
         self.acc = AttentionAccelerator(batch=self.B, n_q_heads=self.HQ, n_kv_heads=self.HKV, head_dim=self.D, max_seq_len=self.L,
-                                        max_q_len=self.L, kv_format=kv_format, page_size=page)
+                                        max_q_len=256, kv_format=kv_format, page_size=page)
         for b in range(self.B if page else 0):
             self.acc.reserve(b, self.L)
         self.form = rope.form("halves", **FORM)
@@ -103,9 +104,9 @@ def same(a, b):
 
 
 @pytest.mark.parametrize("kv_format", ["bf16", "e4m3"])
-@pytest.mark.parametrize("page", [None, 64])
-def test_steps_of_a_program(kv_format, page):
-    s = Serving(1, kv_format, page)
+@pytest.mark.parametrize("page,L", [(None, 256), (64, 256), (64, 2176)])
+def test_steps_of_a_program(kv_format, page, L):
+    s = Serving(1, kv_format, page, L=L)
     with s.acc:
         s.prompt(s.B - 1, s.prefix, 0)
         pk, pv = (f64(t) for t in s.acc.read_kv(s.B - 1, 0, s.prefix))
@@ -171,10 +172,11 @@ def twins(*args, **kw):
     return a, b
 
 
+@pytest.mark.parametrize("L", [256, 2176])
 @pytest.mark.parametrize("kv_format", ["bf16", "e4m3"])
-def test_captured_steps_replay(kv_format):
+def test_captured_steps_replay(kv_format, L):
     """Two steps and an eviction in one graph, on a stream that is not the engine's; other work between the replays."""
-    a, b = twins(2, kv_format, 64)
+    a, b = twins(2, kv_format, 64, L=L)
     with a.acc, b.acc:
         for s in (a, b):  # (the first call allocates)
             s.next_token()
@@ -204,7 +206,7 @@ def test_captured_steps_replay(kv_format):
 
 
 def test_the_first_step_over_a_prefix_is_not_captured():
-    s = Serving(3)
+    s = Serving(3, L=4096)  # (short contexts need nothing allocated)
     with s.acc:
         fill(s)
         graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
@@ -225,7 +227,7 @@ def test_two_engines_at_once():
     """Steps of two engines on two streams, nothing waiting between them, and the same steps one engine after the other."""
     alone = []
     for seed in (4, 5):
-        s = Serving(seed)
+        s = Serving(seed, L=2176)
         with s.acc:
             fill(s)
             for _ in range(12):
@@ -236,7 +238,7 @@ def test_two_engines_at_once():
                 torch.cuda.synchronize()
             alone.append(s.results())
     streams = [torch.cuda.Stream(), torch.cuda.Stream()]
-    engines = [Serving(seed) for seed in (4, 5)]
+    engines = [Serving(seed, L=2176) for seed in (4, 5)]
     with engines[0].acc, engines[1].acc:
         tokens = []
         for s in engines:

@@ -41,13 +41,16 @@ def near(o, lse, q, k, v, scale):
     assert np.all(np.abs(lse - want_lse) <= 2 * exponent + 2.0**-22 * np.abs(want_lse))
 
 
+TWO_LAUNCHES = 2112  # a context of this length: prefix and own rows in pieces, joined by a second launch
+
+
 class Batch:
     """An engine whose last slot holds the prefix, and what every sequence's rows are."""
 
     def __init__(self, rng, hq, hkv, d, prefix, lens, kv_format="bf16", page=None, outliers=0.0, max_seq_len=None):
         self.B, self.prefix, self.kv_format = len(lens) + 1, prefix, kv_format
         self.lens = np.append(lens, 0).astype(np.int32)
-        L = max_seq_len or max(prefix, *lens, 1)
+        L = max_seq_len or max(prefix, *lens, TWO_LAUNCHES)
         self.acc = AttentionAccelerator(batch=self.B, n_q_heads=hq, n_kv_heads=hkv, head_dim=d, max_seq_len=L, max_q_len=1,
                                         kv_format=kv_format, page_size=page)
         rows = [*lens, prefix]
@@ -249,7 +252,7 @@ def test_unmapped_rows_are_zeros():
 
 def test_refusals():
     rng = np.random.default_rng(18)
-    batch = Batch(rng, 8, 2, 64, 64, [10, 3])
+    batch = Batch(rng, 8, 2, 64, 64, [10, 3], max_seq_len=64)
     lib, E = batch.acc._lib, _lib
     q, k, v = (ptr(t) for t in batch.dev)
     i32 = torch.zeros(8, dtype=torch.int32, device="cuda")
@@ -301,3 +304,53 @@ def test_any_sequence_can_hold_the_prefix(B, prefix_b):
             p = 0 if b == prefix_b else n
             kk, vv = (np.concatenate((f64(t[prefix_b][:, :p]), f64(t[b][:, :lens[b]])), 1) for t in (k, v))
             near(words(o)[b], lse.cpu().numpy()[b], f64(q[b]), kk, vv, acc.scale)
+
+
+@pytest.mark.parametrize("kv_format", ["bf16", "e4m3"])
+@pytest.mark.parametrize("hq,hkv,d,page", [(8, 2, 64, None), (32, 8, 128, None), (32, 2, 64, 64), (16, 8, 128, 128), (64, 8, 128, 64),
+                                           (4, 4, 64, None), (6, 2, 128, None)])
+@pytest.mark.parametrize("prefix", [0, 1, 64, 337])
+def test_short_contexts_take_one_launch(kv_format, hq, hkv, d, page, prefix):
+    """The same steps where a work-group takes all of a sequence's keys."""
+    if hq == 6 and kv_format == "bf16":
+        pytest.skip("a bf16 engine has no groups of 3")
+    rng = np.random.default_rng(hq * d + prefix + 1)
+    batch = Batch(rng, hq, hkv, d, prefix, [0, 1, 31, 32, 33, 64, 200], kv_format, page, outliers=0.02, max_seq_len=400)
+    with batch.acc:
+        shared = np.array([prefix] * 3 + [prefix // 2, 0, -3, prefix + 5, 0])
+        batch.check(*batch.run(shared, append=False), shared, append=False)
+        batch.check(*batch.run(shared), shared)
+        batch.check(*batch.run(append=False, lens=np.zeros(8, np.int32)), append=False, lens=np.zeros(8, np.int32))
+        for b in range(batch.B - 1):  # the appended row is in the cache
+            if batch.lens[b]:
+                k, v = batch.acc.read_kv(b, batch.lens[b] - 1, 1)
+                assert np.array_equal(f64(k[:, 0]), stored(batch.k_new[b], kv_format)) and np.array_equal(f64(v[:, 0]), stored(batch.v_new[b], kv_format))
+
+
+@pytest.mark.parametrize("L", [400, TWO_LAUNCHES])
+@pytest.mark.parametrize("kv_format", ["bf16", "e4m3"])
+def test_values_of_other_sequences_and_an_output_of_two_byte_alignment(kv_format, L):
+    """Infinities and NaN of the prefix behind what a sequence sees, and of rows behind own lengths; o at an odd word."""
+    rng = np.random.default_rng(19)
+    nan = 0x7FC0
+    batch = Batch(rng, 8, 2, 128, 100, [5, 40, 0], kv_format, max_seq_len=L)
+    with batch.acc:
+        shared = np.array([50, 70, 33, 0])
+        bad = np.full((2, 30, 128), nan, np.uint16)
+        batch.acc.load_kv(bad, bad, b=3, start_pos=70)
+        for b in range(3):
+            batch.acc.load_kv(bad, bad, b=b, start_pos=int(batch.lens[b]))
+        held = torch.full((batch.q.size + 8,), 3, dtype=torch.int16, device="cuda")
+        lens, sh = dev(batch.lens), dev(shared.astype(np.int32))
+        torch.cuda.synchronize()
+        for at in (0, 1, 3):
+            held.fill_(3)
+            torch.cuda.synchronize()
+            batch.acc.decode_prefix_device(batch.dev[0].data_ptr(), 3, 100, lens.data_ptr(), held.data_ptr() + 2 * at, prefix_lens_ptr=sh.data_ptr())
+            torch.cuda.synchronize()
+            o = words(held[at:at + batch.q.size]).reshape(batch.q.shape)
+            assert held[:at].eq(3).all() and held[at + batch.q.size:].eq(3).all()
+            for b in range(3):
+                k, v = (np.concatenate((stored(t[3][:, :shared[b]], kv_format), stored(t[b][:, :batch.lens[b]], kv_format)), 1) for t in (batch.k, batch.v))
+                want, want_lse, _ = so.decode(f64(batch.q[b]), k, v, batch.acc.scale)
+                near(o[b], want_lse, f64(batch.q[b]), k, v, batch.acc.scale)

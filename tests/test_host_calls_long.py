@@ -36,8 +36,8 @@ def calls_of(e):
 
 def device_of_calls(stub):
     """The calls work on their context's device whichever is current, and leave that one current."""
-    for kv8 in (True, False):
-        e = Engine(stub, kv8=kv8)
+    for kv8, room in ((True, 300), (False, 300), (True, 4096), (False, 4096)):
+        e = Engine(stub, kv8=kv8, max_seq_len=room)
         for name, *args in calls_of(e):
             e.ok(name, *args)
             log = e.log()
@@ -48,7 +48,7 @@ def device_of_calls(stub):
 
 def failures(stub):
     """No memory for the partials: the call says so, launches nothing, and others run; a failed launch is reported once."""
-    e = Engine(stub, kv8=False)
+    e = Engine(stub, kv8=False, max_seq_len=4096)  # (short contexts need no partials)
     calls = calls_of(e)
     e.stub.stub_fail_malloc_above(1 << 20)
     name, *args = calls[2]
