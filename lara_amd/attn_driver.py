@@ -1048,7 +1048,7 @@ class AttentionAccelerator:
         """One token of every sequence over the first rows of sequence ``prefix_b`` (``prefix_lens`` of them each, None:
         ``prefix_len``) and its own ``ctx_lens`` rows (device pointers; ``gqa_decode_prefix_device``); with ``k_rows``,
         ``v_rows`` and ``positions``, those rows are appended first (``gqa_decode_append_prefix_device``).  Enqueued, not
-        synchronised; the first call allocates the partials."""
+        synchronised; the first call that needs partials (not in short contexts) allocates them."""
         given = [p is not None for p in (k_rows_ptr, v_rows_ptr, positions_ptr)]
         if any(given) != all(given):
             raise ValueError("k_rows, v_rows and positions go together")

@@ -6,7 +6,7 @@
 // The prefix's keys are cut into pieces and its query rows -- those of all sequences and of a kv head's group, [b][g] --
 // into blocks of 32 * row_tiles; a work-group has a piece and a block.  Own rows are cut into pieces of a power of two keys,
 // which the waves take when that is done.  All leave fp32 partials (O, m, l), which a second launch joins with log-sum-exp
-// weights.
+// weights.  Short contexts of few sequences take one launch without partials instead (decode_prefix_whole_kernel).
 //
 // One step, for 32 query rows and 32 or 64 keys, in both:
 //   S^T [keys x 32 rows] = K . Q^T, O^T [D x 32 rows] += V^T . P^T by v_mfma_f32_32x32x16_bf16, with K and V in LDS (E4M3
