@@ -308,7 +308,7 @@ def test_any_sequence_can_hold_the_prefix(B, prefix_b):
 
 @pytest.mark.parametrize("kv_format", ["bf16", "e4m3"])
 @pytest.mark.parametrize("hq,hkv,d,page", [(8, 2, 64, None), (32, 8, 128, None), (32, 2, 64, 64), (16, 8, 128, 128), (64, 8, 128, 64),
-                                           (4, 4, 64, None), (6, 2, 128, None)])
+                                           (4, 4, 64, None), (6, 2, 128, None), (16, 1, 128, 64)])
 @pytest.mark.parametrize("prefix", [0, 1, 64, 337])
 def test_short_contexts_take_one_launch(kv_format, hq, hkv, d, page, prefix):
     """The same steps where a work-group takes all of a sequence's keys."""
