@@ -494,7 +494,7 @@ int gqa_qk_norm_rotary_step_device(gqa_ctx* ctx, const void* qkv, int64_t ld, co
  * prefix's rows and those behind for one that goes on itself).  gqa_decode_append_prefix_device appends first, as
  * gqa_decode_append_device does, one row of each sequence's own; a row below prefix_len of sequence prefix_b is not written.
  * bf16 and E4M3 caches, contiguous and paged (rows 0 .. prefix_len - 1 of prefix_b are mapped, else GQA_ERR_RANGE), groups of
- * 1 .. 16; batch * n_kv_heads * max_seq_len up to 2^35 (GQA_ERR_UNSUPPORTED above).  Error as of decode; a V row that holds an infinity or NaN reaches the sequences that see it and no others.
+ * 1 .. 16; batch * n_kv_heads * max_seq_len up to 2^35 (GQA_ERR_UNSUPPORTED above, and with KV260 numerics, as decode).  Error as of decode; a V row that holds an infinity or NaN reaches the sequences that see it and no others.
  * Two launches, or one where (prefix_len + max_seq_len) * head_dim <= 2^17 and batch * n_kv_heads is at most the number of CUs.
  * The two launches' partials are the context's: the first such call allocates them (GQA_ERR_UNSUPPORTED under a stream capture),
  * and the caller orders the calls of one context, replays of captured ones among them, as for decode. */

@@ -1,0 +1,46 @@
+"""What the long-context calls refuse beyond missing and misplaced operands, against a HIP runtime that runs nothing
+(tests/hip_stub.cpp), on the CPU.  Every scenario is a process of its own, as in test_host_calls.py.
+"""
+import subprocess
+import sys
+from pathlib import Path
+
+import pytest
+
+ROOT = Path(__file__).resolve().parents[1]
+if str(ROOT) not in sys.path:
+    sys.path.insert(0, str(ROOT))
+
+from tests.test_host_calls import DEV, OUT, Engine, kernels, stub  # noqa: E402, F401  (stub: the fixture)
+from tests.test_host_calls_long import calls_of  # noqa: E402
+
+
+def numerics_of_a_prefix(stub):
+    """Decode over a prefix is exact arithmetic alone, as decode: refused under KV260 numerics, in one launch and in two."""
+    for room in (300, 4096):
+        e = Engine(stub, kv8=False, max_seq_len=room)
+        L = e._lib
+        calls = [call for call in calls_of(e) if "prefix" in call[0]]
+        assert len(calls) == 2
+        e.ok("gqa_set_option", e.ctx, L.GQA_OPT_NUMERICS, L.GQA_NUMERICS_KV260)
+        for name, *args in calls:
+            assert e.call("gqa_decode_device", e.ctx, DEV, DEV, OUT, None, None) == L.GQA_ERR_UNSUPPORTED
+            assert e.call(name, *args) == L.GQA_ERR_UNSUPPORTED, (name, room)
+            log = e.log()
+            assert not kernels(log) and not any(line[1] == "hipMalloc" for line in log), (name, room)
+        e.ok("gqa_set_option", e.ctx, L.GQA_OPT_NUMERICS, L.GQA_NUMERICS_EXACT)
+        for name, *args in calls:
+            e.ok(name, *args)
+
+
+SCENARIOS = {f.__name__: f for f in (numerics_of_a_prefix,)}
+
+
+@pytest.mark.parametrize("name", SCENARIOS)
+def test_scenario(stub, name):  # noqa: F811
+    run = subprocess.run([sys.executable, str(Path(__file__).resolve()), str(stub), name], capture_output=True, text=True, timeout=60)
+    assert run.returncode == 0, run.stdout + run.stderr
+
+
+if __name__ == "__main__":
+    SCENARIOS[sys.argv[2]](sys.argv[1])
