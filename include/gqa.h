@@ -457,7 +457,7 @@ int gqa_qk_norm_rope_step_device(gqa_ctx* ctx, const void* qkv, int64_t ld, cons
  *   GQA_ROPE_RAMP    f_p (1 - w) + f_p / factor w, w = (p - i) / max(j - i, 0.001) held to 0 .. 1, where i = max(0,
  *                    floor(P(high))) and j = min(R - 1, ceil(P(low))), P(T) = R ln(original_len / (2 pi T)) / (2 ln base) the
  *                    index at which a pair makes T turns over original_len
- * magnitude 0 stands for 1 (RAMP: 0.1 ln(factor) + 1).  base > 1, factor >= 1, 0 < low < high, original_len >= 1 where they
+ * magnitude 0 stands for 1 (RAMP: 0.1 ln(factor) + 1); it is finite as fp32.  base > 1, factor >= 1, 0 < low < high, original_len >= 1 where they
  * are used.  Everything else as above; angles are 64-bit, in turns (of which the whole ones go before the rounding).
  * gqa_rope_frequencies: f_p [R / 2] and the magnitude (NULL: not wanted) of a form, on the host. */
 #define GQA_ROPE_PAIRS  0

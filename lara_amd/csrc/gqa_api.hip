@@ -2407,7 +2407,7 @@ int rope_frequencies(const gqa_rope& r, int head_dim, int* rotary_dim, double* f
     const int R = r.rotary_dim == 0 ? head_dim : r.rotary_dim;
     if (R < 8 || R > head_dim || R % 8 != 0 || !(r.base > 1.0) || !isfinite(r.base)) return GQA_ERR_RANGE;
     if (r.layout != GQA_ROPE_PAIRS && r.layout != GQA_ROPE_HALVES) return GQA_ERR_RANGE;
-    if (!(r.magnitude >= 0.0) || !isfinite(r.magnitude)) return GQA_ERR_RANGE;
+    if (!(r.magnitude >= 0.0) || !isfinite((float)r.magnitude)) return GQA_ERR_RANGE;  // (the kernels take it as fp32)
     const bool ends = r.scaling == GQA_ROPE_BANDS || r.scaling == GQA_ROPE_RAMP;
     if (r.scaling != GQA_ROPE_PLAIN) {
         if (r.scaling != GQA_ROPE_LINEAR && !ends) return GQA_ERR_RANGE;

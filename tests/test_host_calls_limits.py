@@ -1,6 +1,7 @@
 """What the long-context calls refuse beyond missing and misplaced operands, against a HIP runtime that runs nothing
 (tests/hip_stub.cpp), on the CPU.  Every scenario is a process of its own, as in test_host_calls.py.
 """
+import ctypes
 import subprocess
 import sys
 from pathlib import Path
@@ -33,7 +34,23 @@ def numerics_of_a_prefix(stub):
             e.ok(name, *args)
 
 
-SCENARIOS = {f.__name__: f for f in (numerics_of_a_prefix,)}
+def magnitude_of_a_rotary_form(stub):
+    """What multiplies cosine and sine is an fp32 number: one that fp32 does not hold would make every head NaN."""
+    e = Engine(stub)
+    L, top = e._lib, (2 - 2.0**-23) * 2.0**127
+    out = (ctypes.c_double * 32)()
+    for magnitude, want in ((0.0, 0), (1.25, 0), (top, 0), (2.0**128, L.GQA_ERR_RANGE), (1e300, L.GQA_ERR_RANGE), (-1.0, L.GQA_ERR_RANGE),
+                            (float("inf"), L.GQA_ERR_RANGE), (float("nan"), L.GQA_ERR_RANGE)):
+        form = ctypes.byref(L.GqaRope(layout=1, base=1e4, factor=1.0, magnitude=magnitude))
+        assert e.call("gqa_rope_frequencies", form, 64, out, None) == want, magnitude
+        for name, *args in calls_of(e):
+            if "rotary" in name:
+                args[-3] = form
+                assert e.call(name, *args) == want, (name, magnitude)
+                assert len(kernels(e.log())) == (0 if want else 1), (name, magnitude)
+
+
+SCENARIOS = {f.__name__: f for f in (numerics_of_a_prefix, magnitude_of_a_rotary_form)}
 
 
 @pytest.mark.parametrize("name", SCENARIOS)
