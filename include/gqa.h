@@ -457,8 +457,9 @@ int gqa_qk_norm_rope_step_device(gqa_ctx* ctx, const void* qkv, int64_t ld, cons
  *   GQA_ROPE_RAMP    f_p (1 - w) + f_p / factor w, w = (p - i) / max(j - i, 0.001) held to 0 .. 1, where i = max(0,
  *                    floor(P(high))) and j = min(R - 1, ceil(P(low))), P(T) = R ln(original_len / (2 pi T)) / (2 ln base) the
  *                    index at which a pair makes T turns over original_len
- * magnitude 0 stands for 1 (RAMP: 0.1 ln(factor) + 1); it is finite as fp32.  base > 1, factor >= 1, 0 < low < high, original_len >= 1 where they
- * are used.  Everything else as above; angles are 64-bit, in turns (of which the whole ones go before the rounding).
+ * magnitude 0 stands for 1 (RAMP: 0.1 ln(factor) + 1); it is finite as fp32.  base > 1, factor >= 1, 0 < low < high,
+ * original_len >= 1 where they are used.  Everything else as above; angles are 64-bit, in turns (of which the whole ones go
+ * before the rounding).
  * gqa_rope_frequencies: f_p [R / 2] and the magnitude (NULL: not wanted) of a form, on the host. */
 #define GQA_ROPE_PAIRS  0
 #define GQA_ROPE_HALVES 1
@@ -494,7 +495,9 @@ int gqa_qk_norm_rotary_step_device(gqa_ctx* ctx, const void* qkv, int64_t ld, co
  * prefix's rows and those behind for one that goes on itself).  gqa_decode_append_prefix_device appends first, as
  * gqa_decode_append_device does, one row of each sequence's own; a row below prefix_len of sequence prefix_b is not written.
  * bf16 and E4M3 caches, contiguous and paged (rows 0 .. prefix_len - 1 of prefix_b are mapped, else GQA_ERR_RANGE), groups of
- * 1 .. 16; batch * n_kv_heads * max_seq_len up to 2^35 (GQA_ERR_UNSUPPORTED above, and with KV260 numerics, as decode).  Error as of decode; a V row that holds an infinity or NaN reaches the sequences that see it and no others.
+ * 1 .. 16; batch * n_kv_heads * (max_seq_len in whole steps of 32) up to 2^35 (GQA_ERR_UNSUPPORTED above, and with KV260
+ * numerics, as decode).  Error as of decode; a V row that holds an infinity or NaN reaches the sequences that see it and no
+ * others.
  * Two launches, or one where (prefix_len + max_seq_len) * head_dim <= 2^17 and batch * n_kv_heads is at most the number of CUs.
  * The two launches' partials are the context's: the first such call allocates them (GQA_ERR_UNSUPPORTED under a stream capture),
  * and the caller orders the calls of one context, replays of captured ones among them, as for decode. */

@@ -2512,7 +2512,7 @@ int run_decode_prefix(gqa_ctx* c, const void* q, const void* k_rows, const void*
         return GQA_ERR_RANGE;
     if (c->numerics != GQA_NUMERICS_EXACT) return GQA_ERR_UNSUPPORTED;
     // (the steps of own rows are counted in 32 bits)
-    if ((double)c->cfg.batch * c->cfg.n_kv_heads * (c->cfg.max_seq_len / kPrefixOwnKeys + 1.0) > 1 << 30 ||
+    if ((double)c->cfg.batch * c->cfg.n_kv_heads * ((c->cfg.max_seq_len + kPrefixOwnKeys - 1) / kPrefixOwnKeys) > 1 << 30 ||
         (int64_t)c->cfg.batch * c->cfg.n_q_heads > INT32_MAX)
         return GQA_ERR_UNSUPPORTED;
     const DeviceScope device(c->cfg.device);

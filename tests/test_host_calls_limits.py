@@ -50,7 +50,21 @@ def magnitude_of_a_rotary_form(stub):
                 assert len(kernels(e.log())) == (0 if want else 1), (name, magnitude)
 
 
-SCENARIOS = {f.__name__: f for f in (numerics_of_a_prefix, magnitude_of_a_rotary_form)}
+def largest_batches_of_a_prefix(stub):
+    """batch * n_kv_heads * max_seq_len up to 2^35, lengths in whole steps of 32 rows; above that refused."""
+    for batch, room, want in ((1 << 10, 1 << 22, 0), (1 << 10, (1 << 22) - 31, 0), (1 << 10, (1 << 22) + 1, 0x27), ((1 << 10) + 1, 1 << 22, 0x27)):
+        # (of a paged cache: pages for one sequence each, tables for all of their rows)
+        e = Engine(stub, page=1 << 16, batch=batch, n_q_heads=8, n_kv_heads=8, max_seq_len=room, max_q_len=1)
+        assert e._lib.GQA_ERR_UNSUPPORTED == 0x27
+        for name, *args in calls_of(e):
+            if "prefix" in name:
+                args[2 if name == "gqa_decode_prefix_device" else 5] = 0
+                args[3 if name == "gqa_decode_prefix_device" else 6] = 0
+                assert e.call(name, *args) == want, (name, batch, room)
+                assert bool(kernels(e.log())) == (want == 0)
+
+
+SCENARIOS = {f.__name__: f for f in (numerics_of_a_prefix, magnitude_of_a_rotary_form, largest_batches_of_a_prefix)}
 
 
 @pytest.mark.parametrize("name", SCENARIOS)
