@@ -460,6 +460,8 @@ int gqa_qk_norm_rope_step_device(gqa_ctx* ctx, const void* qkv, int64_t ld, cons
  * magnitude 0 stands for 1 (RAMP: 0.1 ln(factor) + 1); it is finite as fp32.  base > 1, factor >= 1, 0 < low < high,
  * original_len >= 1 where they are used.  Everything else as above; angles are 64-bit, in turns (of which the whole ones go
  * before the rounding).
+ * The step writes whatever row it is given, those of a prefix that others attend (gqa_decode_prefix_device) among them: the
+ * position of a sequence that only holds one is negative, and one that goes on itself has rows from prefix_len on.
  * gqa_rope_frequencies: f_p [R / 2] and the magnitude (NULL: not wanted) of a form, on the host. */
 #define GQA_ROPE_PAIRS  0
 #define GQA_ROPE_HALVES 1
@@ -498,6 +500,8 @@ int gqa_qk_norm_rotary_step_device(gqa_ctx* ctx, const void* qkv, int64_t ld, co
  * 1 .. 16; batch * n_kv_heads * (max_seq_len in whole steps of 32) up to 2^35 (GQA_ERR_UNSUPPORTED above, and with KV260
  * numerics, as decode).  Error as of decode; a V row that holds an infinity or NaN reaches the sequences that see it and no
  * others.
+ * The prefix's rows stay where and what they are while others attend them.  Only these calls know of them: loads, appends and
+ * heads' steps write any row of prefix_b.
  * Two launches, or one where (prefix_len + max_seq_len) * head_dim <= 2^17 and batch * n_kv_heads is at most the number of CUs.
  * The two launches' partials are the context's: the first such call allocates them (GQA_ERR_UNSUPPORTED under a stream capture),
  * and the caller orders the calls of one context, replays of captured ones among them, as for decode. */

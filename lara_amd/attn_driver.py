@@ -1034,7 +1034,8 @@ class AttentionAccelerator:
     def qk_norm_rotary_step_device(self, qkv_ptr: int, ld: int, q_weight_ptr: int | None, k_weight_ptr: int | None,
                                    positions_ptr: int, q_out_ptr: int, rope: "_lib.GqaRope", *, rows_ptr: int | None = None,
                                    eps: float = RMS_NORM_EPS, stream: int | None = None) -> None:
-        """``qk_norm_rope_step_device`` with any rotary form (``gqa_qk_norm_rotary_step_device``)."""
+        """``qk_norm_rope_step_device`` with any rotary form (``gqa_qk_norm_rotary_step_device``).  It writes row ``rows[b]`` of
+        every sequence whose position is not negative: a slot that only holds a shared prefix keeps position -1."""
         self._call("gqa_qk_norm_rotary_step_device", ctypes.c_void_p(qkv_ptr), int(ld),
                    ctypes.c_void_p(q_weight_ptr) if q_weight_ptr else None,
                    ctypes.c_void_p(k_weight_ptr) if k_weight_ptr else None, float(eps), ctypes.c_void_p(positions_ptr),
