@@ -501,7 +501,7 @@ int gqa_qk_norm_rotary_step_device(gqa_ctx* ctx, const void* qkv, int64_t ld, co
  * numerics, as decode).  Error as of decode; a V row that holds an infinity or NaN reaches the sequences that see it and no
  * others.
  * The prefix's rows stay where and what they are while others attend them.  Only these calls know of them: loads, appends and
- * heads' steps write any row of prefix_b.
+ * heads' steps write any row of prefix_b, and gqa_evict_device moves its rows like any other's (see there).
  * Two launches, or one where (prefix_len + max_seq_len) * head_dim <= 2^17 and batch * n_kv_heads is at most the number of CUs.
  * The two launches' partials are the context's: the first such call allocates them (GQA_ERR_UNSUPPORTED under a stream capture),
  * and the caller orders the calls of one context, replays of captured ones among them, as for decode. */
@@ -526,6 +526,8 @@ int gqa_decode_append_prefix_device(gqa_ctx* ctx, const void* q, const void* k_r
  * least).  They move, in their order, to rows 0 .. keep - 1, in place; rows behind them keep what they hold.  sinks + recent
  * <= keep.  new_lens[b] is min(ctx_lens[b], keep); kept [B][H_kv][keep] the former rows (-1 past new_lens[b]); new_mass the
  * kept rows' mass, 0 for the rows keep .. ctx_lens[b] - 1, as mass for sequences that are not cut, and otherwise as it was.
+ * A sequence whose rows are to stay in place, such as the holder of a prefix that others attend (gqa_decode_prefix_device), is
+ * left out by a length of at most keep in the ctx_lens of this call: 0, in an array of its own where the sequence is longer.
  * new_mass may be mass and new_lens ctx_lens; no other operands overlap (GQA_ERR_RANGE).  Lengths are held to 0 ..
  * max_seq_len.  Rows keep their rotation, so positions go on counting tokens, not rows.  Paged contexts: pages stay mapped,
  * rows of unmapped ones are zeros and not written.

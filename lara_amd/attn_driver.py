@@ -1079,7 +1079,8 @@ class AttentionAccelerator:
                      new_mass_ptr: int | None = None, new_lens_ptr: int | None = None, stream: int | None = None) -> None:
         """Cuts every sequence down to its first ``sinks`` rows, its last ``recent`` ones and the heaviest between, ``keep``
         in all, for each kv head by itself (device pointers; ``gqa_evict_device``): ``kept`` [batch, H_kv, keep] gets their
-        former rows; mass and lengths are replaced in place unless given places of their own."""
+        former rows; mass and lengths are replaced in place unless given places of their own.  Nothing tells a sequence whose
+        first rows others attend (``decode_prefix_device``): it is left out by a length of 0 here, in an array of its own."""
         self._call("gqa_evict_device", ctypes.c_void_p(mass_ptr), ctypes.c_void_p(ctx_lens_ptr), int(keep), int(sinks),
                    int(recent), ctypes.c_void_p(new_mass_ptr or mass_ptr), ctypes.c_void_p(new_lens_ptr or ctx_lens_ptr),
                    ctypes.c_void_p(kept_ptr), ctypes.c_void_p(stream) if stream else None)

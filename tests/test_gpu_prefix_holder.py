@@ -17,7 +17,7 @@ pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
 
-@pytest.mark.parametrize("goes_on", [False])
+@pytest.mark.parametrize("goes_on", [False, True])
 @pytest.mark.parametrize("kv_format,page,L", [("bf16", None, 256), ("bf16", 64, 2176), ("e4m3", 64, 256), ("e4m3", None, 2176)])
 def test_the_prefix_stays_through_steps_and_evictions(kv_format, page, L, goes_on):
     s = Serving(21, kv_format, page, prefix=60, prompts=(0, 33, 45), L=L)  # (a prefix of more rows than evictions keep)

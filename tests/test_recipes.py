@@ -59,7 +59,7 @@ class Rows:
                 self.tensor(lens)[b] = keep
 
 
-@pytest.mark.parametrize("goes_on", [False])
+@pytest.mark.parametrize("goes_on", [False, True])
 def test_a_shared_prefix_stays_what_it_is(goes_on):
     """Steps and evictions as the recipe has them leave the rows that all sequences attend alone, also where the slot that
     holds them goes on itself."""
