@@ -503,6 +503,8 @@ int gqa_qk_norm_rotary_step_device(gqa_ctx* ctx, const void* qkv, int64_t ld, co
  * The prefix's rows stay where and what they are while others attend them.  Only these calls know of them: loads, appends and
  * heads' steps write any row of prefix_b, and gqa_evict_device moves its rows like any other's (see there).
  * Two launches, or one where (prefix_len + max_seq_len) * head_dim <= 2^17 and batch * n_kv_heads is at most the number of CUs.
+ * With two, own rows are shared out by the batch's steps of 32 rows, so that a sequence with more than one of them may differ by
+ * roundings with the others' lengths.
  * The two launches' partials are the context's: the first such call allocates them (GQA_ERR_UNSUPPORTED under a stream capture),
  * and the caller orders the calls of one context, replays of captured ones among them, as for decode. */
 int gqa_decode_prefix_device(gqa_ctx* ctx, const void* q, int32_t prefix_b, int32_t prefix_len, const int32_t* prefix_lens,
