@@ -27,7 +27,6 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kMassWaves = 4;
-constexpr int kRowTiles = 1;  // of a stage
 constexpr int kMassWgs = 32;  // work-groups a CU, of a step
 
 __device__ __forceinline__ f32x4 mfma16(const u32x4& a, const u32x4& b, const f32x4& c) {
@@ -174,12 +173,11 @@ __global__ __launch_bounds__(kMassWaves * 64) void mass_step_kernel(MassArgs a) 
     }
 }
 
-// A block of query rows of sequence b: the rows of a kv head's group, [group][q_len] in order, in stages of RT tiles of 32;
-// a work-group takes the stages part, part + parts, ... and KT * 32 keys a wave.  The stage is as long as it is because one
-// tile's products take a quarter of the time that the next rows are on their way from the L2.
-template <int D, bool E4M3, int KT, int RT>
+// A block of query rows of sequence b: the rows of a kv head's group, [group][q_len] in order, in stages of 32;
+// a work-group takes the stages part, part + parts, ... and KT * 32 keys a wave.
+template <int D, bool E4M3, int KT>
 __global__ __launch_bounds__(kMassWaves * 64, 2) void mass_block_kernel(MassArgs a) {
-    constexpr int NCH = D / 8, STEPS = D / 16, KEYS = 32 * KT, ROWS = 32 * RT;
+    constexpr int NCH = D / 8, STEPS = D / 16, KEYS = 32 * KT, ROWS = 32;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, half = lane >> 5;
     // kv heads in turn over the work-groups (XCDs), so that one's query rows stay in few L2s.
@@ -193,7 +191,6 @@ __global__ __launch_bounds__(kMassWaves * 64, 2) void mass_block_kernel(MassArgs
     __shared__ __attribute__((aligned(16))) u32x4 rows_in[2][ROWS * NCH];
     __shared__ __attribute__((aligned(16))) float shifts[2][ROWS];
     __shared__ int silent[2];  // whether some row of the stage adds nothing
-    static_assert(ROWS <= 64, "silent is wave 0's");
 
     // Operand B: lane l keeps dims 16 s + 8 (l / 32) .. of key l % 32 of each tile.
     u32x4 k[KT][STEPS];
@@ -234,7 +231,7 @@ __global__ __launch_bounds__(kMassWaves * 64, 2) void mass_block_kernel(MassArgs
         return st;
     };
     constexpr int THREADS = kMassWaves * 64, PER = ROWS * NCH / THREADS;  // 16-byte chunks of a stage per thread
-    static_assert(PER >= 1 && ROWS <= THREADS, "a stage is a load a thread at least");
+    static_assert(PER >= 1, "a stage is a load a thread at least");
     u32x4 in[PER];
     float in_lse = 0.f;
     auto load = [&](int st) __attribute__((always_inline)) {
@@ -275,39 +272,36 @@ __global__ __launch_bounds__(kMassWaves * 64, 2) void mass_block_kernel(MassArgs
         const bool several = i0 + ROWS > a.q_len;
         const bool mask = a.causal && (several || i0 < sees + KEYS - 1);
         const int silence = silent[at];
+        f32x16 acc[KT];
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            f32x16 acc[KT];
+        for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt)
+            for (int i = 0; i < 16; ++i) acc[kt][i] = 0.f;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) acc[kt][i] = 0.f;
+        for (int s = 0; s < STEPS; ++s) {
+            const u32x4 qa = rows_in[at][col * NCH + ((2 * s + half) ^ (NCH == 16 ? col & 15 : (col >> 1) & 7))];
 #pragma unroll
-            for (int s = 0; s < STEPS; ++s) {
-                const u32x4 qa = rows_in[at][(32 * rt + col) * NCH + ((2 * s + half) ^ (NCH == 16 ? col & 15 : (col >> 1) & 7))];
+            for (int kt = 0; kt < KT; ++kt) acc[kt] = mfma32(qa, k[kt][s], acc[kt]);
+        }
+        auto add = [&](auto masked) __attribute__((always_inline)) {
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt) acc[kt] = mfma32(qa, k[kt][s], acc[kt]);
-            }
-            auto add = [&](auto masked) __attribute__((always_inline)) {
+            for (int i4 = 0; i4 < 4; ++i4) {
+                const f32x4 shift = *reinterpret_cast<const f32x4*>(&shifts[at][8 * i4 + 4 * half]);
 #pragma unroll
-                for (int i4 = 0; i4 < 4; ++i4) {
-                    const f32x4 shift = *reinterpret_cast<const f32x4*>(&shifts[at][32 * rt + 8 * i4 + 4 * half]);
+                for (int i = 0; i < 4; ++i) {
+                    int row = i0 + 8 * i4 + 4 * half + i;
+                    if (masked && several) row %= a.q_len;
+                    if (masked) row = shift[i] == INFINITY ? INT_MIN : row;  // (it adds nothing, whatever its scores)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        int row = i0 + 32 * rt + 8 * i4 + 4 * half + i;
-                        if (masked && several) row %= a.q_len;
-                        if (masked) row = shift[i] == INFINITY ? INT_MIN : row;  // (it adds nothing, whatever its scores)
-#pragma unroll
-                        for (int kt = 0; kt < KT; ++kt) {
-                            const float p = fast_exp2(fmaf(acc[kt][4 * i4 + i], scale[kt], -shift[i]));
-                            sum[kt] += masked && row < first_row + 32 * kt ? 0.f : p;
-                        }
+                    for (int kt = 0; kt < KT; ++kt) {
+                        const float p = fast_exp2(fmaf(acc[kt][4 * i4 + i], scale[kt], -shift[i]));
+                        sum[kt] += masked && row < first_row + 32 * kt ? 0.f : p;
                     }
                 }
-            };
-            if (((mask ? 1 : 0) | __builtin_amdgcn_readfirstlane(silence)) != 0) add(std::true_type{});
-            else add(std::false_type{});
-        }
+            }
+        };
+        if (((mask ? 1 : 0) | __builtin_amdgcn_readfirstlane(silence)) != 0) add(std::true_type{});
+        else add(std::false_type{});
         st = next;
     }
 #pragma unroll
@@ -376,7 +370,7 @@ static hipError_t launch_mass_block_t(const MassArgs& a, int key_tiles, const La
     const int64_t wgs = (int64_t)a.cache.n_kv_heads * a.parts * ((a.kv_len + keys - 1) / keys);
     if (wgs > INT32_MAX) return hipErrorInvalidValue;
     const dim3 grid = wide_grid(wgs), block(kMassWaves * 64);
-    return key_tiles == 2 ? launch_kernel(mass_block_kernel<D, E4M3, 2, kRowTiles>, grid, block, l, a) : launch_kernel(mass_block_kernel<D, E4M3, 1, kRowTiles>, grid, block, l, a);
+    return key_tiles == 2 ? launch_kernel(mass_block_kernel<D, E4M3, 2>, grid, block, l, a) : launch_kernel(mass_block_kernel<D, E4M3, 1>, grid, block, l, a);
 }
 
 hipError_t launch_mass_block(int head_dim, const MassArgs& a, int key_tiles, const Launch& l) {
