@@ -8,12 +8,16 @@
 // p, the sums and the mass are fp32.  A row whose lse is not finite (it has no keys, or a NaN among its scores) adds nothing.
 //
 // One row of every sequence: a wave loads 64 keys, whose 16-byte chunks are operand B as they lie (the order of the dims in
-// the sum is free), and the group's query heads are the 16 rows of operand A, so nothing passes through LDS.  K bounds it: 137
-// us for 64 sequences of 4000 .. 8192 keys of 8 kv heads of 128 (6.0 TB/s).
+// the sum is free), and the group's query heads are the 16 rows of operand A, so nothing passes through LDS.  K bounds it: 64
+// sequences of 4000 .. 8192 keys of 8 kv heads of 128 take 137-139 us beside other launches (6.0 TB/s) and 133 alone; of the
+// E4M3 cache 87 (half the bytes, 5.0 TB/s).
 // A block of query rows: a wave keeps 32 or 64 keys as operand B and the rows stream through LDS for the work-group's four
 // waves, 32 at a time; rows are shared out over several work-groups where the keys alone do not fill the GPU, and their
-// sums meet in a second launch, in a fixed order.  Exponentials beside the products bound it: 22 us for 2048 causal rows of 32
-// heads of 128 over 8 kv heads (785 TFLOP/s), 5.7 for the last 64 rows behind 8192 keys.
+// sums meet in a second launch, in a fixed order.  Exponentials beside the products bound it, while other launches fill what a
+// wave's chain leaves: 22.0-22.6 us for 2048 causal rows of 32 heads of 128 over 8 kv heads (760-780 TFLOP/s), 5.7 for the last
+// 64 rows behind 8192 keys.  Alone, as one engine's calls follow each other, the chain and the shares' uneven lengths bound it:
+// 32.5 and 5.1 for the sum (460 TFLOP/s), and 13.9.  The E4M3 cache, whose
+// keys are converted once, takes as long: on one stream 33.8 us for 33.2, and 13.5 for 13.3.
 #include "decode_common.h"
 #include "kv8_device.h"
 
@@ -355,8 +359,9 @@ MassPlan plan_mass_block(int group, int n_kv_heads, int q_len, int kv_len, int n
     MassPlan p;
     p.key_tiles = kv_len > 128 ? 2 : 1;
     const int64_t keys = 32 * p.key_tiles * kMassWaves, of_keys = n_kv_heads * ((kv_len + keys - 1) / keys);
-    // (a few stages on every CU are sooner done than shared out and summed by a second launch: 64 rows of 4 heads after 8128
-    // keys, 8 stages, 5.5 us against 7.1)
+    // A few stages on every CU are sooner done than shared out and summed by a second launch.  One launch against two, 64 rows of
+    // 4 heads (8 stages) of 8 kv heads at the end of 8192 keys: 5.8 us against 7.1 beside other launches, 13.3 / 13.5 on one
+    // stream.  (Below the border, 7168 keys, 5.7 / 6.7 and 13.3 / 13.5, 4200 keys 4.9 / 6.5 and 12.7 / 12.9: it could be lower.)
     if (of_keys >= n_cu && tiles <= 16)
         p.parts = 1;
     else  // (a prompt of 2048 rows and 32 heads: 3 work-groups a CU, which all are on it at once, 21.9 us; 4 of them 22.9)
